@@ -249,6 +249,105 @@ TATARA_API int32_t tatara_op_quantise_ft_noalloc(const float* w, uint64_t rows, 
                                                  uint64_t out_capacity, uint64_t* out_bytes);
 
 /* ------------------------------------------------------------------------ */
+/* Learned bucket choice and orthogonalised updates                          */
+/* ------------------------------------------------------------------------ */
+
+/* No counterparts in the reference, whose buckets follow fixed rules and whose
+ * optimizers are element-wise: layer norm, a gate that chooses a LayerStack's
+ * buckets by learned scores, and Muon updates of its matrices.
+ *
+ * These calls queue their work on `stream` (NULL: the device's null stream) and
+ * return; nothing is allocated and nothing waits, so they can be captured.  The
+ * stream must be of the thread's current device.  Tensors are device memory;
+ * `dtype` is the element type of the tensors that are void*, strides count
+ * elements from one row (or matrix) to the next and rows may start at any
+ * element.  Inputs and outputs must not overlap unless stated.  `workspace` has
+ * at least the bytes that the call's *_workspace function gives, aligned to 16
+ * bytes, and is used by one call at a time (calls on one stream may share it);
+ * its contents need not be kept or cleared.  Results do not depend on the run:
+ * every sum has a fixed order. */
+#define TATARA_F32 0
+#define TATARA_F16 1
+#define TATARA_BF16 2
+
+/* Layer norm of rows of 1..32768 columns:
+ *   y = (x - mean) * rstd * weight + bias,
+ *   mean = sum(x) / cols,  rstd = 1 / sqrt(sum((x - mean)^2) / cols + eps).
+ * weight and bias are f32 and may be NULL (1 and 0); mean and rstd, f32 per row,
+ * are what the backward pass reads and may be NULL. */
+TATARA_API int32_t tatara_op_layer_norm_forward(const void* x, int64_t x_stride, const float* weight,
+                                                const float* bias, void* y, int64_t y_stride, float* mean,
+                                                float* rstd, uint64_t rows, uint32_t cols, float eps, int32_t dtype,
+                                                TataraStream* stream);
+/* With h = (x - mean) * rstd and g = dy * weight:
+ *   dx = rstd * (g - sum(g) / cols - h * sum(g * h) / cols),
+ *   dweight = sum over rows of dy * h,  dbias = sum over rows of dy
+ * (f32, overwritten; either may be NULL, and with both NULL no workspace is
+ * needed).  No rows: both become 0. */
+TATARA_API int32_t tatara_op_layer_norm_backward_workspace(uint32_t cols, uint64_t* bytes);
+TATARA_API int32_t tatara_op_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                                 const float* weight, const float* mean, const float* rstd, void* dx,
+                                                 int64_t dx_stride, float* dweight, float* dbias, uint64_t rows,
+                                                 uint32_t cols, int32_t dtype, void* workspace,
+                                                 uint64_t workspace_bytes, TataraStream* stream);
+
+/* The choice of top_k of 1..1024 buckets for each position (top_k 1..16) from
+ * logits [positions][buckets]:
+ *   p = softmax(logits),  bucket = the top_k largest logits (equal ones: lowest
+ *   bucket first; NaN above every number),  gate = p at bucket, divided by
+ *   its sum over the position's choices with renormalise != 0,
+ *   count[e] = how often e was chosen,  prob_sum[e] = sum of p[e],
+ *   counted = number of positions that count,
+ *   loss = balance * buckets / (top_k * counted^2) * sum_e count[e] * prob_sum[e].
+ * A logit of -infinity masks a bucket for the position: bucket -1 and gate 0
+ * stand where fewer than top_k are left.  A position with valid[t] == 0 (valid
+ * may be NULL) or with every bucket masked does not count and chooses nothing.
+ * bucket and gate are [positions][top_k]; counted and loss one value each; all
+ * outputs are overwritten. */
+TATARA_API int32_t tatara_op_bucket_gate_workspace(uint32_t buckets, uint64_t* bytes);
+TATARA_API int32_t tatara_op_bucket_gate_forward(const void* logits, int64_t stride, const uint8_t* valid,
+                                                 uint64_t positions, uint32_t buckets, uint32_t top_k,
+                                                 int32_t renormalise, float balance, int32_t dtype, int32_t* bucket,
+                                                 float* gate, int32_t* count, float* prob_sum, int32_t* counted,
+                                                 float* loss, void* workspace, uint64_t workspace_bytes,
+                                                 TataraStream* stream);
+/* Gradient of the logits from the gates' (dgate, may be NULL) and the loss's:
+ * with h = dloss * balance * buckets / (top_k * counted^2) * count, plus the
+ * gates' gradient at the chosen buckets,  dlogits = p * (h - sum(p * h)).
+ * bucket, count and counted are the forward call's; the counts, a step function
+ * of the logits, have no gradient.  A position that does not count gets 0. */
+TATARA_API int32_t tatara_op_bucket_gate_backward(const void* logits, int64_t stride, const uint8_t* valid,
+                                                  uint64_t positions, uint32_t buckets, uint32_t top_k,
+                                                  int32_t renormalise, float balance, int32_t dtype,
+                                                  const int32_t* bucket, const int32_t* count,
+                                                  const int32_t* counted, const float* dgate, float dloss,
+                                                  void* dlogits, int64_t dlogits_stride, TataraStream* stream);
+
+/* Newton-Schulz orthogonalisation of `batch` matrices of rows x cols (sides up
+ * to 32768): X = in / (|in|_F + 1e-7), then `steps` (1..32, usually 5) times
+ *   A = X X^T,  X = 3.4445 X + (-4.7750 A + 2.0315 A^2) X
+ * on the matrix's shorter side.  Every singular value that is not tiny beside
+ * the largest ends between about 0.7 and 1.2.  A matrix of zeros stays zero; one
+ * with a NaN or an infinity becomes NaN.  out may be in. */
+TATARA_API int32_t tatara_op_orthogonalise_workspace(uint32_t batch, uint32_t rows, uint32_t cols, int32_t dtype,
+                                                     uint64_t* bytes);
+TATARA_API int32_t tatara_op_orthogonalise(const void* in, int64_t in_row_stride, int64_t in_batch_stride, void* out,
+                                           int64_t out_row_stride, int64_t out_batch_stride, uint32_t batch,
+                                           uint32_t rows, uint32_t cols, int32_t dtype, uint32_t steps,
+                                           void* workspace, uint64_t workspace_bytes, TataraStream* stream);
+/* Muon update of `batch` matrices (a per-bucket weight group, the king blocks
+ * of the FT table), weights and momentum f32 and contiguous, grad of grad_dtype:
+ *   momentum = beta * momentum + (1 - beta) * grad,
+ *   u = nesterov ? (1 - beta) * grad + beta * momentum : momentum,
+ *   weights = clamp(weights * (1 - lr * decay) - lr * scale * orthogonalise(u), min_w, max_w).
+ * The workspace is tatara_op_orthogonalise_workspace's for TATARA_F32. */
+TATARA_API int32_t tatara_op_muon_step(float* weights, float* momentum, const void* grad, uint32_t batch,
+                                       uint32_t rows, uint32_t cols, int32_t grad_dtype, double beta,
+                                       int32_t nesterov, float lr, float decay, float scale, float min_w, float max_w,
+                                       uint32_t steps, void* workspace, uint64_t workspace_bytes,
+                                       TataraStream* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Dataloader: PSV records -> batch (Batch::push_decoded + BucketMode)       */
 /* ------------------------------------------------------------------------ */
 

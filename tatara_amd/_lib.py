@@ -270,6 +270,39 @@ SIGNATURES = {
         C.c_int32,
         [C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_double, C.c_int32, C.c_void_p, C.c_uint64, c_u64p],
     ),
+    "tatara_op_layer_norm_forward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_uint64,
+         C.c_uint32, C.c_float, C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_layer_norm_backward_workspace": (C.c_int32, [C.c_uint32, c_u64p]),
+    "tatara_op_layer_norm_backward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64] + [C.c_void_p] * 4
+        + [C.c_int64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p],
+    ),
+    "tatara_op_bucket_gate_workspace": (C.c_int32, [C.c_uint32, c_u64p]),
+    "tatara_op_bucket_gate_forward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int32, C.c_float, C.c_int32]
+        + [C.c_void_p] * 7 + [C.c_uint64, C.c_void_p],
+    ),
+    "tatara_op_bucket_gate_backward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int32, C.c_float, C.c_int32]
+        + [C.c_void_p] * 4 + [C.c_float, C.c_void_p, C.c_int64, C.c_void_p],
+    ),
+    "tatara_op_orthogonalise_workspace": (C.c_int32, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32, c_u64p]),
+    "tatara_op_orthogonalise": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_uint32, C.c_uint32, C.c_uint32,
+         C.c_int32, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p],
+    ),
+    "tatara_op_muon_step": (
+        C.c_int32,
+        [C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32, C.c_double, C.c_int32]
+        + [C.c_float] * 5 + [C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p],
+    ),
     "tatara_feature_set_info": (C.c_int32, [C.c_int32, c_i32p, c_i32p, c_i32p, c_i32p, C.POINTER(C.c_uint32)]),
     "tatara_psv_to_batch": (
         C.c_int32,

@@ -18,16 +18,8 @@
 
 #include "../../include/tatara_hip.h"
 #include "common.hpp"
-
-struct TataraStream {
-    hipStream_t s;
-    int device;
-};
-
-struct TataraEvent {
-    hipEvent_t e;
-    int device;
-};
+#include "elem.hpp"
+#include "streams.hpp"
 
 struct TataraModule {
     hipModule_t m;
@@ -39,8 +31,6 @@ struct TataraModule {
 namespace tatara {
 namespace {
 
-inline hipStream_t raw(TataraStream* s) { return s ? s->s : nullptr; }
-
 // A code object as hipcc --genco writes it: an ELF image, or a clang offload
 // bundle holding one.  Anything else is refused before the loader sees it.
 bool looks_like_code_object(const void* image, uint64_t bytes) {
@@ -51,6 +41,15 @@ bool looks_like_code_object(const void* image, uint64_t bytes) {
 }
 
 }  // namespace
+
+int32_t check_stream(TataraStream* stream) {
+    if (!stream) return kOk;
+    int device = 0;
+    TATARA_HIP(hipGetDevice(&device), "hipGetDevice");
+    TATARA_REQUIRE(stream->device == device, "the stream is not of the thread's current device");
+    return kOk;
+}
+
 }  // namespace tatara
 
 using namespace tatara;

@@ -1,0 +1,276 @@
+"""Operators for a learned bucket choice and for orthogonalised updates.
+
+A LayerStack's bucket follows a fixed rule and its optimizers work element by
+element, as in the reference, which has no counterpart of these operators: layer
+norm (`LayerNorm`), a gate that chooses buckets by learned scores and keeps them
+balanced (`BucketGate`), and Newton-Schulz orthogonalised updates of weight
+matrices (`Orthogonaliser`, `Muon`), over the C ABI (tatara_op_layer_norm_*,
+tatara_op_bucket_gate_*, tatara_op_orthogonalise, tatara_op_muon_step).
+
+An operator is made once for a layer's shape and holds its workspace.  Tensors
+are device memory: a `DeviceArray`, or any object with data_ptr(), shape,
+stride(), dtype and element_size() (a torch tensor on the GPU).  The last
+dimension is contiguous; rows may lie inside wider ones.  An operator's element
+type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16.  Calls queue
+their work on `stream` (a runtime.Stream; None is the null stream) and return;
+one operator's calls belong on one stream at a time, since they share the
+workspace.  Wrong shapes and types raise ValueError, device errors TataraError.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _lib
+from ._lib import check
+
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+# an operator's element type -> names of the array types that hold it
+_HELD = {
+    "f32": ("float32", "torch.float32"),
+    "f16": ("float16", "torch.float16"),
+    "bf16": ("torch.bfloat16", "uint16"),
+    "i32": ("int32", "torch.int32"),
+    "u8": ("uint8", "torch.uint8"),
+}
+
+
+class _Workspace:
+    """Device memory that an operator keeps for its calls."""
+
+    def __init__(self, nbytes: int):
+        p = C.c_void_p()
+        check(_lib.load().tatara_malloc(C.byref(p), nbytes))
+        self.ptr, self.nbytes = p.value, nbytes
+
+    def __del__(self):
+        try:
+            if self.ptr:
+                _lib.load().tatara_free(self.ptr)  # waits for the device's work
+                self.ptr = None
+        except Exception:
+            pass
+
+
+def _dtype(dtype: str) -> int:
+    if dtype not in DTYPES:
+        raise ValueError(f"dtype must be one of {', '.join(DTYPES)}, not {dtype!r}")
+    return DTYPES[dtype]
+
+
+_HELD_TYPES: dict = {}  # array type -> the element types it can hold
+
+
+def _is(array_dtype, dtype: str) -> bool:
+    held = _HELD_TYPES.get(array_dtype)
+    if held is None:
+        name = str(array_dtype)
+        held = _HELD_TYPES[array_dtype] = frozenset(k for k, v in _HELD.items() if name in v)
+    return dtype in held
+
+
+def _wrong(name: str, x, shape, dtype: str):
+    raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on the device with a contiguous last "
+                     f"dimension, not {getattr(x, 'dtype', type(x).__name__)} {tuple(getattr(x, 'shape', ()))}")
+
+
+def _dense(name: str, x, shape: tuple, dtype: str):
+    """The address of a contiguous tensor of this shape."""
+    if x is None or tuple(x.shape) != shape or not _is(x.dtype, dtype):
+        _wrong(name, x, shape, dtype)
+    if hasattr(x, "data_ptr"):
+        if not x.is_cuda or not x.is_contiguous():
+            _wrong(name, x, shape, dtype)
+        return x.data_ptr()
+    return x.ptr
+
+
+def _rows(name: str, x, shape: tuple, dtype: str):
+    """Address and row stride of a [rows, cols] tensor."""
+    if x is None or tuple(x.shape) != shape or not _is(x.dtype, dtype):
+        _wrong(name, x, shape, dtype)
+    if hasattr(x, "data_ptr"):
+        stride = x.stride()
+        if not x.is_cuda or (stride[1] != 1 and shape[1] > 1):
+            _wrong(name, x, shape, dtype)
+        # a single row's stride says nothing
+        return x.data_ptr(), stride[0] if shape[0] > 1 else shape[1]
+    return x.ptr, shape[1]
+
+
+def _matrices(name: str, x, shape: tuple, dtype: str):
+    """Address, row stride and matrix stride of a [batch, rows, cols] tensor."""
+    if x is None or tuple(x.shape) != shape or not _is(x.dtype, dtype):
+        _wrong(name, x, shape, dtype)
+    if hasattr(x, "data_ptr"):
+        stride = x.stride()
+        if not x.is_cuda or (stride[2] != 1 and shape[2] > 1):
+            _wrong(name, x, shape, dtype)
+        return x.data_ptr(), stride[1] if shape[1] > 1 else shape[2], stride[0]
+    return x.ptr, shape[2], shape[1] * shape[2]
+
+
+def _handle(stream):
+    return None if stream is None else stream.handle
+
+
+class LayerNorm:
+    """y = (x - mean) * rstd * weight + bias over rows of `cols` values.
+
+    x, y, dy and dx are [rows, cols] of `dtype`; weight, bias, mean, rstd and the
+    weight's and bias's gradients are f32.  weight and bias may be None."""
+
+    def __init__(self, cols: int, dtype: str = "f32", eps: float = 1e-5):
+        self.cols, self.dtype, self.eps = int(cols), dtype, float(eps)
+        self._code = _dtype(dtype)
+        if not 1 <= self.cols <= 32768:
+            raise ValueError(f"cols must be 1 to 32768, not {cols}")
+        if not self.eps >= 0.0:
+            raise ValueError(f"eps must not be negative, not {eps}")
+        self._lib = _lib.load()
+        self._ws = None
+
+    def _param(self, name, x):
+        return None if x is None else _dense(name, x, (self.cols,), "f32")
+
+    def forward(self, x, weight, bias, y, mean=None, rstd=None, stream=None) -> None:
+        """Writes y, and mean and rstd [rows] for the backward pass if given."""
+        rows = x.shape[0]
+        shape = (rows, self.cols)
+        xp, xs = _rows("x", x, shape, self.dtype)
+        yp, ys = _rows("y", y, shape, self.dtype)
+        check(self._lib.tatara_op_layer_norm_forward(
+            xp, xs, self._param("weight", weight), self._param("bias", bias), yp, ys,
+            None if mean is None else _dense("mean", mean, (rows,), "f32"),
+            None if rstd is None else _dense("rstd", rstd, (rows,), "f32"),
+            rows, self.cols, self.eps, self._code, _handle(stream)))
+
+    def backward(self, dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, stream=None) -> None:
+        """Writes dx, and the weight's and bias's gradients [cols] if given (overwritten)."""
+        rows = x.shape[0]
+        shape = (rows, self.cols)
+        if self._ws is None:
+            n = C.c_uint64()
+            check(self._lib.tatara_op_layer_norm_backward_workspace(self.cols, C.byref(n)))
+            self._ws = _Workspace(n.value)
+        dyp, dys = _rows("dy", dy, shape, self.dtype)
+        xp, xs = _rows("x", x, shape, self.dtype)
+        dxp, dxs = _rows("dx", dx, shape, self.dtype)
+        check(self._lib.tatara_op_layer_norm_backward(
+            dyp, dys, xp, xs, self._param("weight", weight), _dense("mean", mean, (rows,), "f32"),
+            _dense("rstd", rstd, (rows,), "f32"), dxp, dxs, self._param("dweight", dweight),
+            self._param("dbias", dbias), rows, self.cols, self._code, self._ws.ptr, self._ws.nbytes,
+            _handle(stream)))
+
+
+class BucketGate:
+    """The best top_k of `buckets` for each position by its logits, with the loss
+    that keeps them balanced: balance * buckets / (top_k * counted^2) *
+    sum_e count[e] * prob_sum[e], which is `balance` when all are taken alike.
+
+    Logits are [positions, buckets] of `dtype`; a logit of -infinity masks the
+    bucket for the position, and valid [positions] (uint8) of 0 leaves the position out."""
+
+    def __init__(self, buckets: int, top_k: int = 1, dtype: str = "f32", renormalise: bool = False,
+                 balance: float = 0.01):
+        self.buckets, self.top_k, self.dtype = int(buckets), int(top_k), dtype
+        self.renormalise, self.balance = int(bool(renormalise)), float(balance)
+        self._code = _dtype(dtype)
+        if not 1 <= self.buckets <= 1024:
+            raise ValueError(f"buckets must be 1 to 1024, not {buckets}")
+        if not 1 <= self.top_k <= min(16, self.buckets):
+            raise ValueError(f"top_k must be 1 to 16 and no more than buckets, not {top_k}")
+        self._lib = _lib.load()
+        self._ws = None
+
+    def forward(self, logits, bucket, gate, count, prob_sum, counted, loss, valid=None, stream=None) -> None:
+        """Writes bucket (int32) and gate (f32) [positions, top_k], count (int32)
+        and prob_sum (f32) [buckets], counted (int32) and loss (f32) [1]."""
+        n = logits.shape[0]
+        if self._ws is None:
+            b = C.c_uint64()
+            check(self._lib.tatara_op_bucket_gate_workspace(self.buckets, C.byref(b)))
+            self._ws = _Workspace(b.value)
+        lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype)
+        chosen = (n, self.top_k)
+        check(self._lib.tatara_op_bucket_gate_forward(
+            lp, ls, None if valid is None else _dense("valid", valid, (n,), "u8"), n, self.buckets, self.top_k,
+            self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32"),
+            _dense("gate", gate, chosen, "f32"), _dense("count", count, (self.buckets,), "i32"),
+            _dense("prob_sum", prob_sum, (self.buckets,), "f32"), _dense("counted", counted, (1,), "i32"),
+            _dense("loss", loss, (1,), "f32"), self._ws.ptr, self._ws.nbytes, _handle(stream)))
+
+    def backward(self, logits, bucket, count, counted, dlogits, dgate=None, dloss: float = 1.0, valid=None,
+                 stream=None) -> None:
+        """Writes dlogits from dgate (f32 [positions, top_k], None: no gradient) and
+        dloss; bucket, count and counted are the forward call's."""
+        n = logits.shape[0]
+        lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype)
+        dp, ds = _rows("dlogits", dlogits, (n, self.buckets), self.dtype)
+        chosen = (n, self.top_k)
+        check(self._lib.tatara_op_bucket_gate_backward(
+            lp, ls, None if valid is None else _dense("valid", valid, (n,), "u8"), n, self.buckets, self.top_k,
+            self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32"),
+            _dense("count", count, (self.buckets,), "i32"), _dense("counted", counted, (1,), "i32"),
+            None if dgate is None else _dense("dgate", dgate, chosen, "f32"), dloss, dp, ds, _handle(stream)))
+
+
+class Orthogonaliser:
+    """Newton-Schulz orthogonalisation of `batch` matrices [rows, cols]: called
+    with input and output [batch, rows, cols] of `dtype` (out may be the input)."""
+
+    def __init__(self, batch: int, rows: int, cols: int, dtype: str = "f32", steps: int = 5):
+        self.batch, self.rows, self.cols = int(batch), int(rows), int(cols)
+        self.shape, self.dtype, self.steps = (self.batch, self.rows, self.cols), dtype, int(steps)
+        self._code = _dtype(dtype)
+        if self.batch < 1:
+            raise ValueError(f"batch must be at least 1, not {batch}")
+        if not 1 <= self.steps <= 32:
+            raise ValueError(f"steps must be 1 to 32, not {steps}")
+        if not (1 <= self.rows <= 32768 and 1 <= self.cols <= 32768):
+            raise ValueError(f"a matrix has sides of 1 to 32768, not {rows} x {cols}")
+        self._lib = _lib.load()
+        n = C.c_uint64()
+        check(self._lib.tatara_op_orthogonalise_workspace(self.batch, self.rows, self.cols, self._code, C.byref(n)))
+        self._bytes, self._ws = n.value, None
+
+    def _workspace(self) -> int:
+        if self._ws is None:
+            self._ws = _Workspace(self._bytes)
+        return self._ws.ptr
+
+    def __call__(self, x, out, stream=None) -> None:
+        xp, xr, xb = _matrices("x", x, self.shape, self.dtype)
+        op, orow, ob = _matrices("out", out, self.shape, self.dtype)
+        check(self._lib.tatara_op_orthogonalise(xp, xr, xb, op, orow, ob, self.batch, self.rows, self.cols,
+                                                self._code, self.steps, self._workspace(), self._bytes,
+                                                _handle(stream)))
+
+
+class Muon:
+    """Muon updates of `batch` weight matrices [rows, cols]: momentum of the
+    gradient, orthogonalised, subtracted from the weights.
+
+    weights and momentum are f32 [batch, rows, cols], updated in place; the
+    gradient is of `grad_dtype`.  step's scale multiplies lr in the update
+    (sqrt(max(1, rows / cols)) keeps an update's size alike over shapes);
+    weights are clamped to [min_w, max_w]."""
+
+    def __init__(self, batch: int, rows: int, cols: int, beta: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, grad_dtype: str = "f32", steps: int = 5, min_w: float = -1e30,
+                 max_w: float = 1e30):
+        if not 0.0 <= beta < 1.0:
+            raise ValueError(f"beta must be in [0, 1), not {beta}")
+        if not min_w <= max_w:
+            raise ValueError(f"min_w {min_w} exceeds max_w {max_w}")
+        self.grad_dtype, self._grad_code = grad_dtype, _dtype(grad_dtype)
+        self._ortho = Orthogonaliser(batch, rows, cols, "f32", steps)
+        self.shape, self.beta, self.nesterov = self._ortho.shape, float(beta), int(bool(nesterov))
+        self.weight_decay, self.min_w, self.max_w = float(weight_decay), float(min_w), float(max_w)
+
+    def step(self, weights, momentum, grad, lr: float, scale: float = 1.0, stream=None) -> None:
+        o, shape = self._ortho, self.shape
+        check(o._lib.tatara_op_muon_step(
+            _dense("weights", weights, shape, "f32"), _dense("momentum", momentum, shape, "f32"),
+            _dense("grad", grad, shape, self.grad_dtype), o.batch, o.rows, o.cols, self._grad_code, self.beta,
+            self.nesterov, lr, self.weight_decay, scale, self.min_w, self.max_w, o.steps, o._workspace(), o._bytes,
+            _handle(stream)))

@@ -1,6 +1,6 @@
 // Orthogonalised updates (Muon): a batch of matrices U of one shape becomes
 //
-//   X_0 = U / (|U|_F + 1e-7),  A = X X^T,  B = b A + c A^2,  X <- a X + B X,
+//   X_0 = U / (|U|_F + 1e-7),  A = X X^T,  B = a I + b A + c A^2,  X <- B X,
 //
 // X standing with its shorter side first, for a number of steps.  With (a, b,
 // c) = (3.4445, -4.7750, 2.0315) every singular value of X_0 in (0, 1] is taken
@@ -12,7 +12,7 @@
 // The products run on the f16 matrix cores with f32 sums.  A value v of X, A or
 // B is held as two f16 numbers of 2^14 v, hi = f16(2^14 v) and lo = f16(2^14 v
 // - hi): 22 bits, and |v| < 4 cannot overflow (|X| <= 1.21, |A| <= 1.46, |B| <=
-// 2.9 by the map above).  A product takes hi hi + hi lo + lo hi, three f16
+// 3.45 by the map above).  A product takes hi hi + hi lo + lo hi, three f16
 // products at 16 times the f32 matrix rate each, and leaves out lo lo, 2^-22 of
 // the result.  Errors against 64-bit steps are those of f32 products (1e-6 to
 // 1e-5 of |X|, from the sums' rounding).
@@ -34,11 +34,15 @@ using half8 = f16_t __attribute__((ext_vector_type(8)));
 using half4 = f16_t __attribute__((ext_vector_type(4)));
 using floatx16 = float __attribute__((ext_vector_type(16)));
 
-// A matrix held as two f16 planes.
-struct Held {
-    f16_t* hi;
-    f16_t* lo;
-};
+// Where a held matrix has the hi of (row, col); lo lies kLow further.  Two rows'
+// 32 columns of hi fill a 128-byte line, the next line has their lo: a stage's
+// loads take whole lines, also where they take hi alone.  Loads of half lines ran
+// at 22 to 27 bytes a clock and CU, of whole ones at 35.
+using Held = f16_t*;
+constexpr uint32_t kLow = 64;
+__device__ __forceinline__ uint64_t held_at(uint64_t row, uint32_t col, uint32_t cols) {
+    return ((row / 2) * (cols / 32) + col / 32) * 128 + row % 2 * 32 + col % 32;
+}
 
 __device__ __forceinline__ void split(float v, f16_t& hi, f16_t& lo) {
     const float s = v * kHeld;
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(256) void muon_split_kernel(Source s, const double*
     for (uint32_t i = 0; i < n_parts; ++i) sum += parts[(uint64_t)b * kNormParts + i];
     const double inv = 1.0 / (sqrt(sum) + kNormEps);
     const T* g = static_cast<const T*>(s.grad) + (int64_t)b * s.batch_stride;
-    const uint64_t n = (uint64_t)s.rows * s.cols, plane = (uint64_t)b * rows_up * cols_up;
+    const uint64_t n = (uint64_t)s.rows * s.cols, first = 2ull * b * rows_up * cols_up;
     const uint32_t c = threadIdx.x % 64, q = threadIdx.x / 64;
     for (uint32_t r = q; r < 64; r += 4) {
         float v = 0.0f;
@@ -110,13 +114,245 @@ __global__ __launch_bounds__(256) void muon_split_kernel(Source s, const double*
             v = (float)((double)source_value<T>(s, b * n + (uint64_t)(r0 + r) * s.cols + c0 + c, gv) * inv);
         }
         tile[r][c] = v;
-        const uint64_t at = plane + (uint64_t)(r0 + r) * cols_up + c0 + c;
-        split(v, straight.hi[at], straight.lo[at]);
+        f16_t* to = straight + first + held_at(r0 + r, c0 + c, cols_up);
+        split(v, to[0], to[kLow]);
     }
     __syncthreads();
     for (uint32_t r = q; r < 64; r += 4) {
-        const uint64_t at = plane + (uint64_t)(c0 + r) * rows_up + r0 + c;
-        split(tile[c][r], turned.hi[at], turned.lo[at]);
+        f16_t* to = turned + first + held_at(c0 + r, r0 + c, rows_up);
+        split(tile[c][r], to[0], to[kLow]);
+    }
+}
+
+// Where X goes after the last step: to `out`, or into the weights.
+struct Target {
+    void* out;
+    int64_t row_stride, batch_stride;
+    float* weights;
+    float keep, rate, min_w, max_w;  // w = clamp(keep w - rate X)
+};
+
+__device__ __forceinline__ float updated(const Target& t, float w, float x) {
+    const float u = fmaf(-t.rate, x, t.keep * w);
+    return u < t.min_w ? t.min_w : (u > t.max_w ? t.max_w : u);
+}
+
+using floatx4 = float __attribute__((ext_vector_type(4)));
+
+struct Halves {
+    half4 hi, lo;
+};
+
+__device__ __forceinline__ Halves split4(const floatx4& v) {
+    Halves h;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        f16_t a, b;
+        split(v[r], a, b);
+        h.hi[r] = a;
+        h.lo[r] = b;
+    }
+    return h;
+}
+
+__device__ __forceinline__ floatx4 product16(const Halves& a, const Halves& b, floatx4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.lo, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.lo, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.hi, c, 0, 0, 0);
+}
+
+// All steps of a matrix of a few rows in one workgroup: X stays in registers, in
+// blocks of 16 x 16, MB rows of blocks and NT columns of them a wave.  An MFMA
+// result's lane holds four rows of a column, which is also how 16x16x16 takes its
+// right operand, so B X needs no rearrangement; X X^T takes blocks that were
+// turned through LDS.  Each wave sums X X^T over its columns, the workgroup adds
+// the waves' sums in order.
+template <int MB, int NT, typename T>
+__global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, uint32_t steps) {
+    constexpr int NB = MB * (MB + 1) / 2, CHUNK = NB < 4 ? NB : 4, PITCH = MB * 16 + 4;
+    __shared__ __align__(16) float gram[MB * 16][PITCH];
+    __shared__ __align__(16) f16_t poly_hi[MB * 16][PITCH], poly_lo[MB * 16][PITCH];
+    __shared__ floatx4 parts[16][CHUNK][kWave];
+    __shared__ __align__(16) float turned[16][16][20];
+    __shared__ double join[16];
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    const uint32_t col = lane % 16, row4 = lane / 16 * 4;
+    const bool flipped = s.rows > s.cols;
+    const uint32_t m = flipped ? s.cols : s.rows, n = flipped ? s.rows : s.cols, b = blockIdx.x;
+    // element (x, y) of X lies at x * down + y * over of a contiguous matrix
+    const uint32_t down = flipped ? 1 : s.cols, over = flipped ? s.cols : 1;
+    const uint64_t first = (uint64_t)b * s.rows * s.cols;
+    const uint32_t y0 = wave * 16 + col;
+    floatx4 x[MB][NT];
+    double sum = 0.0;
+    {
+        const T* g = static_cast<const T*>(s.grad) + (int64_t)b * s.batch_stride;
+        const int64_t g_down = flipped ? 1 : s.row_stride, g_over = flipped ? s.row_stride : 1;
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            const uint32_t y = tt * waves * 16 + y0;
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t xx = ib * 16 + row4 + r;
+                    const bool in = xx < m && y < n;
+                    const float gv = (float)g[in ? xx * g_down + y * g_over : 0];
+                    x[ib][tt][r] = in ? gv : 0.0f;
+                }
+        }
+    }
+    if (s.momentum) {
+        float* mom = s.momentum + first;
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            const uint32_t y = tt * waves * 16 + y0;
+            float mo[MB][4];
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t xx = ib * 16 + row4 + r;
+                    mo[ib][r] = s.beta * mom[xx < m && y < n ? xx * down + y * over : 0] + s.mix * x[ib][tt][r];
+                }
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t xx = ib * 16 + row4 + r;
+                    const bool in = xx < m && y < n;
+                    if (in) mom[xx * down + y * over] = mo[ib][r];
+                    const float u = s.nesterov ? s.mix * x[ib][tt][r] + s.beta * mo[ib][r] : mo[ib][r];
+                    x[ib][tt][r] = in ? u : 0.0f;
+                }
+        }
+    }
+#pragma unroll
+    for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum += (double)x[ib][tt][r] * (double)x[ib][tt][r];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) join[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll 1
+    for (uint32_t w = 0; w < waves; ++w) sum += join[w];
+    const double inv = 1.0 / (sqrt(sum) + kNormEps);
+#pragma unroll
+    for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[ib][tt][r] = (float)((double)x[ib][tt][r] * inv);
+
+#pragma unroll 1
+    for (uint32_t step = 0; step < steps; ++step) {
+        floatx4 acc[NB] = {};
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            Halves rows[MB];
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) turned[wave][row4 + r][col] = x[ib][tt][r];
+                __builtin_amdgcn_wave_barrier();
+                rows[ib] = split4(*reinterpret_cast<const floatx4*>(&turned[wave][col][row4]));
+                __builtin_amdgcn_wave_barrier();
+            }
+            int k = 0;
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                for (int jb = ib; jb < MB; ++jb, ++k) acc[k] = product16(rows[ib], rows[jb], acc[k]);
+            __builtin_amdgcn_sched_barrier(0);  // columns one after the other: their blocks would not fit
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < NB; k0 += CHUNK) {
+#pragma unroll
+            for (int k = 0; k < CHUNK; ++k)
+                if (k0 + k < NB) parts[wave][k][lane] = acc[k0 + k];
+            __syncthreads();
+            const uint32_t have = (NB - k0 < CHUNK ? NB - k0 : CHUNK) * 256;
+            for (uint32_t e = threadIdx.x; e < have; e += blockDim.x) {
+                float v = 0.0f;
+#pragma unroll 1
+                for (uint32_t w = 0; w < waves; ++w) v += reinterpret_cast<const float*>(parts[w])[e];
+                v *= kProduct;
+                uint32_t k = k0 + e / 256, ib = 0;
+                while (k >= MB - ib) k -= MB - ib, ++ib;
+                const uint32_t jb = ib + k, l = e % 256 / 4;
+                const uint32_t i = ib * 16 + l / 16 * 4 + e % 4, j = jb * 16 + l % 16;
+                gram[i][j] = v;
+                if (ib != jb) gram[j][i] = v;
+            }
+            __syncthreads();
+        }
+        for (uint32_t k = wave; k < MB * MB; k += waves) {
+            const uint32_t ib = k / MB, jb = k % MB;
+            floatx4 v = {};
+#pragma unroll
+            for (int kb = 0; kb < MB; ++kb)
+                v = product16(split4(*reinterpret_cast<const floatx4*>(&gram[ib * 16 + col][kb * 16 + row4])),
+                              split4(*reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][kb * 16 + row4])), v);
+            // B is symmetric: four rows of a column stored as four columns of a row
+            const floatx4 old = *reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][ib * 16 + row4]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                v[r] = fmaf(kC, v[r] * kProduct, fmaf(kB, old[r], ib == jb && row4 + r == col ? kA : 0.0f));
+            const Halves h = split4(v);
+            *reinterpret_cast<half4*>(&poly_hi[jb * 16 + col][ib * 16 + row4]) = h.hi;
+            *reinterpret_cast<half4*>(&poly_lo[jb * 16 + col][ib * 16 + row4]) = h.lo;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int tt = 0; tt < NT; ++tt) {
+            Halves cols[MB];
+#pragma unroll
+            for (int kb = 0; kb < MB; ++kb) cols[kb] = split4(x[kb][tt]);
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib) {
+                floatx4 v = {};
+#pragma unroll
+                for (int kb = 0; kb < MB; ++kb) {
+                    Halves h;
+                    h.hi = *reinterpret_cast<const half4*>(&poly_hi[ib * 16 + col][kb * 16 + row4]);
+                    h.lo = *reinterpret_cast<const half4*>(&poly_lo[ib * 16 + col][kb * 16 + row4]);
+                    v = product16(h, cols[kb], v);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[ib][tt][r] = v[r] * kProduct;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    const int64_t o_down = flipped ? 1 : t.row_stride, o_over = flipped ? t.row_stride : 1;
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+        const uint32_t y = tt * waves * 16 + y0;
+        float w[MB][4];
+        if (t.weights) {
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t xx = ib * 16 + row4 + r;
+                    w[ib][r] = t.weights[first + (xx < m && y < n ? xx * down + y * over : 0)];
+                }
+        }
+#pragma unroll
+        for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t xx = ib * 16 + row4 + r;
+                if (xx >= m || y >= n) continue;
+                if (t.weights)
+                    t.weights[first + xx * down + y * over] = updated(t, w[ib][r], x[ib][tt][r]);
+                else
+                    static_cast<T*>(t.out)[(int64_t)b * t.batch_stride + xx * o_down + y * o_over] = (T)x[ib][tt][r];
+            }
     }
 }
 
@@ -126,147 +362,399 @@ enum Epilogue { kGram, kPoly, kApply, kOut, kUpdate };
 struct ProductArgs {
     Held p, q;           // [m][k] and [n][k]: the product is p q^T
     uint32_t m, n, k;    // multiples of kPad
-    Held old;            // kPoly: A; kApply and later: X transposed, before the step
+    uint32_t tiles_m, tiles_n, tiles;  // of one matrix's product
+    Held old;            // kPoly: A; kApply and later with hi alone: X transposed
     Held to, turned;     // results as they lie and (kApply) transposed
     // kOut, kUpdate: the caller's matrices, [rows][cols]; flipped: X is their transpose
-    void* out;
-    int64_t out_row_stride, out_batch_stride;
+    Target target;
     uint32_t rows, cols;
     int32_t flipped;
-    float* weights;
-    float keep, rate, min_w, max_w;  // w = clamp(keep w - rate X)
 };
 
-// 128 x 128 of p q^T: four waves of 64 x 64, 32 values of k a stage.
-template <int EPI, typename T>
-__global__ __launch_bounds__(256) void muon_product_kernel(ProductArgs a) {
-    constexpr uint32_t TILE = 128, KS = 32, CH = KS / 8;  // 16-byte pieces of a row's stage
-    __shared__ half8 lds[2][4][TILE * CH];                // [buffer][p hi, p lo, q hi, q lo][row, piece]
-    const uint32_t b = blockIdx.z;
+// A workgroup's tile BM x BN of p q^T: WR x WC waves, KS values of k a stage, S
+// stages in LDS.  KG groups of such waves share a stage's values of k, and their
+// sums are joined in order.
+template <int BM_, int BN_, int WR_, int WC_, int KS_, int S_, int KG_ = 1>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, KS = KS_, S = S_, KG = KG_;
+    static constexpr int THREADS = KG * WR * WC * (int)kWave;
+    static constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 blocks of a wave
+    // with P of hi and lo: 16-byte pieces of a row's stage, of the stage, and a thread's loads
+    static constexpr int pieces_row(int P) { return KS / 8 * P; }
+    static constexpr int pieces(int P) { return (BM + BN) * pieces_row(P); }
+    static constexpr int loads(int P) { return pieces(P) / THREADS; }
+    static_assert(pieces(1) % THREADS == 0, "every thread loads alike");
+};
+
+// Which piece of a row's stage lies at a place of it: rows that would share LDS
+// banks turn their pieces, so that 16 rows of one piece cover all of them.
+template <int CH>
+__device__ __forceinline__ uint32_t turn(uint32_t row, uint32_t piece) {
+    return piece ^ ((row / (16 / CH)) % CH);
+}
+
+// 16 bytes a lane from global memory to LDS, the wave's 64 in a row from `to`.
+__device__ __forceinline__ void load_to_lds(const f16_t* from, half8* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// Waits until at most N of the wave's loads are on their way and its LDS reads
+// are done, then for the workgroup.
+template <int N>
+__device__ __forceinline__ void arrive() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A wave's strip of 32 rows in LDS, f32: filled from MFMA results, read in rows.
+template <typename L>
+struct Strip {
+    static constexpr int DOWN = L::TM < 2 ? L::TM : 2, OVER = L::TN < 2 ? L::TN : 2;  // blocks of a strip
+    static constexpr int PITCH = (DOWN > OVER ? DOWN : OVER) * 32 + 4;
+    static constexpr int BYTES = (int)sizeof(float) * 32 * PITCH * L::WR * L::WC;
+    float* base;
+    uint32_t lane;
+    __device__ __forceinline__ Strip(void* lds, uint32_t wave, uint32_t lane_)
+        : base(static_cast<float*>(lds) + wave * 32 * PITCH), lane(lane_) {}
+
+    // block t of the strip, its rows along the strip's
+    __device__ __forceinline__ void put_along(const floatx16& v, int t) const {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) base[(r / 4 * 8 + lane / 32 * 4 + r % 4) * PITCH + t * 32 + lane % 32] = v[r];
+    }
+    // block t, transposed
+    __device__ __forceinline__ void put_across(const floatx16& v, int t) const {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float4 q = {v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]};
+            *reinterpret_cast<float4*>(base + lane % 32 * PITCH + t * 32 + g * 8 + lane / 32 * 4) = q;
+        }
+    }
+    // the strip as rows of a held matrix from (row, col) on, of which `left`
+    // columns exist (a multiple of 32: the side is one of 64, a strip starts at one of 32)
+    template <int WIDTH>
+    __device__ __forceinline__ void store(Held to, uint32_t row, uint32_t col, uint32_t cols, int32_t left) const {
+        constexpr int LANES = WIDTH / 8;  // of a row
+        const uint32_t c = lane % LANES * 8;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += (int)kWave / LANES) {
+            const uint32_t r = r0 + lane / LANES;
+            half8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                f16_t h, l;
+                split(base[r * PITCH + c + j], h, l);
+                hi[j] = h;
+                lo[j] = l;
+            }
+            if ((int32_t)c < left) {
+                f16_t* at = to + held_at(row + r, col + c, cols);
+                *reinterpret_cast<half8*>(at) = hi;
+                *reinterpret_cast<half8*>(at + kLow) = lo;
+            }
+        }
+    }
+    // its values one by one, a batch's loads ahead of its stores:
+    // store(row, column, value, load(row, column))
+    template <int WIDTH, typename F, typename G>
+    __device__ __forceinline__ void each(F&& load, G&& store) const {
+        constexpr int ROWS = (int)kWave / WIDTH, BATCH = 8;
+        const uint32_t c = lane % WIDTH;
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += BATCH * ROWS) {
+            float old[BATCH];
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q) old[q] = load(r0 + q * ROWS + lane / WIDTH, c);
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q) {
+                const uint32_t r = r0 + q * ROWS + lane / WIDTH;
+                store(r, c, base[r * PITCH + c], old[q]);
+            }
+        }
+    }
+};
+
+// P = 2: hi hi + hi lo + lo hi;  P = 1: hi hi alone, with a X added in f32 to the
+// last product of the step instead of a I to B.
+template <int EPI, typename T, typename L, int P>
+__global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a) {
+    constexpr int BM = L::BM, BN = L::BN, CH = L::pieces_row(P), TM = L::TM, TN = L::TN;
+    constexpr int S = L::S, LOADS = L::loads(P);
+    constexpr int DOWN = Strip<L>::DOWN, OVER = Strip<L>::OVER, STAGE = L::pieces(P);
+    // the stages ([stage][rows of p, then of q: pieces]), then the groups' sums, then the strips
+    constexpr int STAGES_BYTES = S * STAGE * 16, SUMS_BYTES = (L::KG - 1) * BM * BN * 4;
+    constexpr int BYTES0 = STAGES_BYTES > SUMS_BYTES ? STAGES_BYTES : SUMS_BYTES;
+    constexpr int BYTES = BYTES0 > Strip<L>::BYTES ? BYTES0 : Strip<L>::BYTES;
+    __shared__ half8 lds[BYTES / 16];
+    // neighbouring tiles on one XCD, so that its L2 holds the panels they share
+    const uint32_t bid = xcd_swizzle(blockIdx.x, gridDim.x);
+    const uint32_t b = bid / a.tiles, at = bid % a.tiles;
     uint32_t ti, tj;
-    if (EPI == kGram || EPI == kPoly) {  // the result is symmetric: tiles on and right of the diagonal
-        const uint32_t nt = (a.n + TILE - 1) / TILE;
-        uint32_t left = blockIdx.x;
+    if (EPI == kGram || EPI == kPoly) {
+        // the result is symmetric: tiles that reach the diagonal or lie right of it
         ti = 0;
-        while (left >= nt - ti) left -= nt - ti, ++ti;
-        tj = ti + left;
+        uint32_t left = at;
+        for (;;) {
+            const uint32_t skip = ti * BM / BN, row = a.tiles_n - skip;
+            if (left < row) {
+                tj = skip + left;
+                break;
+            }
+            left -= row;
+            ++ti;
+        }
     } else {
-        const uint32_t nt = (a.n + TILE - 1) / TILE;
-        ti = blockIdx.x / nt;
-        tj = blockIdx.x % nt;
+        ti = at % a.tiles_m;
+        tj = at / a.tiles_m;
     }
-    const uint32_t i0 = ti * TILE, j0 = tj * TILE;
-    const uint64_t p_at = (uint64_t)b * a.m * a.k, q_at = (uint64_t)b * a.n * a.k;
-    const uint32_t tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    const uint32_t wi = wave / 2 * 64, wj = wave % 2 * 64;
-    floatx16 acc[2][2] = {};
-    half8 next[8];
-    auto fetch = [&](uint32_t k0) {
+    const uint32_t i0 = ti * BM, j0 = tj * BN;
+    const uint64_t p_at = 2ull * b * a.m * a.k, q_at = 2ull * b * a.n * a.k;
+    const uint32_t tid = threadIdx.x, lane = tid % kWave, group = tid / kWave / (L::WR * L::WC);
+    const uint32_t wave = tid / kWave % (L::WR * L::WC);
+    const uint32_t wi = wave / L::WC * (TM * 32), wj = wave % L::WC * (TN * 32);
+    floatx16 acc[TM][TN] = {};
+    const f16_t* from[LOADS];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const uint32_t e = (s % 2) * 256 + tid, row = e / CH, piece = e % CH;
-            const bool isq = s >= 4, islo = (s / 2) % 2;
-            // rows past the matrix (its side is a multiple of 64, not of the tile) are not stored
-            const uint32_t r = isq ? min(j0 + row, a.n - 1) : min(i0 + row, a.m - 1);
-            const f16_t* base = isq ? (islo ? a.q.lo : a.q.hi) + q_at : (islo ? a.p.lo : a.p.hi) + p_at;
-            next[s] = *reinterpret_cast<const half8*>(base + (uint64_t)r * a.k + k0 + piece * 8);
-        }
-    };
-    // pieces of rows four apart share banks: the piece's place turns with the row
-    auto place = [](uint32_t row, uint32_t piece) { return row * CH + (piece ^ ((row >> 2) & 3)); };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const uint32_t e = (s % 2) * 256 + tid;
-            lds[buf][s / 2][place(e / CH, e % CH)] = next[s];
-        }
-    };
-    fetch(0);
-    put(0);
-    __syncthreads();
-    int buf = 0;
-    for (uint32_t k0 = 0; k0 < a.k; k0 += KS) {
-        const bool more = k0 + KS < a.k;
-        if (more) fetch(k0 + KS);
-#pragma unroll
-        for (uint32_t kk = 0; kk < KS / 16; ++kk) {
-            half8 fp[2][2], fq[2][2];  // [hi, lo][block of 32]
-#pragma unroll
-            for (int pl = 0; pl < 2; ++pl)
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const uint32_t piece = kk * 2 + lane / 32;
-                    fp[pl][t] = lds[buf][pl][place(wi + t * 32 + lane % 32, piece)];
-                    fq[pl][t] = lds[buf][2 + pl][place(wj + t * 32 + lane % 32, piece)];
-                }
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[1][x], fq[0][y], acc[x][y], 0, 0, 0);
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][x], fq[1][y], acc[x][y], 0, 0, 0);
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[0][x], fq[0][y], acc[x][y], 0, 0, 0);
-                }
-        }
-        if (more) put(buf ^ 1);
-        __syncthreads();
-        buf ^= 1;
+    for (int s = 0; s < LOADS; ++s) {
+        const uint32_t e = s * L::THREADS + tid, row = e / CH, piece = turn<CH>(row, e % CH);
+        // pieces of 32 columns: four of hi, then (P = 2) four of lo
+        const uint32_t col = piece / (4 * P) * 32 + piece % 4 * 8;
+        // rows past the matrix (its side is a multiple of 64, not of the tile) are not stored
+        const uint32_t r = row < BM ? min(i0 + row, a.m - 1) : min(j0 + row - BM, a.n - 1);
+        from[s] = (row < BM ? a.p + p_at : a.q + q_at) + held_at(r, col, a.k) + piece / 4 % P * kLow;
     }
-    // a lane holds, for four groups of rows, four consecutive rows of one column
+    const uint32_t wave0 = __builtin_amdgcn_readfirstlane(tid / kWave) * kWave;
+    auto fetch = [&](uint32_t stage, uint32_t k0) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+        for (int s = 0; s < LOADS; ++s) load_to_lds(from[s] + k0 * 4, &lds[stage * STAGE + s * L::THREADS + wave0]);
+    };
+    const uint32_t stages = a.k / L::KS;
+    for (uint32_t s = 0; s + 1 < S && s < stages; ++s) fetch(s, s * L::KS);
+    uint32_t buf = 0;
+    for (uint32_t it = 0; it < stages; ++it) {
+        // this stage has arrived, and nobody reads the one before it any more
+        if (it + S - 1 <= stages)
+            arrive<(S - 2) * LOADS>();
+        else
+            arrive<0>();
+        if (it + S - 1 < stages) fetch(buf == 0 ? S - 1 : buf - 1, (it + S - 1) * L::KS);
+        // the next 16 values of k are read while these are multiplied
+        constexpr int STEPS = L::KS / 16 / L::KG;
+        half8 fp[2][P][TM], fq[2][P][TN];  // [this, next][hi, lo][block]
+        auto read = [&](int kk) {
+            const uint32_t at = kk * L::KG + group, piece = at / 2 * (4 * P) + at % 2 * 2 + lane / 32;
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
+            for (int lo = 0; lo < P; ++lo) {
+                // in the order of the products below
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const uint32_t i = i0 + wi + x * 32 + g * 8 + (lane / 32) * 4, j = j0 + wj + y * 32 + lane % 32;
-                if (i >= a.m || j >= a.n) continue;
-                float v[4];
-                half4 hi, lo;
-                // the same elements of the transposed matrix, four in a row
-                const uint64_t across = (uint64_t)b * a.m * a.n + (uint64_t)j * a.m + i;
-                if (EPI != kGram) {
-                    hi = *reinterpret_cast<const half4*>(a.old.hi + across);
-                    lo = *reinterpret_cast<const half4*>(a.old.lo + across);
+                for (int x = 0; x < TM; ++x) {
+                    const uint32_t row = wi + x * 32 + lane % 32;
+                    fp[kk % 2][P - 1 - lo][x] = lds[buf * STAGE + row * CH + turn<CH>(row, piece + (P - 1 - lo) * 4)];
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float s = acc[x][y][g * 4 + r] * kProduct;
-                    const float o = EPI == kGram ? 0.0f : ((float)hi[r] + (float)lo[r]) * kUnheld;
-                    v[r] = EPI == kGram ? s : EPI == kPoly ? fmaf(kC, s, kB * o) : fmaf(kA, o, s);
-                }
-                if (EPI == kOut || EPI == kUpdate) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t row = a.flipped ? j : i + r, col = a.flipped ? i + r : j;
-                        if (row >= a.rows || col >= a.cols) continue;
-                        if (EPI == kOut) {
-                            static_cast<T*>(a.out)[(int64_t)b * a.out_batch_stride + (int64_t)row * a.out_row_stride +
-                                                   col] = (T)v[r];
-                        } else {
-                            float* w = a.weights + ((uint64_t)b * a.rows + row) * a.cols + col;
-                            const float u = fmaf(-a.rate, v[r], a.keep * *w);
-                            *w = u < a.min_w ? a.min_w : (u > a.max_w ? a.max_w : u);
-                        }
-                    }
-                    continue;
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    f16_t h, l;
-                    split(v[r], h, l);
-                    hi[r] = h;
-                    lo[r] = l;
-                    const uint64_t at = (uint64_t)b * a.m * a.n + (uint64_t)(i + r) * a.n + j;
-                    a.to.hi[at] = h;
-                    a.to.lo[at] = l;
-                }
-                if (EPI == kApply || ti != tj) {
-                    const Held& t = EPI == kApply ? a.turned : a.to;
-                    *reinterpret_cast<half4*>(t.hi + across) = hi;
-                    *reinterpret_cast<half4*>(t.lo + across) = lo;
+                for (int y = 0; y < TN; ++y) {
+                    const uint32_t row = BM + wj + y * 32 + lane % 32;
+                    fq[kk % 2][lo][y] = lds[buf * STAGE + row * CH + turn<CH>(row, piece + lo * 4)];
                 }
             }
+        };
+        read(0);
+#pragma unroll
+        for (int kk = 0; kk < STEPS; ++kk) {
+            if (kk + 1 < STEPS) read(kk + 1);
+            const int c = kk % 2;
+#pragma unroll
+            for (int pass = P == 2 ? 2 : 0; pass >= 0; --pass)  // lo hi, hi lo, hi hi
+#pragma unroll
+                for (int x = 0; x < TM; ++x)
+#pragma unroll
+                    for (int y = 0; y < TN; ++y)
+                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fp[c][pass == 2][x], fq[c][pass == 1][y],
+                                                                           acc[x][y], 0, 0, 0);
+        }
+        buf = buf + 1 == S ? 0 : buf + 1;
+    }
+    // A lane holds, of each 32 x 32 block, four groups of four consecutive rows of
+    // one column.  Strips of 32 rows (or columns) go through LDS, a region a wave,
+    // so that they are stored in whole rows.
+    arrive<0>();
+    if constexpr (L::KG > 1) {
+        floatx4* sums = reinterpret_cast<floatx4*>(lds);
+        constexpr int WAVES = L::WR * L::WC, QUADS = TM * TN * 4;
+        if (group > 0) {
+#pragma unroll
+            for (int x = 0; x < TM; ++x)
+#pragma unroll
+                for (int y = 0; y < TN; ++y)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        sums[(((group - 1) * WAVES + wave) * QUADS + (x * TN + y) * 4 + q) * kWave + lane] =
+                            floatx4{acc[x][y][q * 4], acc[x][y][q * 4 + 1], acc[x][y][q * 4 + 2], acc[x][y][q * 4 + 3]};
+        }
+        __syncthreads();
+        if (group > 0) return;  // no barrier follows
+#pragma unroll
+        for (int x = 0; x < TM; ++x)
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int o = 0; o < L::KG - 1; ++o) {
+                        const floatx4 v = sums[((o * WAVES + wave) * QUADS + (x * TN + y) * 4 + q) * kWave + lane];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[x][y][q * 4 + r] += v[r];
+                    }
+    }
+    const Strip<L> strip{lds, wave, lane};
+    const uint64_t first = 2ull * b * a.m * a.n;
+#pragma unroll
+    for (int x = 0; x < TM; ++x) {
+        const uint32_t i = i0 + wi + x * 32;
+        if ((EPI == kPoly || (P == 1 && EPI != kGram)) && i < a.m) {
+            // A, which is symmetric, or X transposed: four rows of a column are four columns of a row
+            half4 hi[TN][4], lo[TN][4];
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const uint32_t j = min(j0 + wj + y * 32 + lane % 32, a.n - 1);
+                    const f16_t* o = a.old + first + held_at(j, i + g * 8 + lane / 32 * 4, a.m);
+                    hi[y][g] = *reinterpret_cast<const half4*>(o);
+                    lo[y][g] = *reinterpret_cast<const half4*>(o + kLow);
+                }
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float o = ((float)hi[y][g][r] + (float)lo[y][g][r]) * kUnheld;
+                        const float v = acc[x][y][g * 4 + r] * kProduct;
+                        const bool diagonal =
+                            P == 2 && i + g * 8 + lane / 32 * 4 + r == j0 + wj + y * 32 + lane % 32;
+                        acc[x][y][g * 4 + r] =
+                            EPI == kPoly ? fmaf(kC, v, fmaf(kB, o, diagonal ? kA : 0.0f)) : fmaf(kA, o, v);
+                    }
+        } else {
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[x][y][r] *= kProduct;
+        }
+    }
+    if (EPI == kOut || EPI == kUpdate) {
+        auto read = [&](uint32_t row, uint32_t col) {
+            if (EPI == kOut || row >= a.rows || col >= a.cols) return 0.0f;
+            return a.target.weights[((uint64_t)b * a.rows + row) * a.cols + col];
+        };
+        auto write = [&](uint32_t row, uint32_t col, float v, float w) {
+            if (row >= a.rows || col >= a.cols) return;
+            if (EPI == kOut) {
+                static_cast<T*>(a.target.out)[(int64_t)b * a.target.batch_stride +
+                                              (int64_t)row * a.target.row_stride + col] = (T)v;
+            } else {
+                a.target.weights[((uint64_t)b * a.rows + row) * a.cols + col] = updated(a.target, w, v);
+            }
+        };
+        if (a.flipped) {
+#pragma unroll
+            for (int y = 0; y < TN; ++y)
+#pragma unroll
+                for (int x = 0; x < TM; x += DOWN) {
+                    const uint32_t j = j0 + wj + y * 32, i = i0 + wi + x * 32;
+#pragma unroll
+                    for (int t = 0; t < DOWN; ++t) strip.put_across(acc[x + t][y], t);
+                    strip.template each<DOWN * 32>(
+                        [&](uint32_t r, uint32_t c) { return read(j + r, i + c); },
+                        [&](uint32_t r, uint32_t c, float v, float w) { write(j + r, i + c, v, w); });
+                }
+        } else {
+#pragma unroll
+            for (int x = 0; x < TM; ++x)
+#pragma unroll
+                for (int y = 0; y < TN; y += OVER) {
+                    const uint32_t j = j0 + wj + y * 32, i = i0 + wi + x * 32;
+#pragma unroll
+                    for (int t = 0; t < OVER; ++t) strip.put_along(acc[x][y + t], t);
+                    strip.template each<OVER * 32>(
+                        [&](uint32_t r, uint32_t c) { return read(i + r, j + c); },
+                        [&](uint32_t r, uint32_t c, float v, float w) { write(i + r, j + c, v, w); });
+                }
+        }
+        return;
+    }
+#pragma unroll
+    for (int x = 0; x < TM; ++x)
+#pragma unroll
+        for (int y = 0; y < TN; y += OVER) {
+            const uint32_t i = i0 + wi + x * 32, j = j0 + wj + y * 32;
+#pragma unroll
+            for (int t = 0; t < OVER; ++t) strip.put_along(acc[x][y + t], t);
+            strip.template store<OVER * 32>(a.to + first, i, j, a.n, i < a.m ? a.n - j : 0);
+        }
+    // a symmetric result's other half; a tile on the diagonal has both
+    if (EPI == kApply || j0 >= i0 + BM) {
+#pragma unroll
+        for (int y = 0; y < TN; ++y)
+#pragma unroll
+            for (int x = 0; x < TM; x += DOWN) {
+                const uint32_t i = i0 + wi + x * 32, j = j0 + wj + y * 32;
+#pragma unroll
+                for (int t = 0; t < DOWN; ++t) strip.put_across(acc[x + t][y], t);
+                strip.template store<DOWN * 32>((EPI == kApply ? a.turned : a.to) + first, j, i, a.m,
+                                                j < a.n ? a.m - i : 0);
+            }
+    }
+}
+
+template <int EPI, typename T, typename L, int P>
+void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
+    p.tiles_m = ceil_div(p.m, L::BM);
+    p.tiles_n = ceil_div(p.n, L::BN);
+    p.tiles = p.tiles_m * p.tiles_n;
+    if (EPI == kGram || EPI == kPoly) {
+        p.tiles = 0;
+        for (uint32_t i = 0; i < p.tiles_m; ++i) p.tiles += p.tiles_n - i * L::BM / L::BN;
+    }
+    muon_product_kernel<EPI, T, L, P><<<p.tiles * batch, L::THREADS, 0, stream>>>(p);
+}
+
+struct Step {
+    Held x, xt, next_xt, gram, poly;
+    uint32_t m, n;
+    bool last;
+};
+
+template <typename T, typename L, int P>
+void launch_step(const Step& s, const Source& from, const Target& t, uint32_t batch, hipStream_t stream) {
+    ProductArgs p{};
+    p.p = p.q = s.x;
+    p.m = p.n = s.m;
+    p.k = s.n;
+    p.to = s.gram;
+    launch_product<kGram, T, L, P>(p, batch, stream);
+    p.p = p.q = p.old = s.gram;
+    p.k = s.m;
+    p.to = s.poly;
+    launch_product<kPoly, T, L, P>(p, batch, stream);
+    p.p = s.poly;
+    p.q = p.old = s.xt;
+    p.n = s.n;
+    p.to = s.x;
+    p.turned = s.next_xt;
+    p.target = t;
+    p.rows = from.rows;
+    p.cols = from.cols;
+    p.flipped = from.rows > from.cols;
+    if (!s.last)
+        launch_product<kApply, T, L, P>(p, batch, stream);
+    else if (t.weights)
+        launch_product<kUpdate, T, L, P>(p, batch, stream);
+    else
+        launch_product<kOut, T, L, P>(p, batch, stream);
 }
 
 uint32_t up(uint32_t n) { return (n + kPad - 1) / kPad * kPad; }
@@ -274,13 +762,11 @@ uint32_t up(uint32_t n) { return (n + kPad - 1) / kPad * kPad; }
 // The workspace's parts, by their byte offsets.
 struct Layout {
     uint64_t parts, x, xt[2], a, b, bytes;
-    uint64_t side, full;  // elements of one plane of all A and of all X
     uint32_t m, n;
     Layout(uint32_t batch, uint32_t rows, uint32_t cols) {
         m = up(std::min(rows, cols));
         n = up(std::max(rows, cols));
-        full = (uint64_t)batch * m * n;
-        side = (uint64_t)batch * m * m;
+        const uint64_t full = (uint64_t)batch * m * n, side = (uint64_t)batch * m * m;
         uint64_t at = 0;
         auto take = [&](uint64_t n_bytes) {
             const uint64_t o = at;
@@ -297,71 +783,94 @@ struct Layout {
     }
 };
 
-Held held(void* ws, uint64_t offset, uint64_t plane) {
-    f16_t* p = reinterpret_cast<f16_t*>(static_cast<uint8_t*>(ws) + offset);
-    return {p, p + plane};
+Held held(void* ws, uint64_t offset) { return reinterpret_cast<Held>(static_cast<uint8_t*>(ws) + offset); }
+
+// Columns of blocks that a wave of muon_small_kernel holds, 0 where a workgroup
+// cannot hold the matrix: twelve blocks a wave are 48 of its 128 registers.
+uint32_t small_blocks(uint32_t rows, uint32_t cols) {
+    const uint32_t mb = ceil_div(std::min(rows, cols), 16), nt = ceil_div(std::max(rows, cols), 256);
+    if (mb > 4 || nt * mb > 12) return 0;
+    for (uint32_t have : {1u, 2u, 3u, 4u, 6u, 12u})
+        if (nt <= have && have * mb <= 12) return have;
+    return 0;
 }
 
-struct Target {
-    void* out;
-    int64_t row_stride, batch_stride;
-    float* weights;
-    float keep, rate, min_w, max_w;
-};
-
 template <typename T>
-int32_t launch_steps(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws, hipStream_t stream) {
+int32_t launch_small(const Source& s, const Target& t, uint32_t batch, uint32_t steps, hipStream_t stream) {
+    const uint32_t mb = ceil_div(std::min(s.rows, s.cols), 16), nt = small_blocks(s.rows, s.cols);
+    const uint32_t threads = std::min<uint32_t>(16, ceil_div(std::max(s.rows, s.cols), 16)) * kWave;
+    auto go = [&](auto m, auto n) {
+        muon_small_kernel<decltype(m)::value, decltype(n)::value, T><<<batch, threads, 0, stream>>>(s, t, steps);
+    };
+    auto with_columns = [&](auto m) {
+        constexpr int MB = decltype(m)::value;
+        using std::integral_constant;
+        if (nt == 1) return go(m, integral_constant<int, 1>{});
+        if (nt == 2) return go(m, integral_constant<int, 2>{});
+        if (nt == 3) return go(m, integral_constant<int, 3>{});
+        if constexpr (MB <= 3)
+            if (nt == 4) return go(m, integral_constant<int, 4>{});
+        if constexpr (MB <= 2)
+            if (nt == 6) return go(m, integral_constant<int, 6>{});
+        if constexpr (MB == 1)
+            if (nt == 12) return go(m, integral_constant<int, 12>{});
+    };
+    if (mb == 1)
+        with_columns(std::integral_constant<int, 1>{});
+    else if (mb == 2)
+        with_columns(std::integral_constant<int, 2>{});
+    else if (mb == 3)
+        with_columns(std::integral_constant<int, 3>{});
+    else
+        with_columns(std::integral_constant<int, 4>{});
+    TATARA_LAUNCHED("muon_small");
+    return kOk;
+}
+
+// Tiles of 64 where those of 128 would leave CUs without work: a workgroup of the
+// smaller ones has two groups of waves, which keep loads, LDS reads and products
+// of different stages under way on a CU that holds one workgroup.
+using WideTile = Tile<128, 128, 2, 2, 32, 2>;
+using NarrowTile = Tile<64, 64, 2, 2, 64, 3, 2>;
+
+template <typename T, typename L>
+int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws, hipStream_t stream,
+                        uint32_t rough = 0) {
     const Layout l(batch, s.rows, s.cols);
     const bool flipped = s.rows > s.cols;
     double* parts = reinterpret_cast<double*>(static_cast<uint8_t*>(ws) + l.parts);
-    const Held x = held(ws, l.x, l.full), ga = held(ws, l.a, l.side), gb = held(ws, l.b, l.side);
-    const Held xt[2] = {held(ws, l.xt[0], l.full), held(ws, l.xt[1], l.full)};
+    const Held x = held(ws, l.x), ga = held(ws, l.a), gb = held(ws, l.b), xt[2] = {held(ws, l.xt[0]), held(ws, l.xt[1])};
     const uint32_t n_parts = std::min<uint32_t>(kNormParts, ceil_div((uint64_t)s.rows * s.cols, 2048));
     muon_moment_kernel<T><<<dim3(n_parts, batch), 256, 0, stream>>>(s, parts);
     TATARA_LAUNCHED("muon_moment");
     muon_split_kernel<T><<<dim3(up(s.cols) / 64, up(s.rows) / 64, batch), 256, 0, stream>>>(
         s, parts, n_parts, flipped ? xt[0] : x, flipped ? x : xt[0], up(s.rows), up(s.cols));
     TATARA_LAUNCHED("muon_split");
-    const uint32_t tm = ceil_div(l.m, 128), tn = ceil_div(l.n, 128);
     for (uint32_t i = 0; i < steps; ++i) {
-        ProductArgs p{};
-        p.p = p.q = x;
-        p.m = p.n = l.m;
-        p.k = l.n;
-        p.to = ga;
-        muon_product_kernel<kGram, T><<<dim3(tm * (tm + 1) / 2, 1, batch), 256, 0, stream>>>(p);
-        TATARA_LAUNCHED("muon_gram");
-        p.p = p.q = p.old = ga;
-        p.k = l.m;
-        p.to = gb;
-        muon_product_kernel<kPoly, T><<<dim3(tm * (tm + 1) / 2, 1, batch), 256, 0, stream>>>(p);
-        TATARA_LAUNCHED("muon_poly");
-        p.p = gb;
-        p.q = p.old = xt[i % 2];
-        p.n = l.n;
-        p.to = x;
-        p.turned = xt[(i + 1) % 2];
-        p.out = t.out;
-        p.out_row_stride = t.row_stride;
-        p.out_batch_stride = t.batch_stride;
-        p.rows = s.rows;
-        p.cols = s.cols;
-        p.flipped = flipped;
-        p.weights = t.weights;
-        p.keep = t.keep;
-        p.rate = t.rate;
-        p.min_w = t.min_w;
-        p.max_w = t.max_w;
-        const dim3 grid(tm * tn, 1, batch);
-        if (i + 1 < steps)
-            muon_product_kernel<kApply, T><<<grid, 256, 0, stream>>>(p);
-        else if (t.weights)
-            muon_product_kernel<kUpdate, T><<<grid, 256, 0, stream>>>(p);
+        Step step{};
+        step.x = x;
+        step.xt = xt[i % 2];
+        step.next_xt = xt[(i + 1) % 2];
+        step.gram = ga;
+        step.poly = gb;
+        step.m = l.m;
+        step.n = l.n;
+        step.last = i + 1 == steps;
+        if (i < rough)
+            launch_step<T, L, 1>(step, s, t, batch, stream);
         else
-            muon_product_kernel<kOut, T><<<grid, 256, 0, stream>>>(p);
-        TATARA_LAUNCHED("muon_apply");
+            launch_step<T, L, 2>(step, s, t, batch, stream);
+        TATARA_LAUNCHED("muon_product");
     }
     return kOk;
+}
+
+template <typename T>
+int32_t launch_steps(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws, hipStream_t stream) {
+    if (small_blocks(s.rows, s.cols)) return launch_small<T>(s, t, batch, steps, stream);
+    const uint64_t wide = (uint64_t)ceil_div(s.rows, 128) * ceil_div(s.cols, 128) * batch;
+    return wide >= 512 ? launch_products<T, WideTile>(s, t, batch, steps, ws, stream)
+                       : launch_products<T, NarrowTile>(s, t, batch, steps, ws, stream);
 }
 
 int32_t check_matrices(uint32_t batch, uint32_t rows, uint32_t cols, int32_t dtype) {

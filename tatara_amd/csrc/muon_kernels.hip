@@ -27,7 +27,7 @@ constexpr float kHeld = 16384.0f;             // a held value's factor
 constexpr float kUnheld = 1.0f / 16384.0f;
 constexpr float kProduct = 1.0f / (16384.0f * 16384.0f);
 constexpr uint32_t kPad = 64;                 // sides of the held matrices are multiples of it
-constexpr uint32_t kNormParts = 128;          // partial sums of a matrix's norm
+constexpr uint32_t kNormParts = 512;          // partial sums of a matrix's norm, at most
 constexpr uint32_t kMaxSide = 32768;
 
 using half8 = f16_t __attribute__((ext_vector_type(8)));
@@ -61,11 +61,61 @@ struct Source {
     int32_t nesterov;
 };
 
-template <typename T>
-__device__ __forceinline__ float source_value(const Source& s, uint64_t at, float g) {
-    if (!s.momentum) return g;
-    const float m = s.momentum[at];
-    return s.nesterov ? s.mix * g + s.beta * m : m;
+// 1 / (sqrt(sum of squares) + 1e-7) as a power of two and a factor near 1, so that
+// f32 products with a matrix's values neither overflow nor lose bits at any size.
+struct Inverse {
+    float power, factor;
+    __device__ __forceinline__ explicit Inverse(double squares) {
+        const double norm = sqrt(squares) + kNormEps;
+        const int e = norm > 1.0 && norm < 1e300 ? ilogb(norm) : 0;
+        power = (float)ldexp(1.0, -e);
+        factor = (float)(ldexp(1.0, e) / norm);
+    }
+    __device__ __forceinline__ float times(float x) const { return x * power * factor; }
+};
+
+constexpr int kPiece = 8;  // elements of a row that a thread takes at once
+
+// Eight elements of U from (row, col) on, zeros past the row's end.
+template <typename T, bool FIRST>
+__device__ __forceinline__ void source_values(const Source& s, uint32_t b, uint32_t row, uint32_t col,
+                                              float (&u)[kPiece]) {
+    const T* g = static_cast<const T*>(s.grad) + (int64_t)b * s.batch_stride + (int64_t)row * s.row_stride + col;
+    const int left = (int)s.cols - (int)col;
+    Piece<T> p[kPiece / Piece<T>::V];
+#pragma unroll
+    for (int i = 0; i < kPiece; i += Piece<T>::V) p[i / Piece<T>::V].load(g + i, left - i);
+    float m[kPiece];
+    float* at = s.momentum + ((uint64_t)b * s.rows + row) * s.cols + col;
+    if (s.momentum) load_f32(m, at, left, 0.0f);
+#pragma unroll
+    for (int j = 0; j < kPiece; ++j) {
+        const float gv = (float)p[j / Piece<T>::V].v[j % Piece<T>::V];
+        if (!s.momentum) {
+            u[j] = gv;
+            continue;
+        }
+        if (FIRST) m[j] = s.beta * m[j] + s.mix * gv;
+        u[j] = s.nesterov ? s.mix * gv + s.beta * m[j] : m[j];
+    }
+    if (FIRST && s.momentum) {
+        if (left >= kPiece) {
+            __builtin_memcpy(at, m, sizeof(m));
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPiece; ++j)
+                if (j < left) at[j] = m[j];
+        }
+    }
+}
+
+// Sum over the workgroup's 256 threads, the same in all of them.
+__device__ __forceinline__ double block_sum(double x, double (&join)[256 / kWave]) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    if (threadIdx.x % kWave == 0) join[threadIdx.x / kWave] = x;
+    __syncthreads();
+    return join[0] + join[1] + join[2] + join[3];
 }
 
 // Adds the gradient to the momentum and leaves partial sums of |U|^2.  Squares
@@ -73,54 +123,70 @@ __device__ __forceinline__ float source_value(const Source& s, uint64_t at, floa
 template <typename T>
 __global__ __launch_bounds__(256) void muon_moment_kernel(Source s, double* __restrict__ parts) {
     __shared__ double join[256 / kWave];
-    const uint32_t b = blockIdx.y;
-    const T* g = static_cast<const T*>(s.grad) + (int64_t)b * s.batch_stride;
-    const uint64_t n = (uint64_t)s.rows * s.cols;
+    const uint32_t b = blockIdx.y, row_pieces = (s.cols + kPiece - 1) / kPiece, n = s.rows * row_pieces;
     double sum = 0.0;
-    for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t r = i / s.cols;
-        const float gv = (float)g[(int64_t)r * s.row_stride + (int64_t)(i - r * s.cols)];
-        if (s.momentum) {
-            const uint64_t at = b * n + i;
-            s.momentum[at] = s.beta * s.momentum[at] + s.mix * gv;
-        }
-        const double u = (double)source_value<T>(s, b * n + i, gv);
-        sum += u * u;
-    }
+#pragma unroll 2
+    for (uint32_t e = blockIdx.x * 256 + threadIdx.x; e < n; e += gridDim.x * 256) {
+        const uint32_t row = e / row_pieces;
+        float u[kPiece];
+        source_values<T, true>(s, b, row, (e - row * row_pieces) * kPiece, u);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    if (threadIdx.x % kWave == 0) join[threadIdx.x / kWave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) parts[(uint64_t)b * kNormParts + blockIdx.x] = join[0] + join[1] + join[2] + join[3];
+        for (int j = 0; j < kPiece; ++j) sum = fma((double)u[j], (double)u[j], sum);
+    }
+    sum = block_sum(sum, join);
+    if (threadIdx.x == 0) parts[(uint64_t)b * kNormParts + blockIdx.x] = sum;
 }
 
-// Writes X_0 as U lies (straight, [rows up][cols up]) and transposed.
+// Writes X_0 as U lies (straight, [rows up][cols up]) and transposed, 64 x 64 a workgroup.
 template <typename T>
 __global__ __launch_bounds__(256) void muon_split_kernel(Source s, const double* __restrict__ parts, uint32_t n_parts,
                                                          Held straight, Held turned, uint32_t rows_up,
                                                          uint32_t cols_up) {
     __shared__ float tile[64][65];
+    __shared__ double join[256 / kWave];
     const uint32_t b = blockIdx.z, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-    double sum = 0.0;
-    for (uint32_t i = 0; i < n_parts; ++i) sum += parts[(uint64_t)b * kNormParts + i];
-    const double inv = 1.0 / (sqrt(sum) + kNormEps);
-    const T* g = static_cast<const T*>(s.grad) + (int64_t)b * s.batch_stride;
-    const uint64_t n = (uint64_t)s.rows * s.cols, first = 2ull * b * rows_up * cols_up;
-    const uint32_t c = threadIdx.x % 64, q = threadIdx.x / 64;
-    for (uint32_t r = q; r < 64; r += 4) {
-        float v = 0.0f;
-        if (r0 + r < s.rows && c0 + c < s.cols) {
-            const float gv = (float)g[(int64_t)(r0 + r) * s.row_stride + c0 + c];
-            v = (float)((double)source_value<T>(s, b * n + (uint64_t)(r0 + r) * s.cols + c0 + c, gv) * inv);
+    const uint64_t first = 2ull * b * rows_up * cols_up;
+    // two pieces a thread; of the straight matrix, then of the turned one
+    float u[2][kPiece];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t r = r0 + threadIdx.x / 8 + i * 32, c = c0 + threadIdx.x % 8 * 8;
+        if (r < s.rows && c < s.cols) {
+            source_values<T, false>(s, b, r, c, u[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPiece; ++j) u[i][j] = 0.0f;
         }
-        tile[r][c] = v;
-        f16_t* to = straight + first + held_at(r0 + r, c0 + c, cols_up);
-        split(v, to[0], to[kLow]);
+    }
+    double sum = 0.0;
+    for (uint32_t i = threadIdx.x; i < n_parts; i += 256) sum += parts[(uint64_t)b * kNormParts + i];
+    const Inverse inv(block_sum(sum, join));
+    auto put = [&](Held to, const float (&v)[kPiece]) {
+        half8 hi, lo;
+#pragma unroll
+        for (int j = 0; j < kPiece; ++j) {
+            f16_t h, l;
+            split(v[j], h, l);
+            hi[j] = h;
+            lo[j] = l;
+        }
+        *reinterpret_cast<half8*>(to) = hi;
+        *reinterpret_cast<half8*>(to + kLow) = lo;
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t r = threadIdx.x / 8 + i * 32, c = threadIdx.x % 8 * 8;
+#pragma unroll
+        for (int j = 0; j < kPiece; ++j) tile[r][c + j] = u[i][j] = inv.times(u[i][j]);
+        put(straight + first + held_at(r0 + r, c0 + c, cols_up), u[i]);
     }
     __syncthreads();
-    for (uint32_t r = q; r < 64; r += 4) {
-        f16_t* to = turned + first + held_at(c0 + r, r0 + c, rows_up);
-        split(tile[c][r], to[0], to[kLow]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t c = threadIdx.x / 8 + i * 32, r = threadIdx.x % 8 * 8;
+#pragma unroll
+        for (int j = 0; j < kPiece; ++j) u[i][j] = tile[r + j][c];
+        put(turned + first + held_at(c0 + c, r0 + r, rows_up), u[i]);
     }
 }
 
@@ -143,132 +209,257 @@ struct Halves {
     half4 hi, lo;
 };
 
-__device__ __forceinline__ Halves split4(const floatx4& v) {
+using half2 = f16_t __attribute__((ext_vector_type(2)));
+using floatx2 = float __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ half4 to_halves(const floatx4& v) {
+    const half2 a = __builtin_convertvector(__builtin_shufflevector(v, v, 0, 1), half2);
+    const half2 b = __builtin_convertvector(__builtin_shufflevector(v, v, 2, 3), half2);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3);
+}
+// Of values that have their factor already.
+__device__ __forceinline__ Halves split_held(const floatx4& v) {
     Halves h;
+    h.hi = to_halves(v);
+    floatx4 rest;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        f16_t a, b;
-        split(v[r], a, b);
-        h.hi[r] = a;
-        h.lo[r] = b;
-    }
+    for (int r = 0; r < 4; ++r) rest[r] = fmaf((float)h.hi[r], -1.0f, v[r]);
+    h.lo = to_halves(rest);
     return h;
 }
+__device__ __forceinline__ Halves split4(const floatx4& v) { return split_held(v * kHeld); }
 
-__device__ __forceinline__ floatx4 product16(const Halves& a, const Halves& b, floatx4 c) {
-    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.lo, b.hi, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.lo, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.hi, c, 0, 0, 0);
+__device__ __forceinline__ half8 join8(const half4& a, const half4& b) {
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// Products of 16 x 16 blocks, which fill the 32 values of k of an instruction by
+// twos; which k a lane's values stand for does not matter as long as both operands
+// agree.  (16x16x16 takes as long for half the work, and one right behind a
+// 16x16x32 whose sum it adds to has been seen to read that sum too early.)
+__device__ __forceinline__ floatx4 mfma32(const half8& a, const half8& b, const floatx4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+// Two blocks: lo hi, hi lo, hi hi of both.
+__device__ __forceinline__ void products(const Halves& a0, const Halves& a1, const Halves& b0, const Halves& b1,
+                                         floatx4& low, floatx4& mid, floatx4& c) {
+    const half8 ah = join8(a0.hi, a1.hi), bh = join8(b0.hi, b1.hi);
+    low = mfma32(join8(a0.lo, a1.lo), bh, low);
+    mid = mfma32(ah, join8(b0.lo, b1.lo), mid);
+    c = mfma32(ah, bh, c);
+}
+// One block: a's hi, then its lo, with both halves of b (lo lo comes for nothing).
+__device__ __forceinline__ floatx4 product(const half8& a_hi, const half8& a_lo, const Halves& b, floatx4 c) {
+    const half8 both = join8(b.hi, b.lo);
+    c = mfma32(a_lo, both, c);
+    return mfma32(a_hi, both, c);
+}
+__device__ __forceinline__ floatx4 product(const Halves& a, const Halves& b, const floatx4& c) {
+    return product(join8(a.hi, a.hi), join8(a.lo, a.lo), b, c);
+}
+
+// Four elements of a row: at a byte offset from the matrix that is the same for all
+// lanes, plus the lane's.  WHOLE: every lane's four exist, and nothing is worked out
+// a load.  Otherwise `left` exist, with zeros in the place of the others; their
+// loads are in no branch, which would wait for each: they read the matrix's start.
+template <bool WHOLE, typename V>
+__device__ __forceinline__ floatx4 load4(const V* base, uint32_t uniform, uint32_t lane, int left) {
+    const char* p = reinterpret_cast<const char*>(base);
+    floatx4 f;
+    if (WHOLE) {
+        V v[4];
+        __builtin_memcpy(v, p + uniform + lane, sizeof(v));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = (float)v[r];
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const V v = *reinterpret_cast<const V*>(p + (r < left ? uniform + lane + r * (uint32_t)sizeof(V) : 0u));
+            f[r] = r < left ? (float)v : 0.0f;
+        }
+    }
+    return f;
+}
+template <bool WHOLE, typename V>
+__device__ __forceinline__ void store4(V* base, uint32_t uniform, uint32_t lane, int left, const floatx4& f) {
+    V* p = reinterpret_cast<V*>(reinterpret_cast<char*>(base) + uniform + lane);
+    const V v[4] = {(V)f[0], (V)f[1], (V)f[2], (V)f[3]};
+    if (WHOLE) {
+        __builtin_memcpy(p, v, sizeof(v));
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < left) p[r] = v[r];
+    }
 }
 
 // All steps of a matrix of a few rows in one workgroup: X stays in registers, in
 // blocks of 16 x 16, MB rows of blocks and NT columns of them a wave.  An MFMA
 // result's lane holds four rows of a column, which is also how 16x16x16 takes its
-// right operand, so B X needs no rearrangement; X X^T takes blocks that were
-// turned through LDS.  Each wave sums X X^T over its columns, the workgroup adds
-// the waves' sums in order.
+// right operand, so B X needs no rearrangement; X X^T takes the blocks
+// transposed, which a product with the identity gives (exactly: one term a sum).
+// Each wave sums X X^T over its columns, the workgroup adds the waves' sums in
+// order.
 template <int MB, int NT, typename T>
 __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, uint32_t steps) {
     constexpr int NB = MB * (MB + 1) / 2, CHUNK = NB < 4 ? NB : 4, PITCH = MB * 16 + 4;
     __shared__ __align__(16) float gram[MB * 16][PITCH];
     __shared__ __align__(16) f16_t poly_hi[MB * 16][PITCH], poly_lo[MB * 16][PITCH];
     __shared__ floatx4 parts[16][CHUNK][kWave];
-    __shared__ __align__(16) float turned[16][16][20];
     __shared__ double join[16];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
     const uint32_t col = lane % 16, row4 = lane / 16 * 4;
     const bool flipped = s.rows > s.cols;
     const uint32_t m = flipped ? s.cols : s.rows, n = flipped ? s.rows : s.cols, b = blockIdx.x;
-    // element (x, y) of X lies at x * down + y * over of a contiguous matrix
-    const uint32_t down = flipped ? 1 : s.cols, over = flipped ? s.cols : 1;
+    half4 identity;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) identity[r] = row4 + r == col ? (f16_t)1.0f : (f16_t)0.0f;
+    const half8 of_hi = join8(identity, half4{}), of_lo = join8(half4{}, identity);
+    const floatx4 zero = {};
+    // a block transposed, exactly: a sum of one term
+    auto turn16 = [&](const Halves& h) {
+        Halves o;
+        o.hi = to_halves(mfma32(join8(h.hi, h.lo), of_hi, zero));
+        o.lo = to_halves(mfma32(join8(h.hi, h.lo), of_lo, zero));
+        return o;
+    };
+    // A lane reads and writes four neighbours of a row of U, neighbouring lanes the
+    // next ones (lane by lane from row to row, loads took ten times as long), which
+    // LDS puts where the products take them.  A lane's part of the offset is the
+    // same for all its blocks, the rest the same for all lanes.
+    const uint32_t my_row = lane / 4, my_col = lane % 4 * 4;
+    auto moved = [&](int slot, const Halves& h, uint32_t from, uint32_t to) {
+        half8* at = reinterpret_cast<half8*>(parts[wave][slot % CHUNK]);
+        at[from] = join8(h.hi, h.lo);
+        __builtin_amdgcn_wave_barrier();
+        const half8 v = at[to];
+        __builtin_amdgcn_wave_barrier();
+        Halves o;
+        o.hi = __builtin_shufflevector(v, v, 0, 1, 2, 3);
+        o.lo = __builtin_shufflevector(v, v, 4, 5, 6, 7);
+        return o;
+    };
     const uint64_t first = (uint64_t)b * s.rows * s.cols;
-    const uint32_t y0 = wave * 16 + col;
-    floatx4 x[MB][NT];
-    double sum = 0.0;
-    {
+    const uint32_t y0 = __builtin_amdgcn_readfirstlane(wave) * 16;
+    auto left = [&](int ib, int tt) {
+        const uint32_t y = tt * waves * 16 + y0;
+        const uint32_t r = flipped ? y + my_row : ib * 16 + my_row, c = flipped ? ib * 16 + my_col : y + my_col;
+        return r < s.rows ? (int)s.cols - (int)c : 0;
+    };
+    auto uniform = [&](int64_t row_stride, uint32_t size, int ib, int tt) {
+        const uint32_t pitch = (uint32_t)row_stride * size, y = tt * waves * 16 + y0;
+        return flipped ? y * pitch + ib * 16 * size : ib * 16 * pitch + y * size;
+    };
+    auto mine = [&](int64_t row_stride, uint32_t size) {
+        return my_row * (uint32_t)row_stride * size + my_col * size;
+    };
+    // all of the wave's blocks lie inside
+    const bool whole = m == MB * 16 && (NT - 1) * waves * 16 + y0 + 16 <= n;
+    // The weights are read with the rest where registers last (6 blocks a lane).
+    constexpr bool EARLY = MB * NT <= 6;
+    floatx4 u[MB][NT], w[EARLY ? MB : 1][EARLY ? NT : 1];
+    auto read = [&](auto is_whole) {
+        constexpr bool WHOLE = decltype(is_whole)::value;
         const T* g = static_cast<const T*>(s.grad) + (int64_t)b * s.batch_stride;
-        const int64_t g_down = flipped ? 1 : s.row_stride, g_over = flipped ? s.row_stride : 1;
+        const uint32_t g_lane = mine(s.row_stride, sizeof(T)), w_lane = mine(s.cols, 4);
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) {
-            const uint32_t y = tt * waves * 16 + y0;
+        for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
             for (int ib = 0; ib < MB; ++ib)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t xx = ib * 16 + row4 + r;
-                    const bool in = xx < m && y < n;
-                    const float gv = (float)g[in ? xx * g_down + y * g_over : 0];
-                    x[ib][tt][r] = in ? gv : 0.0f;
-                }
-        }
-    }
-    if (s.momentum) {
+                u[ib][tt] = load4<WHOLE>(g, uniform(s.row_stride, sizeof(T), ib, tt), g_lane, left(ib, tt));
+        if (!s.momentum) return;
         float* mom = s.momentum + first;
+        // columns of blocks whose loads go out together, ahead of their stores
+        constexpr int BATCH = EARLY ? NT : (6 + MB - 1) / MB;
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) {
-            const uint32_t y = tt * waves * 16 + y0;
-            float mo[MB][4];
+        for (int t0 = 0; t0 < NT; t0 += BATCH) {
+            floatx4 mo[BATCH][MB];
 #pragma unroll
-            for (int ib = 0; ib < MB; ++ib)
+            for (int q = 0; q < BATCH && t0 + q < NT; ++q)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t xx = ib * 16 + row4 + r;
-                    mo[ib][r] = s.beta * mom[xx < m && y < n ? xx * down + y * over : 0] + s.mix * x[ib][tt][r];
-                }
+                for (int ib = 0; ib < MB; ++ib)
+                    mo[q][ib] = load4<WHOLE>((const float*)mom, uniform(s.cols, 4, ib, t0 + q), w_lane, left(ib, t0 + q));
+            if constexpr (EARLY) {  // momentum comes with weights
 #pragma unroll
-            for (int ib = 0; ib < MB; ++ib)
+                for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t xx = ib * 16 + row4 + r;
-                    const bool in = xx < m && y < n;
-                    if (in) mom[xx * down + y * over] = mo[ib][r];
-                    const float u = s.nesterov ? s.mix * x[ib][tt][r] + s.beta * mo[ib][r] : mo[ib][r];
-                    x[ib][tt][r] = in ? u : 0.0f;
+                    for (int ib = 0; ib < MB; ++ib)
+                        w[ib][tt] = load4<WHOLE>((const float*)t.weights + first, uniform(s.cols, 4, ib, tt), w_lane,
+                                                 left(ib, tt));
+            }
+#pragma unroll
+            for (int q = 0; q < BATCH && t0 + q < NT; ++q)
+#pragma unroll
+                for (int ib = 0; ib < MB; ++ib) {
+                    const floatx4 gv = u[ib][t0 + q], m1 = s.beta * mo[q][ib] + s.mix * gv;
+                    store4<WHOLE>(mom, uniform(s.cols, 4, ib, t0 + q), w_lane, left(ib, t0 + q), m1);
+                    u[ib][t0 + q] = s.nesterov ? s.mix * gv + s.beta * m1 : m1;  // zeros stay zeros
                 }
         }
-    }
+    };
+    if (whole)
+        read(std::true_type{});
+    else
+        read(std::false_type{});
+    double sum = 0.0;
 #pragma unroll
     for (int ib = 0; ib < MB; ++ib)
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) sum += (double)x[ib][tt][r] * (double)x[ib][tt][r];
+            for (int r = 0; r < 4; ++r) sum = fma((double)u[ib][tt][r], (double)u[ib][tt][r], sum);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (lane == 0) join[wave] = sum;
     __syncthreads();
     sum = 0.0;
-#pragma unroll 1
-    for (uint32_t w = 0; w < waves; ++w) sum += join[w];
-    const double inv = 1.0 / (sqrt(sum) + kNormEps);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += (uint32_t)i < waves ? join[i] : 0.0;
+    const Inverse inv(sum);
+    // X as it is held; its f32 values only pass through
+    Halves x[MB][NT];
 #pragma unroll
     for (int ib = 0; ib < MB; ++ib)
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt)
+        for (int tt = 0; tt < NT; ++tt) {
+            floatx4 v;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[ib][tt][r] = (float)((double)x[ib][tt][r] * inv);
+            for (int r = 0; r < 4; ++r) v[r] = inv.times(u[ib][tt][r]) * kHeld;
+            x[ib][tt] = moved(ib * NT + tt, split_held(v), lane, col * 4 + row4 / 4);
+        }
+    if (!flipped) {
+#pragma unroll
+        for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+            for (int tt = 0; tt < NT; ++tt) x[ib][tt] = turn16(x[ib][tt]);
+    }
 
 #pragma unroll 1
     for (uint32_t step = 0; step < steps; ++step) {
-        floatx4 acc[NB] = {};
+        floatx4 low[NB], mid[NB], acc[NB];
 #pragma unroll
-        for (int tt = 0; tt < NT; ++tt) {
-            Halves rows[MB];
+        for (int k = 0; k < NB; ++k) low[k] = mid[k] = acc[k] = zero;
 #pragma unroll
-            for (int ib = 0; ib < MB; ++ib) {
+        for (int tt = 0; tt < NT; tt += 2) {
+            Halves rows[2][MB];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) turned[wave][row4 + r][col] = x[ib][tt][r];
-                __builtin_amdgcn_wave_barrier();
-                rows[ib] = split4(*reinterpret_cast<const floatx4*>(&turned[wave][col][row4]));
-                __builtin_amdgcn_wave_barrier();
-            }
+            for (int o = 0; o < 2 && tt + o < NT; ++o)
+#pragma unroll
+                for (int ib = 0; ib < MB; ++ib) rows[o][ib] = turn16(x[ib][tt + o]);
             int k = 0;
 #pragma unroll
             for (int ib = 0; ib < MB; ++ib)
 #pragma unroll
-                for (int jb = ib; jb < MB; ++jb, ++k) acc[k] = product16(rows[ib], rows[jb], acc[k]);
-            __builtin_amdgcn_sched_barrier(0);  // columns one after the other: their blocks would not fit
+                for (int jb = ib; jb < MB; ++jb, ++k) {
+                    // separate sums where there are too few blocks to fill the wait for one
+                    floatx4 &l = MB == 1 ? low[k] : acc[k], &m_ = MB == 1 ? mid[k] : acc[k];
+                    if (tt + 1 < NT)
+                        products(rows[0][ib], rows[1][ib], rows[0][jb], rows[1][jb], l, m_, acc[k]);
+                    else
+                        acc[k] = product(rows[0][ib], rows[0][jb], acc[k]);
+                }
+            if (MB > 1) __builtin_amdgcn_sched_barrier(0);  // more columns' blocks at once would not fit
         }
+        if (MB == 1) acc[0] += low[0] + mid[0];
 #pragma unroll
         for (int k0 = 0; k0 < NB; k0 += CHUNK) {
 #pragma unroll
@@ -276,11 +467,17 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
                 if (k0 + k < NB) parts[wave][k][lane] = acc[k0 + k];
             __syncthreads();
             const uint32_t have = (NB - k0 < CHUNK ? NB - k0 : CHUNK) * 256;
-            for (uint32_t e = threadIdx.x; e < have; e += blockDim.x) {
+            // four lanes an element, four waves' sums a lane
+            for (uint32_t q = threadIdx.x; q < have * 4; q += blockDim.x) {
+                const uint32_t e = q / 4, w0 = q % 4 * 4;
                 float v = 0.0f;
-#pragma unroll 1
-                for (uint32_t w = 0; w < waves; ++w) v += reinterpret_cast<const float*>(parts[w])[e];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i)
+                    v += w0 + i < waves ? reinterpret_cast<const float*>(parts[w0 + i])[e] : 0.0f;
+                v += __shfl_xor(v, 1);
+                v += __shfl_xor(v, 2);
                 v *= kProduct;
+                if (w0) continue;
                 uint32_t k = k0 + e / 256, ib = 0;
                 while (k >= MB - ib) k -= MB - ib, ++ib;
                 const uint32_t jb = ib + k, l = e % 256 / 4;
@@ -290,70 +487,95 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
             }
             __syncthreads();
         }
-        for (uint32_t k = wave; k < MB * MB; k += waves) {
-            const uint32_t ib = k / MB, jb = k % MB;
-            floatx4 v = {};
+        // block (ib, jb) of B, four rows of a column a lane
+        auto poly = [&](uint32_t ib, uint32_t jb) {
+            floatx4 v = zero;
 #pragma unroll
             for (int kb = 0; kb < MB; ++kb)
-                v = product16(split4(*reinterpret_cast<const floatx4*>(&gram[ib * 16 + col][kb * 16 + row4])),
-                              split4(*reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][kb * 16 + row4])), v);
-            // B is symmetric: four rows of a column stored as four columns of a row
+                v = product(split4(*reinterpret_cast<const floatx4*>(&gram[ib * 16 + col][kb * 16 + row4])),
+                            split4(*reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][kb * 16 + row4])), v);
             const floatx4 old = *reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][ib * 16 + row4]);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 v[r] = fmaf(kC, v[r] * kProduct, fmaf(kB, old[r], ib == jb && row4 + r == col ? kA : 0.0f));
-            const Halves h = split4(v);
-            *reinterpret_cast<half4*>(&poly_hi[jb * 16 + col][ib * 16 + row4]) = h.hi;
-            *reinterpret_cast<half4*>(&poly_lo[jb * 16 + col][ib * 16 + row4]) = h.lo;
+            // without the factor, so that B X has X's: of B's entries, up to 3.45, no
+            // more than 2^-25 is lost to f16's smallest numbers
+            return split_held(v);
+        };
+        // B is symmetric: four rows of a column are four columns of a row, as the
+        // left operand takes them.  One block every wave computes for itself.
+        Halves only;
+        if constexpr (MB == 1) {
+            only = poly(0, 0);
+        } else {
+            for (uint32_t k = wave; k < MB * MB; k += waves) {
+                const uint32_t ib = k / MB, jb = k % MB;
+                const Halves h = poly(ib, jb);
+                *reinterpret_cast<half4*>(&poly_hi[jb * 16 + col][ib * 16 + row4]) = h.hi;
+                *reinterpret_cast<half4*>(&poly_lo[jb * 16 + col][ib * 16 + row4]) = h.lo;
+            }
+            __syncthreads();
         }
-        __syncthreads();
 #pragma unroll
         for (int tt = 0; tt < NT; ++tt) {
             Halves cols[MB];
 #pragma unroll
-            for (int kb = 0; kb < MB; ++kb) cols[kb] = split4(x[kb][tt]);
+            for (int kb = 0; kb < MB; ++kb) cols[kb] = x[kb][tt];
 #pragma unroll
             for (int ib = 0; ib < MB; ++ib) {
-                floatx4 v = {};
-#pragma unroll
-                for (int kb = 0; kb < MB; ++kb) {
+                floatx4 v = zero;
+                auto block = [&](int kb) {
+                    if (MB == 1) return only;
                     Halves h;
                     h.hi = *reinterpret_cast<const half4*>(&poly_hi[ib * 16 + col][kb * 16 + row4]);
                     h.lo = *reinterpret_cast<const half4*>(&poly_lo[ib * 16 + col][kb * 16 + row4]);
-                    v = product16(h, cols[kb], v);
-                }
+                    return h;
+                };
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[ib][tt][r] = v[r] * kProduct;
+                for (int kb = 0; kb + 1 < MB; kb += 2)
+                    products(block(kb), block(kb + 1), cols[kb], cols[kb + 1], v, v, v);
+                if (MB % 2) v = product(block(MB - 1), cols[MB - 1], v);
+                x[ib][tt] = split_held(v);
             }
-            __builtin_amdgcn_sched_barrier(0);
+            if (MB > 1) __builtin_amdgcn_sched_barrier(0);
         }
     }
-    const int64_t o_down = flipped ? 1 : t.row_stride, o_over = flipped ? t.row_stride : 1;
+    auto write = [&](auto is_whole) {
+        constexpr bool WHOLE = decltype(is_whole)::value;
+        const uint32_t w_lane = mine(s.cols, 4), o_lane = mine(t.row_stride, sizeof(T));
 #pragma unroll
-    for (int tt = 0; tt < NT; ++tt) {
-        const uint32_t y = tt * waves * 16 + y0;
-        float w[MB][4];
-        if (t.weights) {
+        for (int tt = 0; tt < NT; ++tt) {
+            if constexpr (!EARLY) {
+                if (t.weights) {
 #pragma unroll
-            for (int ib = 0; ib < MB; ++ib)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t xx = ib * 16 + row4 + r;
-                    w[ib][r] = t.weights[first + (xx < m && y < n ? xx * down + y * over : 0)];
+                    for (int ib = 0; ib < MB; ++ib)
+                        u[ib][tt] = load4<WHOLE>((const float*)t.weights + first, uniform(s.cols, 4, ib, tt), w_lane,
+                                                 left(ib, tt));
                 }
-        }
-#pragma unroll
-        for (int ib = 0; ib < MB; ++ib)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t xx = ib * 16 + row4 + r;
-                if (xx >= m || y >= n) continue;
-                if (t.weights)
-                    t.weights[first + xx * down + y * over] = updated(t, w[ib][r], x[ib][tt][r]);
-                else
-                    static_cast<T*>(t.out)[(int64_t)b * t.batch_stride + xx * o_down + y * o_over] = (T)x[ib][tt][r];
             }
-    }
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib) {
+                const Halves h =
+                    moved(ib * NT + tt, flipped ? x[ib][tt] : turn16(x[ib][tt]), col * 4 + row4 / 4, lane);
+                floatx4 v;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = ((float)h.hi[r] + (float)h.lo[r]) * kUnheld;
+                if (t.weights) {
+                    const floatx4 old = EARLY ? w[EARLY ? ib : 0][EARLY ? tt : 0] : u[ib][tt];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = updated(t, old[r], v[r]);
+                    store4<WHOLE>(t.weights + first, uniform(s.cols, 4, ib, tt), w_lane, left(ib, tt), v);
+                } else {
+                    store4<WHOLE>(static_cast<T*>(t.out) + (int64_t)b * t.batch_stride,
+                                  uniform(t.row_stride, sizeof(T), ib, tt), o_lane, left(ib, tt), v);
+                }
+            }
+        }
+    };
+    if (whole)
+        write(std::true_type{});
+    else
+        write(std::false_type{});
 }
 
 // What becomes of a product's tile.
@@ -835,12 +1057,12 @@ using NarrowTile = Tile<64, 64, 2, 2, 64, 3, 2>;
 
 template <typename T, typename L>
 int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws, hipStream_t stream,
-                        uint32_t rough = 0) {
+                        uint32_t rough) {
     const Layout l(batch, s.rows, s.cols);
     const bool flipped = s.rows > s.cols;
     double* parts = reinterpret_cast<double*>(static_cast<uint8_t*>(ws) + l.parts);
     const Held x = held(ws, l.x), ga = held(ws, l.a), gb = held(ws, l.b), xt[2] = {held(ws, l.xt[0]), held(ws, l.xt[1])};
-    const uint32_t n_parts = std::min<uint32_t>(kNormParts, ceil_div((uint64_t)s.rows * s.cols, 2048));
+    const uint32_t n_parts = std::min<uint32_t>(kNormParts, ceil_div((uint64_t)s.rows * ceil_div(s.cols, kPiece), 256));
     muon_moment_kernel<T><<<dim3(n_parts, batch), 256, 0, stream>>>(s, parts);
     TATARA_LAUNCHED("muon_moment");
     muon_split_kernel<T><<<dim3(up(s.cols) / 64, up(s.rows) / 64, batch), 256, 0, stream>>>(
@@ -865,12 +1087,29 @@ int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32
     return kOk;
 }
 
+// First steps that multiply hi parts alone (11 bits; X itself keeps its 22).  Their
+// rounding is an error of X that later steps see as part of X: the steps that
+// follow in full move it along with the rest, so it fades.  Five steps end with an
+// error of X, from the products, of 2e-3 to 4e-3 (none full), 2e-4 to 3e-3 (two,
+// the less the larger the matrix: up to 8e-4 from a short side of 256 on) or 3e-5
+// to 7e-4 (three).  A result of 16 bits is rounded to 1.7e-3 (bf16) or 2e-4 (f16),
+// so bf16 takes two full steps from 256 on and three below, f16 three: 9 or 11
+// products of 15.  f32 results take full products throughout.
+template <typename T>
+uint32_t rough_steps(uint32_t steps, uint32_t side) {
+    const uint32_t full = sizeof(T) == 4 ? steps : std::is_same<T, bf16_t>::value && side >= 256 ? 2 : 3;
+    return steps > full ? steps - full : 0;
+}
+
 template <typename T>
 int32_t launch_steps(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws, hipStream_t stream) {
-    if (small_blocks(s.rows, s.cols)) return launch_small<T>(s, t, batch, steps, stream);
+    // its offsets within a matrix are of 32 bits
+    const bool near = (uint64_t)s.rows * std::max(s.row_stride, t.row_stride) < (1u << 29);
+    if (near && small_blocks(s.rows, s.cols)) return launch_small<T>(s, t, batch, steps, stream);
     const uint64_t wide = (uint64_t)ceil_div(s.rows, 128) * ceil_div(s.cols, 128) * batch;
-    return wide >= 512 ? launch_products<T, WideTile>(s, t, batch, steps, ws, stream)
-                       : launch_products<T, NarrowTile>(s, t, batch, steps, ws, stream);
+    const uint32_t rough = t.weights ? 0 : rough_steps<T>(steps, std::min(s.rows, s.cols));
+    return wide >= 512 ? launch_products<T, WideTile>(s, t, batch, steps, ws, stream, rough)
+                       : launch_products<T, NarrowTile>(s, t, batch, steps, ws, stream, rough);
 }
 
 int32_t check_matrices(uint32_t batch, uint32_t rows, uint32_t cols, int32_t dtype) {

@@ -264,7 +264,7 @@ TATARA_API int32_t tatara_op_quantise_ft_noalloc(const float* w, uint64_t rows, 
  * element.  Inputs and outputs must not overlap unless stated.  `workspace` has
  * at least the bytes that the call's *_workspace function gives, aligned to 16
  * bytes, and is used by one call at a time (calls on one stream may share it);
- * its contents need not be kept or cleared.  Results do not depend on the run:
+ * its contents need not be kept or cleared unless stated.  Results do not depend on the run:
  * every sum has a fixed order. */
 #define TATARA_F32 0
 #define TATARA_F16 1
@@ -303,7 +303,9 @@ TATARA_API int32_t tatara_op_layer_norm_backward(const void* dy, int64_t dy_stri
  * stand where fewer than top_k are left.  A position with valid[t] == 0 (valid
  * may be NULL) or with every bucket masked does not count and chooses nothing.
  * bucket and gate are [positions][top_k]; counted and loss one value each; all
- * outputs are overwritten. */
+ * outputs are overwritten.
+ * The forward call's workspace begins with a count that is zero between calls:
+ * its first 4096 bytes must be zero before the first. */
 TATARA_API int32_t tatara_op_bucket_gate_workspace(uint32_t buckets, uint64_t* bytes);
 TATARA_API int32_t tatara_op_bucket_gate_forward(const void* logits, int64_t stride, const uint8_t* valid,
                                                  uint64_t positions, uint32_t buckets, uint32_t top_k,

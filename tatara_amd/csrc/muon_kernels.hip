@@ -83,11 +83,18 @@ __device__ __forceinline__ void source_values(const Source& s, uint32_t b, uint3
     const T* g = static_cast<const T*>(s.grad) + (int64_t)b * s.batch_stride + (int64_t)row * s.row_stride + col;
     const int left = (int)s.cols - (int)col;
     Piece<T> p[kPiece / Piece<T>::V];
-#pragma unroll
-    for (int i = 0; i < kPiece; i += Piece<T>::V) p[i / Piece<T>::V].load(g + i, left - i);
     float m[kPiece];
     float* at = s.momentum + ((uint64_t)b * s.rows + row) * s.cols + col;
-    if (s.momentum) load_f32(m, at, left, 0.0f);
+    if (left >= kPiece) {
+        __builtin_memcpy(p, g, sizeof(p));
+        if (s.momentum) __builtin_memcpy(m, at, sizeof(m));
+    } else {
+#pragma unroll
+        for (int j = 0; j < kPiece; ++j) {
+            p[j / Piece<T>::V].v[j % Piece<T>::V] = j < left ? g[j] : (T)0.0f;
+            m[j] = s.momentum && j < left ? at[j] : 0.0f;
+        }
+    }
 #pragma unroll
     for (int j = 0; j < kPiece; ++j) {
         const float gv = (float)p[j / Piece<T>::V].v[j % Piece<T>::V];

@@ -17,8 +17,13 @@ namespace {
 // 32768 columns.
 constexpr int kLaneValues = 32;
 constexpr uint32_t kMaxCols = 16 * kWave * kLaneValues;
-// Workgroups of the backward pass, each of which leaves a partial sum of dw and db.
+// Workgroups of the backward pass, each of which leaves a partial sum of dw and db:
+// two a CU (65536 x 1536 bf16: 121 us, with four 130), one where rows are few
+// (1009 x 769 f32: 8.9 us, with two 9.8).
 constexpr uint32_t kGradBlocks = 512;
+uint32_t grad_blocks(uint64_t units) {
+    return (uint32_t)std::min<uint64_t>(units, units >= 2048 ? kGradBlocks : kGradBlocks / 2);
+}
 
 // Sum over the W waves of a row; `slot` alternates so that one barrier a sum is enough.
 template <int W>
@@ -34,7 +39,8 @@ __device__ __forceinline__ float row_sum(float x, float (*part)[W], int slot) {
     return x;
 }
 
-template <typename T, int W, int N>
+// FEW: rows of fewer elements than a piece has.
+template <typename T, int W, int N, bool FEW>
 __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_forward_kernel(
     const T* __restrict__ x, int64_t x_stride, const float* __restrict__ weight, const float* __restrict__ bias,
     T* __restrict__ y, int64_t y_stride, float* __restrict__ mean, float* __restrict__ rstd, uint64_t rows,
@@ -44,23 +50,31 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_forward_kernel(
     const uint32_t lane = threadIdx.x % (kWave * W);
     const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x / (kWave * W)) + threadIdx.x / (kWave * W);
     if (row >= rows) return;  // W > 1: one row a workgroup, so all of it returns
-    const T* xr = x + (int64_t)row * x_stride;
+    auto column = [&](int i) { return (int)(i * kWave * W + lane) * V; };
+    auto read = [&](auto& piece, const auto* from, int i) {
+        if (FEW)
+            piece.load_few(from, (int)cols - column(i));
+        else
+            piece.load(from, column(i), (int)cols);
+    };
+    auto fix = [&](auto& piece, int i) {
+        if (!FEW) piece.fix((int)cols - column(i));
+    };
     Piece<T> in[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int c = (i * kWave * W + lane) * V;
-        in[i].load(xr + c, (int)cols - c);
-    }
+    for (int i = 0; i < N; ++i) read(in[i], x + (int64_t)row * x_stride, i);
     float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < N; ++i) {
+        fix(in[i], i);
 #pragma unroll
         for (int j = 0; j < V; ++j) s += (float)in[i].v[j];
+    }
     const float m = row_sum<W>(s, part, 0) / (float)cols;
     s = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int left = (int)cols - (int)(i * kWave * W + lane) * V;
+        const int left = (int)cols - column(i);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float d = j < left ? (float)in[i].v[j] - m : 0.0f;
@@ -75,23 +89,24 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_forward_kernel(
     T* yr = y + (int64_t)row * y_stride;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int c = (i * kWave * W + lane) * V;
-        const int left = (int)cols - c;
+        const int left = (int)cols - column(i);
         if (left <= 0) break;
-        float w[V], b[V];
-        if (weight) load_f32(w, weight + c, left, 0.0f);
-        if (bias) load_f32(b, bias + c, left, 0.0f);
+        Floats<V> w, b;
+        if (weight) read(w, weight, i);
+        if (bias) read(b, bias, i);
+        if (weight) fix(w, i);
+        if (bias) fix(b, i);
         Piece<T> out;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const float h = ((float)in[i].v[j] - m) * r;
             out.v[j] = (T)fmaf(h, weight ? w[j] : 1.0f, bias ? b[j] : 0.0f);
         }
-        out.store(yr + c, left);
+        out.store(yr + column(i), left);
     }
 }
 
-template <typename T, int W, int N>
+template <typename T, int W, int N, bool FEW>
 __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_backward_kernel(
     const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ x, int64_t x_stride,
     const float* __restrict__ weight, const float* __restrict__ mean, const float* __restrict__ rstd,
@@ -101,54 +116,87 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_backward_kernel(
     __shared__ float part[4][W];
     __shared__ float join[G == 1 ? 1 : (G - 1) * kWave * N * V];
     const uint32_t lane = threadIdx.x % (kWave * W), group = threadIdx.x / (kWave * W);
+    auto column = [&](int i) { return (int)(i * kWave * W + lane) * V; };
+    auto read = [&](auto& piece, const auto* from, int i) {
+        if (FEW)
+            piece.load_few(from, (int)cols - column(i));
+        else
+            piece.load(from, column(i), (int)cols);
+    };
+    auto fix = [&](auto& piece, int i) {
+        if (!FEW) piece.fix((int)cols - column(i));
+    };
+    // the weight stays in registers where they last
+    constexpr bool KEEP = N * V <= 24 || sizeof(T) == 2;
     float dw[N * V], db[N * V];
+    Floats<V> kept[KEEP ? N : 1];
 #pragma unroll
     for (int i = 0; i < N * V; ++i) dw[i] = db[i] = 0.0f;
-    int slot = 0;
-    for (uint64_t row = (uint64_t)blockIdx.x * G + group; row < rows; row += (uint64_t)gridDim.x * G) {
-        Piece<T> px[N], pd[N];
+    auto weights = [&](int i) {
+        Floats<V> w;
+        if (weight) {
+            read(w, weight, i);
+            fix(w, i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w.p[j / 4].v[j % 4] = 1.0f;
+        }
+        return w;
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) kept[i] = weights(i);
+    }
+    Piece<T> px[N], pd[N];
+    float m = 0.0f, r = 0.0f;
+    auto read_row = [&](uint64_t row) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = (i * kWave * W + lane) * V;
-            px[i].load(x + (int64_t)row * x_stride + c, (int)cols - c);
-            pd[i].load(dy + (int64_t)row * dy_stride + c, (int)cols - c);
+            read(px[i], x + (int64_t)row * x_stride, i);
+            read(pd[i], dy + (int64_t)row * dy_stride, i);
         }
-        const float m = mean[row], r = rstd[row];
+        m = mean[row];
+        r = rstd[row];
+    };
+    int slot = 0;
+    const uint64_t step = (uint64_t)gridDim.x * G;
+    uint64_t row = (uint64_t)blockIdx.x * G + group;
+    if (row < rows) read_row(row);
+    for (; row < rows; row += step) {
+        float h[N * V], g[N * V];
         float sg = 0.0f, sgh = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = (i * kWave * W + lane) * V;
-            float w[V];
-            if (weight) load_f32(w, weight + c, (int)cols - c, 0.0f);
+            fix(px[i], i);
+            fix(pd[i], i);
+            const Floats<V> w = KEEP ? kept[KEEP ? i : 0] : weights(i);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
+                const int e = i * V + j;
                 // past the row's end dy is zero, and with it every sum's term
-                const float d = (float)pd[i].v[j], h = ((float)px[i].v[j] - m) * r;
-                const float g = weight ? d * w[j] : d;
-                sg += g;
-                sgh = fmaf(g, h, sgh);
-                dw[i * V + j] = fmaf(d, c + j < (int)cols ? h : 0.0f, dw[i * V + j]);
-                db[i * V + j] += d;
+                const float d = (float)pd[i].v[j];
+                h[e] = column(i) + j < (int)cols ? ((float)px[i].v[j] - m) * r : 0.0f;
+                g[e] = d * w[j];
+                sg += g[e];
+                sgh = fmaf(g[e], h[e], sgh);
+                dw[e] = fmaf(d, h[e], dw[e]);
+                db[e] += d;
             }
         }
+        const float scale = r;
+        // the next row's values are on their way while this one's sums are joined
+        const uint64_t next = row + step;
+        read_row(next < rows ? next : row);
         const float a = row_sum<W>(sg, part, slot) / (float)cols;
         const float b = row_sum<W>(sgh, part, slot + 1) / (float)cols;
         slot ^= 2;
+        T* to = dx + (int64_t)row * dx_stride;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int c = (i * kWave * W + lane) * V;
-            const int left = (int)cols - c;
-            if (left <= 0) break;
-            float w[V];
-            if (weight) load_f32(w, weight + c, left, 0.0f);
             Piece<T> out;
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float d = (float)pd[i].v[j], h = ((float)px[i].v[j] - m) * r;
-                const float g = weight ? d * w[j] : d;
-                out.v[j] = (T)((g - a - h * b) * r);
-            }
-            out.store(dx + (int64_t)row * dx_stride + c, left);
+            for (int j = 0; j < V; ++j) out.v[j] = (T)((g[i * V + j] - a - h[i * V + j] * b) * scale);
+            out.store(to + column(i), (int)cols - column(i));
         }
     }
     if (!partial) return;
@@ -204,12 +252,13 @@ __global__ __launch_bounds__(1024) void norm_param_grad_kernel(const float* __re
 }
 
 struct NormForm {
-    int waves, pieces;  // waves on a row and 16-byte pieces a lane
+    int waves, pieces;  // waves on a row and 16-byte pieces a lane (0: less than one)
 };
 
 // Rows wide enough for it, or too few to fill the GPU with a wave each, take
 // several waves.
 NormForm norm_form(uint64_t rows, uint32_t cols, int v) {
+    if (cols < (uint32_t)v) return {1, 0};
     const int most = kLaneValues / v;
     for (int w : {1, 4, 16}) {
         const int n = (int)ceil_div(cols, kWave * w * v);
@@ -222,29 +271,31 @@ NormForm norm_form(uint64_t rows, uint32_t cols, int v) {
 // Calls f with the form's constants.
 template <typename T, typename F>
 void with_form(NormForm form, F&& f) {
+    using std::integral_constant;
+    const std::false_type many;
     auto pieces = [&](auto w) {
-        constexpr int W = decltype(w)::value;
         switch (form.pieces) {
-            case 1: f(w, std::integral_constant<int, 1>{}); break;
-            case 2: f(w, std::integral_constant<int, 2>{}); break;
-            case 3: f(w, std::integral_constant<int, 3>{}); break;
-            case 4: f(w, std::integral_constant<int, 4>{}); break;
+            case 1: f(w, integral_constant<int, 1>{}, many); break;
+            case 2: f(w, integral_constant<int, 2>{}, many); break;
+            case 3: f(w, integral_constant<int, 3>{}, many); break;
+            case 4: f(w, integral_constant<int, 4>{}, many); break;
             default:
                 if constexpr (Piece<T>::V == 4) {
                     if (form.pieces == 6)
-                        f(w, std::integral_constant<int, 6>{});
+                        f(w, integral_constant<int, 6>{}, many);
                     else
-                        f(w, std::integral_constant<int, 8>{});
+                        f(w, integral_constant<int, 8>{}, many);
                 }
         }
-        (void)W;
     };
-    if (form.waves == 1)
-        pieces(std::integral_constant<int, 1>{});
+    if (form.pieces == 0)
+        f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, std::true_type{});
+    else if (form.waves == 1)
+        pieces(integral_constant<int, 1>{});
     else if (form.waves == 4)
-        pieces(std::integral_constant<int, 4>{});
+        pieces(integral_constant<int, 4>{});
     else
-        pieces(std::integral_constant<int, 16>{});
+        pieces(integral_constant<int, 16>{});
 }
 
 uint64_t partial_bytes(uint32_t cols) { return 4ull * kGradBlocks * 2 * cols; }
@@ -270,10 +321,10 @@ int32_t tatara_op_layer_norm_forward(const void* x, int64_t x_stride, const floa
     TATARA_REQUIRE_ALIGNED(y, elem_bytes(dtype));
     if (int32_t st = check_stream(stream)) return st;
     TATARA_FOR_DTYPE(dtype, {
-        with_form<T>(norm_form(rows, cols, Piece<T>::V), [&](auto w, auto n) {
+        with_form<T>(norm_form(rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
             constexpr int W = decltype(w)::value;
             constexpr int N = decltype(n)::value;
-            norm_forward_kernel<T, W, N><<<W == 1 ? ceil_div(rows, 4) : (uint32_t)rows, W == 16 ? 1024 : 256, 0,
+            norm_forward_kernel<T, W, N, decltype(few)::value><<<W == 1 ? ceil_div(rows, 4) : (uint32_t)rows, W == 16 ? 1024 : 256, 0,
                                            raw(stream)>>>(static_cast<const T*>(x), x_stride, weight, bias,
                                                           static_cast<T*>(y), y_stride, mean, rstd, rows, cols, eps);
         });
@@ -313,11 +364,11 @@ int32_t tatara_op_layer_norm_backward(const void* dy, int64_t dy_stride, const v
     uint32_t blocks = 0;
     if (rows) {
         TATARA_FOR_DTYPE(dtype, {
-            with_form<T>(norm_form(rows, cols, Piece<T>::V), [&](auto w, auto n) {
+            with_form<T>(norm_form(rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
                 constexpr int W = decltype(w)::value;
                 constexpr int N = decltype(n)::value;
-                blocks = (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, kGradBlocks);
-                norm_backward_kernel<T, W, N><<<blocks, W == 16 ? 1024 : 256, 0, raw(stream)>>>(
+                blocks = grad_blocks(W == 1 ? (rows + 3) / 4 : rows);
+                norm_backward_kernel<T, W, N, decltype(few)::value><<<blocks, W == 16 ? 1024 : 256, 0, raw(stream)>>>(
                     static_cast<const T*>(dy), dy_stride, static_cast<const T*>(x), x_stride, weight, mean, rstd,
                     static_cast<T*>(dx), dx_stride, partial, rows, cols);
             });

@@ -24,14 +24,20 @@ from . import _lib
 from ._lib import check
 
 DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
-# an operator's element type -> names of the array types that hold it
-_HELD = {
-    "f32": ("float32", "torch.float32"),
-    "f16": ("float16", "torch.float16"),
-    "bf16": ("torch.bfloat16", "uint16"),
-    "i32": ("int32", "torch.int32"),
-    "u8": ("uint8", "torch.uint8"),
-}
+# names of array types -> the element type that they hold
+_HOLDS = {"float32": "f32", "torch.float32": "f32", "float16": "f16", "torch.float16": "f16", "uint16": "bf16",
+          "torch.bfloat16": "bf16", "int32": "i32", "torch.int32": "i32", "uint8": "u8", "torch.uint8": "u8"}
+
+
+class _TypeNames(dict):
+    """Array type -> element type (None: no operator's), filled as types are met."""
+
+    def __missing__(self, array_type):
+        self[array_type] = name = _HOLDS.get(str(array_type))
+        return name
+
+
+_TYPE = _TypeNames()
 
 
 class _Workspace:
@@ -41,6 +47,8 @@ class _Workspace:
         p = C.c_void_p()
         check(_lib.load().tatara_malloc(C.byref(p), nbytes))
         self.ptr, self.nbytes = p.value, nbytes
+        check(_lib.load().tatara_memset(self.ptr, 0, min(nbytes, 4096)))  # counts that begin at zero
+        check(_lib.load().tatara_synchronize())  # before any stream's work
 
     def __del__(self):
         try:
@@ -57,60 +65,54 @@ def _dtype(dtype: str) -> int:
     return DTYPES[dtype]
 
 
-_HELD_TYPES: dict = {}  # array type -> the element types it can hold
-
-
-def _is(array_dtype, dtype: str) -> bool:
-    held = _HELD_TYPES.get(array_dtype)
-    if held is None:
-        name = str(array_dtype)
-        held = _HELD_TYPES[array_dtype] = frozenset(k for k, v in _HELD.items() if name in v)
-    return dtype in held
-
-
 def _wrong(name: str, x, shape, dtype: str):
     raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on the device with a contiguous last "
                      f"dimension, not {getattr(x, 'dtype', type(x).__name__)} {tuple(getattr(x, 'shape', ()))}")
 
 
-def _dense(name: str, x, shape: tuple, dtype: str):
-    """The address of a contiguous tensor of this shape."""
-    if x is None or tuple(x.shape) != shape or not _is(x.dtype, dtype):
+def _owned(name: str, x, shape: tuple, dtype: str) -> int:
+    """The address of a DeviceArray of this shape."""
+    if hasattr(x, "data_ptr") or not hasattr(x, "ptr") or tuple(x.shape) != shape or _TYPE[x.dtype] != dtype:
         _wrong(name, x, shape, dtype)
-    if hasattr(x, "data_ptr"):
-        if not x.is_cuda or not x.is_contiguous():
-            _wrong(name, x, shape, dtype)
-        return x.data_ptr()
     return x.ptr
+
+
+# The checks below are most of a small call's time on the host: each reads a
+# tensor's attributes once, and everything that is not a right tensor goes on to
+# _owned, which takes a DeviceArray and refuses the rest.
+
+def _dense(name: str, x, shape: tuple, dtype: str) -> int:
+    """The address of a contiguous tensor of this shape."""
+    try:
+        if x.shape == shape and _TYPE[x.dtype] == dtype and x.is_cuda and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        pass
+    return _owned(name, x, shape, dtype)
 
 
 def _rows(name: str, x, shape: tuple, dtype: str):
     """Address and row stride of a [rows, cols] tensor."""
-    if x is None or tuple(x.shape) != shape or not _is(x.dtype, dtype):
-        _wrong(name, x, shape, dtype)
-    if hasattr(x, "data_ptr"):
-        stride = x.stride()
-        if not x.is_cuda or (stride[1] != 1 and shape[1] > 1):
-            _wrong(name, x, shape, dtype)
-        # a single row's stride says nothing
-        return x.data_ptr(), stride[0] if shape[0] > 1 else shape[1]
-    return x.ptr, shape[1]
+    try:
+        if x.shape == shape and _TYPE[x.dtype] == dtype and x.is_cuda:
+            stride, one = x.stride()
+            if one == 1 or shape[1] == 1:
+                return x.data_ptr(), stride if shape[0] > 1 else shape[1]  # one row's stride says nothing
+    except AttributeError:
+        pass
+    return _owned(name, x, shape, dtype), shape[1]
 
 
 def _matrices(name: str, x, shape: tuple, dtype: str):
     """Address, row stride and matrix stride of a [batch, rows, cols] tensor."""
-    if x is None or tuple(x.shape) != shape or not _is(x.dtype, dtype):
-        _wrong(name, x, shape, dtype)
-    if hasattr(x, "data_ptr"):
-        stride = x.stride()
-        if not x.is_cuda or (stride[2] != 1 and shape[2] > 1):
-            _wrong(name, x, shape, dtype)
-        return x.data_ptr(), stride[1] if shape[1] > 1 else shape[2], stride[0]
-    return x.ptr, shape[2], shape[1] * shape[2]
-
-
-def _handle(stream):
-    return None if stream is None else stream.handle
+    try:
+        if x.shape == shape and _TYPE[x.dtype] == dtype and x.is_cuda:
+            batch, stride, one = x.stride()
+            if one == 1 or shape[2] == 1:
+                return x.data_ptr(), stride if shape[1] > 1 else shape[2], batch
+    except AttributeError:
+        pass
+    return _owned(name, x, shape, dtype), shape[2], shape[1] * shape[2]
 
 
 class LayerNorm:
@@ -129,37 +131,42 @@ class LayerNorm:
         self._lib = _lib.load()
         self._ws = None
 
-    def _param(self, name, x):
-        return None if x is None else _dense(name, x, (self.cols,), "f32")
-
     def forward(self, x, weight, bias, y, mean=None, rstd=None, stream=None) -> None:
         """Writes y, and mean and rstd [rows] for the backward pass if given."""
+        cols, dtype = self.cols, self.dtype
         rows = x.shape[0]
-        shape = (rows, self.cols)
-        xp, xs = _rows("x", x, shape, self.dtype)
-        yp, ys = _rows("y", y, shape, self.dtype)
-        check(self._lib.tatara_op_layer_norm_forward(
-            xp, xs, self._param("weight", weight), self._param("bias", bias), yp, ys,
-            None if mean is None else _dense("mean", mean, (rows,), "f32"),
-            None if rstd is None else _dense("rstd", rstd, (rows,), "f32"),
-            rows, self.cols, self.eps, self._code, _handle(stream)))
+        shape, vec, param = (rows, cols), (rows,), (cols,)
+        xp, xs = _rows("x", x, shape, dtype)
+        yp, ys = _rows("y", y, shape, dtype)
+        status = self._lib.tatara_op_layer_norm_forward(
+            xp, xs, None if weight is None else _dense("weight", weight, param, "f32"),
+            None if bias is None else _dense("bias", bias, param, "f32"), yp, ys,
+            None if mean is None else _dense("mean", mean, vec, "f32"),
+            None if rstd is None else _dense("rstd", rstd, vec, "f32"), rows, cols, self.eps, self._code,
+            None if stream is None else stream.handle)
+        if status:
+            check(status)
 
     def backward(self, dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, stream=None) -> None:
         """Writes dx, and the weight's and bias's gradients [cols] if given (overwritten)."""
+        cols, dtype = self.cols, self.dtype
         rows = x.shape[0]
-        shape = (rows, self.cols)
+        shape, vec, param = (rows, cols), (rows,), (cols,)
         if self._ws is None:
             n = C.c_uint64()
-            check(self._lib.tatara_op_layer_norm_backward_workspace(self.cols, C.byref(n)))
+            check(self._lib.tatara_op_layer_norm_backward_workspace(cols, C.byref(n)))
             self._ws = _Workspace(n.value)
-        dyp, dys = _rows("dy", dy, shape, self.dtype)
-        xp, xs = _rows("x", x, shape, self.dtype)
-        dxp, dxs = _rows("dx", dx, shape, self.dtype)
-        check(self._lib.tatara_op_layer_norm_backward(
-            dyp, dys, xp, xs, self._param("weight", weight), _dense("mean", mean, (rows,), "f32"),
-            _dense("rstd", rstd, (rows,), "f32"), dxp, dxs, self._param("dweight", dweight),
-            self._param("dbias", dbias), rows, self.cols, self._code, self._ws.ptr, self._ws.nbytes,
-            _handle(stream)))
+        dyp, dys = _rows("dy", dy, shape, dtype)
+        xp, xs = _rows("x", x, shape, dtype)
+        dxp, dxs = _rows("dx", dx, shape, dtype)
+        status = self._lib.tatara_op_layer_norm_backward(
+            dyp, dys, xp, xs, None if weight is None else _dense("weight", weight, param, "f32"),
+            _dense("mean", mean, vec, "f32"), _dense("rstd", rstd, vec, "f32"), dxp, dxs,
+            None if dweight is None else _dense("dweight", dweight, param, "f32"),
+            None if dbias is None else _dense("dbias", dbias, param, "f32"), rows, cols, self._code, self._ws.ptr,
+            self._ws.nbytes, None if stream is None else stream.handle)
+        if status:
+            check(status)
 
 
 class BucketGate:
@@ -197,7 +204,7 @@ class BucketGate:
             self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32"),
             _dense("gate", gate, chosen, "f32"), _dense("count", count, (self.buckets,), "i32"),
             _dense("prob_sum", prob_sum, (self.buckets,), "f32"), _dense("counted", counted, (1,), "i32"),
-            _dense("loss", loss, (1,), "f32"), self._ws.ptr, self._ws.nbytes, _handle(stream)))
+            _dense("loss", loss, (1,), "f32"), self._ws.ptr, self._ws.nbytes, None if stream is None else stream.handle))
 
     def backward(self, logits, bucket, count, counted, dlogits, dgate=None, dloss: float = 1.0, valid=None,
                  stream=None) -> None:
@@ -211,7 +218,7 @@ class BucketGate:
             lp, ls, None if valid is None else _dense("valid", valid, (n,), "u8"), n, self.buckets, self.top_k,
             self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32"),
             _dense("count", count, (self.buckets,), "i32"), _dense("counted", counted, (1,), "i32"),
-            None if dgate is None else _dense("dgate", dgate, chosen, "f32"), dloss, dp, ds, _handle(stream)))
+            None if dgate is None else _dense("dgate", dgate, chosen, "f32"), dloss, dp, ds, None if stream is None else stream.handle))
 
 
 class Orthogonaliser:
@@ -243,7 +250,7 @@ class Orthogonaliser:
         op, orow, ob = _matrices("out", out, self.shape, self.dtype)
         check(self._lib.tatara_op_orthogonalise(xp, xr, xb, op, orow, ob, self.batch, self.rows, self.cols,
                                                 self._code, self.steps, self._workspace(), self._bytes,
-                                                _handle(stream)))
+                                                None if stream is None else stream.handle))
 
 
 class Muon:
@@ -273,4 +280,4 @@ class Muon:
             _dense("weights", weights, shape, "f32"), _dense("momentum", momentum, shape, "f32"),
             _dense("grad", grad, shape, self.grad_dtype), o.batch, o.rows, o.cols, self._grad_code, self.beta,
             self.nesterov, lr, self.weight_decay, scale, self.min_w, self.max_w, o.steps, o._workspace(), o._bytes,
-            _handle(stream)))
+            None if stream is None else stream.handle))

@@ -939,8 +939,8 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
     }
 }
 
-template <int EPI, typename T, typename L, int P>
-void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
+template <int EPI, typename L>
+uint32_t count_tiles(ProductArgs& p) {
     p.tiles_m = ceil_div(p.m, L::BM);
     p.tiles_n = ceil_div(p.n, L::BN);
     p.tiles = p.tiles_m * p.tiles_n;
@@ -948,7 +948,33 @@ void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
         p.tiles = 0;
         for (uint32_t i = 0; i < p.tiles_m; ++i) p.tiles += p.tiles_n - i * L::BM / L::BN;
     }
-    muon_product_kernel<EPI, T, L, P><<<p.tiles * batch, L::THREADS, 0, stream>>>(p);
+    return p.tiles;
+}
+
+template <int EPI, typename T, typename L, int P>
+void launch_tiles(ProductArgs p, uint32_t batch, hipStream_t stream) {
+    const uint32_t tiles = count_tiles<EPI, L>(p);
+    muon_product_kernel<EPI, T, L, P><<<tiles * batch, L::THREADS, 0, stream>>>(p);
+}
+
+// Tiles of 128, two workgroups a CU that fill each other's waits, from two rounds
+// of the GPU's CUs on.  Below, tiles of 64, with two groups of waves for one
+// workgroup on a CU (5 of 320 x 448: 6.3 us against 12); two stages of them let a
+// second workgroup onto a CU (512 tiles, k 1024: 21 us against 25), three go further
+// where it would have nothing to do (136 tiles, k 2048: 19.5 against 21.7).
+template <int EPI, typename T, int P>
+void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
+    using Wide = Tile<128, 128, 2, 2, 32, 2>;
+    using Narrow = Tile<64, 64, 2, 2, 64, 2, 2>;
+    using Deep = Tile<64, 64, 2, 2, 64, 3, 2>;
+    constexpr uint64_t kCus = 256;
+    const uint64_t b = batch;
+    if (b * count_tiles<EPI, Wide>(p) >= 2 * kCus)
+        launch_tiles<EPI, T, Wide, P>(p, batch, stream);
+    else if (b * count_tiles<EPI, Narrow>(p) > kCus || p.k <= 512)
+        launch_tiles<EPI, T, Narrow, P>(p, batch, stream);
+    else
+        launch_tiles<EPI, T, Deep, P>(p, batch, stream);
 }
 
 struct Step {
@@ -957,18 +983,18 @@ struct Step {
     bool last;
 };
 
-template <typename T, typename L, int P>
+template <typename T, int P>
 void launch_step(const Step& s, const Source& from, const Target& t, uint32_t batch, hipStream_t stream) {
     ProductArgs p{};
     p.p = p.q = s.x;
     p.m = p.n = s.m;
     p.k = s.n;
     p.to = s.gram;
-    launch_product<kGram, T, L, P>(p, batch, stream);
+    launch_product<kGram, T, P>(p, batch, stream);
     p.p = p.q = p.old = s.gram;
     p.k = s.m;
     p.to = s.poly;
-    launch_product<kPoly, T, L, P>(p, batch, stream);
+    launch_product<kPoly, T, P>(p, batch, stream);
     p.p = s.poly;
     p.q = p.old = s.xt;
     p.n = s.n;
@@ -979,11 +1005,11 @@ void launch_step(const Step& s, const Source& from, const Target& t, uint32_t ba
     p.cols = from.cols;
     p.flipped = from.rows > from.cols;
     if (!s.last)
-        launch_product<kApply, T, L, P>(p, batch, stream);
+        launch_product<kApply, T, P>(p, batch, stream);
     else if (t.weights)
-        launch_product<kUpdate, T, L, P>(p, batch, stream);
+        launch_product<kUpdate, T, P>(p, batch, stream);
     else
-        launch_product<kOut, T, L, P>(p, batch, stream);
+        launch_product<kOut, T, P>(p, batch, stream);
 }
 
 uint32_t up(uint32_t n) { return (n + kPad - 1) / kPad * kPad; }
@@ -1056,13 +1082,7 @@ int32_t launch_small(const Source& s, const Target& t, uint32_t batch, uint32_t 
     return kOk;
 }
 
-// Tiles of 64 where those of 128 would leave CUs without work: a workgroup of the
-// smaller ones has two groups of waves, which keep loads, LDS reads and products
-// of different stages under way on a CU that holds one workgroup.
-using WideTile = Tile<128, 128, 2, 2, 32, 2>;
-using NarrowTile = Tile<64, 64, 2, 2, 64, 3, 2>;
-
-template <typename T, typename L>
+template <typename T>
 int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws, hipStream_t stream,
                         uint32_t rough) {
     const Layout l(batch, s.rows, s.cols);
@@ -1086,9 +1106,9 @@ int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32
         step.n = l.n;
         step.last = i + 1 == steps;
         if (i < rough)
-            launch_step<T, L, 1>(step, s, t, batch, stream);
+            launch_step<T, 1>(step, s, t, batch, stream);
         else
-            launch_step<T, L, 2>(step, s, t, batch, stream);
+            launch_step<T, 2>(step, s, t, batch, stream);
         TATARA_LAUNCHED("muon_product");
     }
     return kOk;
@@ -1113,10 +1133,8 @@ int32_t launch_steps(const Source& s, const Target& t, uint32_t batch, uint32_t 
     // its offsets within a matrix are of 32 bits
     const bool near = (uint64_t)s.rows * std::max(s.row_stride, t.row_stride) < (1u << 29);
     if (near && small_blocks(s.rows, s.cols)) return launch_small<T>(s, t, batch, steps, stream);
-    const uint64_t wide = (uint64_t)ceil_div(s.rows, 128) * ceil_div(s.cols, 128) * batch;
     const uint32_t rough = t.weights ? 0 : rough_steps<T>(steps, std::min(s.rows, s.cols));
-    return wide >= 512 ? launch_products<T, WideTile>(s, t, batch, steps, ws, stream, rough)
-                       : launch_products<T, NarrowTile>(s, t, batch, steps, ws, stream, rough);
+    return launch_products<T>(s, t, batch, steps, ws, stream, rough);
 }
 
 int32_t check_matrices(uint32_t batch, uint32_t rows, uint32_t cols, int32_t dtype) {

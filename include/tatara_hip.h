@@ -257,8 +257,8 @@ TATARA_API int32_t tatara_op_quantise_ft_noalloc(const float* w, uint64_t rows, 
  * buckets by learned scores, and Muon updates of its matrices.
  *
  * These calls queue their work on `stream` (NULL: the device's null stream) and
- * return; nothing is allocated and nothing waits, so they can be captured.  The
- * stream must be of the thread's current device.  Tensors are device memory;
+ * return; nothing is allocated and nothing waits.  The stream must be of the
+ * thread's current device.  Tensors are device memory;
  * `dtype` is the element type of the tensors that are void*, strides count
  * elements from one row (or matrix) to the next and rows may start at any
  * element.  Inputs and outputs must not overlap unless stated.  `workspace` has

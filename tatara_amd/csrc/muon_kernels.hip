@@ -34,14 +34,14 @@ using half8 = f16_t __attribute__((ext_vector_type(8)));
 using half4 = f16_t __attribute__((ext_vector_type(4)));
 using floatx16 = float __attribute__((ext_vector_type(16)));
 
-// Where a held matrix has the hi of (row, col); lo lies kLow further.  Two rows'
-// 32 columns of hi fill a 128-byte line, the next line has their lo: a stage's
-// loads take whole lines, also where they take hi alone.  Loads of half lines ran
-// at 22 to 27 bytes a clock and CU, of whole ones at 35.
+// Where a held matrix has the hi of (row, col); lo lies kLow further.  Four rows'
+// 16 columns of hi fill a 128-byte line, the next line has their lo: a stage's
+// loads take whole lines, also where they take hi alone or 16 columns.  Loads of
+// half lines ran at 22 to 27 bytes a clock and CU, of whole ones at 35.
 using Held = f16_t*;
 constexpr uint32_t kLow = 64;
 __device__ __forceinline__ uint64_t held_at(uint64_t row, uint32_t col, uint32_t cols) {
-    return ((row / 2) * (cols / 32) + col / 32) * 128 + row % 2 * 32 + col % 32;
+    return ((row / 4) * (cols / 16) + col / 16) * 128 + row % 4 * 16 + col % 16;
 }
 
 __device__ __forceinline__ void split(float v, f16_t& hi, f16_t& lo) {
@@ -601,25 +601,30 @@ struct ProductArgs {
 };
 
 // A workgroup's tile BM x BN of p q^T: WR x WC waves, KS values of k a stage, S
-// stages in LDS.  KG groups of such waves share a stage's values of k, and their
+// stages in LDS (KS 16 or more).  KG groups of such waves share a stage's values of k, and their
 // sums are joined in order.
 template <int BM_, int BN_, int WR_, int WC_, int KS_, int S_, int KG_ = 1>
 struct Tile {
     static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, KS = KS_, S = S_, KG = KG_;
     static constexpr int THREADS = KG * WR * WC * (int)kWave;
     static constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 blocks of a wave
-    // with P of hi and lo: 16-byte pieces of a row's stage, of the stage, and a thread's loads
-    static constexpr int pieces_row(int P) { return KS / 8 * P; }
-    static constexpr int pieces(int P) { return (BM + BN) * pieces_row(P); }
+    // with P of hi and lo: 16-byte pieces of the stage, and a thread's loads
+    static constexpr int pieces(int P) { return (BM + BN) * (KS / 8) * P; }
     static constexpr int loads(int P) { return pieces(P) / THREADS; }
     static_assert(pieces(1) % THREADS == 0, "every thread loads alike");
 };
 
-// Which piece of a row's stage lies at a place of it: rows that would share LDS
-// banks turn their pieces, so that 16 rows of one piece cover all of them.
-template <int CH>
-__device__ __forceinline__ uint32_t turn(uint32_t row, uint32_t piece) {
-    return piece ^ ((row / (16 / CH)) % CH);
+// A stage lies in LDS by blocks of 16 columns, in each the rows of p, then of q, four
+// rows' 8 P pieces together as they lie in memory (hi of the four rows, then lo).
+// Within those the place turns with the row, so that 16 rows of one piece cover all
+// of LDS's banks.
+template <int P>
+__device__ __forceinline__ uint32_t turn(uint32_t row) {
+    return P == 2 ? (row / 4 & 1) | (row / 4 & 2) << 2 : row / 8 & 1;
+}
+template <int P>
+__device__ __forceinline__ uint32_t place(uint32_t row, uint32_t low, uint32_t half) {
+    return row / 4 * (8 * P) + ((low * 8 + row % 4 * 2 + half) ^ turn<P>(row));
 }
 
 // 16 bytes a lane from global memory to LDS, the wave's 64 in a row from `to`.
@@ -709,10 +714,11 @@ struct Strip {
 // last product of the step instead of a I to B.
 template <int EPI, typename T, typename L, int P>
 __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a) {
-    constexpr int BM = L::BM, BN = L::BN, CH = L::pieces_row(P), TM = L::TM, TN = L::TN;
+    constexpr int BM = L::BM, BN = L::BN, TM = L::TM, TN = L::TN;
     constexpr int S = L::S, LOADS = L::loads(P);
-    constexpr int DOWN = Strip<L>::DOWN, OVER = Strip<L>::OVER, STAGE = L::pieces(P);
-    // the stages ([stage][rows of p, then of q: pieces]), then the groups' sums, then the strips
+    constexpr int DOWN = Strip<L>::DOWN, OVER = Strip<L>::OVER;
+    constexpr int STAGE = L::pieces(P), BLOCK = (BM + BN) * 2 * P;  // pieces, of a stage and of 16 columns
+    // the stages, then the groups' sums, then the strips
     constexpr int STAGES_BYTES = S * STAGE * 16, SUMS_BYTES = (L::KG - 1) * BM * BN * 4;
     constexpr int BYTES0 = STAGES_BYTES > SUMS_BYTES ? STAGES_BYTES : SUMS_BYTES;
     constexpr int BYTES = BYTES0 > Strip<L>::BYTES ? BYTES0 : Strip<L>::BYTES;
@@ -747,17 +753,17 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
     const f16_t* from[LOADS];
 #pragma unroll
     for (int s = 0; s < LOADS; ++s) {
-        const uint32_t e = s * L::THREADS + tid, row = e / CH, piece = turn<CH>(row, e % CH);
-        // pieces of 32 columns: four of hi, then (P = 2) four of lo
-        const uint32_t col = piece / (4 * P) * 32 + piece % 4 * 8;
+        const uint32_t e = s * L::THREADS + tid, at = e % BLOCK, four = at / (8 * P);
+        const uint32_t piece = at % (8 * P) ^ turn<P>(four * 4), row = four * 4 + piece % 8 / 2;
         // rows past the matrix (its side is a multiple of 64, not of the tile) are not stored
         const uint32_t r = row < BM ? min(i0 + row, a.m - 1) : min(j0 + row - BM, a.n - 1);
-        from[s] = (row < BM ? a.p + p_at : a.q + q_at) + held_at(r, col, a.k) + piece / 4 % P * kLow;
+        from[s] = (row < BM ? a.p + p_at : a.q + q_at) + held_at(r, e / BLOCK * 16 + piece % 2 * 8, a.k) +
+                  piece / 8 * kLow;
     }
     const uint32_t wave0 = __builtin_amdgcn_readfirstlane(tid / kWave) * kWave;
     auto fetch = [&](uint32_t stage, uint32_t k0) {
 #pragma unroll
-        for (int s = 0; s < LOADS; ++s) load_to_lds(from[s] + k0 * 4, &lds[stage * STAGE + s * L::THREADS + wave0]);
+        for (int s = 0; s < LOADS; ++s) load_to_lds(from[s] + k0 * 8, &lds[stage * STAGE + s * L::THREADS + wave0]);
     };
     const uint32_t stages = a.k / L::KS;
     for (uint32_t s = 0; s + 1 < S && s < stages; ++s) fetch(s, s * L::KS);
@@ -773,19 +779,19 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
         constexpr int STEPS = L::KS / 16 / L::KG;
         half8 fp[2][P][TM], fq[2][P][TN];  // [this, next][hi, lo][block]
         auto read = [&](int kk) {
-            const uint32_t at = kk * L::KG + group, piece = at / 2 * (4 * P) + at % 2 * 2 + lane / 32;
+            const half8* from_lds = lds + buf * STAGE + (kk * L::KG + group) * BLOCK;
 #pragma unroll
             for (int lo = 0; lo < P; ++lo) {
                 // in the order of the products below
 #pragma unroll
                 for (int x = 0; x < TM; ++x) {
                     const uint32_t row = wi + x * 32 + lane % 32;
-                    fp[kk % 2][P - 1 - lo][x] = lds[buf * STAGE + row * CH + turn<CH>(row, piece + (P - 1 - lo) * 4)];
+                    fp[kk % 2][P - 1 - lo][x] = from_lds[place<P>(row, P - 1 - lo, lane / 32)];
                 }
 #pragma unroll
                 for (int y = 0; y < TN; ++y) {
                     const uint32_t row = BM + wj + y * 32 + lane % 32;
-                    fq[kk % 2][lo][y] = lds[buf * STAGE + row * CH + turn<CH>(row, piece + lo * 4)];
+                    fq[kk % 2][lo][y] = from_lds[place<P>(row, lo, lane / 32)];
                 }
             }
         };
@@ -964,7 +970,7 @@ void launch_tiles(ProductArgs p, uint32_t batch, hipStream_t stream) {
 // where it would have nothing to do (136 tiles, k 2048: 19.5 against 21.7).
 template <int EPI, typename T, int P>
 void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
-    using Wide = Tile<128, 128, 2, 2, 32, 2>;
+    using Wide = Tile<128, 128, 2, 2, 16, 4>;
     using Narrow = Tile<64, 64, 2, 2, 64, 2, 2>;
     using Deep = Tile<64, 64, 2, 2, 64, 3, 2>;
     constexpr uint64_t kCus = 256;

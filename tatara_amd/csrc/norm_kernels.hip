@@ -25,6 +25,9 @@ uint32_t grad_blocks(uint64_t units) {
     return (uint32_t)std::min<uint64_t>(units, units >= 2048 ? kGradBlocks : kGradBlocks / 2);
 }
 
+// Workgroups of the forward pass at most: a launch has room for 2^32 threads.
+constexpr uint32_t kMaxGrid = 1u << 20;
+
 // Sum over the W waves of a row; `slot` alternates so that one barrier a sum is enough.
 template <int W>
 __device__ __forceinline__ float row_sum(float x, float (*part)[W], int slot) {
@@ -48,8 +51,6 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_forward_kernel(
     constexpr int V = Piece<T>::V;
     __shared__ float part[2][W];
     const uint32_t lane = threadIdx.x % (kWave * W);
-    const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x / (kWave * W)) + threadIdx.x / (kWave * W);
-    if (row >= rows) return;  // W > 1: one row a workgroup, so all of it returns
     auto column = [&](int i) { return (int)(i * kWave * W + lane) * V; };
     auto read = [&](auto& piece, const auto* from, int i) {
         if (FEW)
@@ -60,49 +61,54 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void norm_forward_kernel(
     auto fix = [&](auto& piece, int i) {
         if (!FEW) piece.fix((int)cols - column(i));
     };
-    Piece<T> in[N];
+    // more rows than the grid has room for are taken in turn
+    constexpr int G = W == 1 ? 4 : 1;
+    const uint64_t step = (uint64_t)gridDim.x * G;
+    for (uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / (kWave * W); row < rows; row += step) {
+        Piece<T> in[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) read(in[i], x + (int64_t)row * x_stride, i);
-    float s = 0.0f;
+        for (int i = 0; i < N; ++i) read(in[i], x + (int64_t)row * x_stride, i);
+        float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        fix(in[i], i);
+        for (int i = 0; i < N; ++i) {
+            fix(in[i], i);
 #pragma unroll
-        for (int j = 0; j < V; ++j) s += (float)in[i].v[j];
-    }
-    const float m = row_sum<W>(s, part, 0) / (float)cols;
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int left = (int)cols - column(i);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float d = j < left ? (float)in[i].v[j] - m : 0.0f;
-            s = fmaf(d, d, s);
+            for (int j = 0; j < V; ++j) s += (float)in[i].v[j];
         }
-    }
-    const float r = 1.0f / sqrtf(row_sum<W>(s, part, 1) / (float)cols + eps);
-    if (lane == 0) {
-        if (mean) mean[row] = m;
-        if (rstd) rstd[row] = r;
-    }
-    T* yr = y + (int64_t)row * y_stride;
+        const float m = row_sum<W>(s, part, 0) / (float)cols;
+        s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const int left = (int)cols - column(i);
-        if (left <= 0) break;
-        Floats<V> w, b;
-        if (weight) read(w, weight, i);
-        if (bias) read(b, bias, i);
-        if (weight) fix(w, i);
-        if (bias) fix(b, i);
-        Piece<T> out;
+        for (int i = 0; i < N; ++i) {
+            const int left = (int)cols - column(i);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float h = ((float)in[i].v[j] - m) * r;
-            out.v[j] = (T)fmaf(h, weight ? w[j] : 1.0f, bias ? b[j] : 0.0f);
+            for (int j = 0; j < V; ++j) {
+                const float d = j < left ? (float)in[i].v[j] - m : 0.0f;
+                s = fmaf(d, d, s);
+            }
         }
-        out.store(yr + column(i), left);
+        const float r = 1.0f / sqrtf(row_sum<W>(s, part, 1) / (float)cols + eps);
+        if (lane == 0) {
+            if (mean) mean[row] = m;
+            if (rstd) rstd[row] = r;
+        }
+        T* yr = y + (int64_t)row * y_stride;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int left = (int)cols - column(i);
+            if (left <= 0) break;
+            Floats<V> w, b;
+            if (weight) read(w, weight, i);
+            if (bias) read(b, bias, i);
+            if (weight) fix(w, i);
+            if (bias) fix(b, i);
+            Piece<T> out;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float h = ((float)in[i].v[j] - m) * r;
+                out.v[j] = (T)fmaf(h, weight ? w[j] : 1.0f, bias ? b[j] : 0.0f);
+            }
+            out.store(yr + column(i), left);
+        }
     }
 }
 
@@ -262,7 +268,7 @@ NormForm norm_form(uint64_t rows, uint32_t cols, int v) {
     const int most = kLaneValues / v;
     for (int w : {1, 4, 16}) {
         const int n = (int)ceil_div(cols, kWave * w * v);
-        if (n > most || (w == 1 && rows < 2048 && n > 1)) continue;
+        if (n > most || (w == 1 && rows < 1024 && n > 1)) continue;
         return {w, n == 5 ? 6 : n == 7 ? 8 : n};
     }
     return {16, most};
@@ -324,9 +330,10 @@ int32_t tatara_op_layer_norm_forward(const void* x, int64_t x_stride, const floa
         with_form<T>(norm_form(rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
             constexpr int W = decltype(w)::value;
             constexpr int N = decltype(n)::value;
-            norm_forward_kernel<T, W, N, decltype(few)::value><<<W == 1 ? ceil_div(rows, 4) : (uint32_t)rows, W == 16 ? 1024 : 256, 0,
-                                           raw(stream)>>>(static_cast<const T*>(x), x_stride, weight, bias,
-                                                          static_cast<T*>(y), y_stride, mean, rstd, rows, cols, eps);
+            const uint32_t blocks = (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, kMaxGrid);
+            norm_forward_kernel<T, W, N, decltype(few)::value><<<blocks, W == 16 ? 1024 : 256, 0, raw(stream)>>>(
+                static_cast<const T*>(x), x_stride, weight, bias, static_cast<T*>(y), y_stride, mean, rstd, rows,
+                cols, eps);
         });
     });
     TATARA_LAUNCHED("norm_forward");

@@ -148,6 +148,20 @@ def test_without_parameters_and_statistics(gpu):
     assert torch.equal(only, db)
 
 
+def test_more_rows_than_a_grid_holds(gpu):
+    """2^20 workgroups of four rows, and some."""
+    rows = 4 * (1 << 20) + 1003
+    x = torch.randn(rows, 5, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0))
+    y, mean = torch.empty_like(x), torch.empty(rows, device="cuda")
+    ops.LayerNorm(5).forward(x, None, None, y, mean)
+    x64 = x.double()
+    em = x64.mean(1, keepdim=True)
+    er = 1 / torch.sqrt(((x64 - em) ** 2).mean(1, keepdim=True) + 1e-5)
+    h = (x64 - em) * er
+    tol = 2.0**-24 * h.abs() + 64 * EPS32 * (x64.abs().mean(1, keepdim=True) * er + 2 * h.abs())
+    assert ((y.double() - h).abs() <= tol).all()
+
+
 def test_no_rows(gpu):
     ln = ops.LayerNorm(50)
     none, z = torch.empty(0, 50, device="cuda"), torch.empty(0, device="cuda")

@@ -7,7 +7,13 @@
 //             dw = sum_r dy h,  db = sum_r dy
 //
 // Every sum is f32 and in a fixed order (no atomics), so results do not change
-// from run to run.
+// from run to run.  The variance is of differences from the mean, which a row held
+// in registers gives without a second read.
+//
+// Both passes read and write each value once and are bound by memory: 65536 x 1536
+// take 153 us forward in f32 (5.3 TB/s; a copy of 2 GiB runs at 4.9) and 121 us
+// backward in bf16 (5.0 TB/s).  Small ones are bound by their launches: 6.4 us
+// forward, 9.8 backward (two launches) up to 512 x 1536.
 #include "elem.hpp"
 
 namespace tatara {
@@ -261,38 +267,52 @@ struct NormForm {
     int waves, pieces;  // waves on a row and 16-byte pieces a lane (0: less than one)
 };
 
-// Rows wide enough for it, or too few to fill the GPU with a wave each, take
-// several waves.
-NormForm norm_form(uint64_t rows, uint32_t cols, int v) {
+// 16-byte pieces that a lane holds with `waves` waves on a row, at most.  A wave
+// alone is fastest where a row's values leave it registers for the next row's: up
+// to 24 values a lane (40000 rows forward: 640 columns f32 34 us, with four waves
+// 42; 1536 bf16 47 and 56; but 2048 f32 134 and 125, bf16 79 and 77), 16 in the f32
+// backward pass (640: 57 and 80; 1536: 143 and 131).  Four waves go up to 32
+// (16384 x 8192 f32: 211, with sixteen 249), backward 24 (bf16: 180 and 163).
+constexpr int most_pieces(bool backward, int waves, int v) {
+    const int values = waves == 1 ? (backward && v == 4 ? 16 : 24) : waves == 4 && backward ? 24 : kLaneValues;
+    return values / v;
+}
+// Sixteen waves take what is too wide for four.
+constexpr int least_pieces(bool backward, int waves, int v) {
+    return waves == 16 ? most_pieces(backward, 4, v) / 4 + 1 : 1;
+}
+
+// Rows wide enough for it, or too few to fill the GPU with a wave each (backward,
+// 1009 x 1536 f32: 13.1 us with one, 10.5 with four; from 2048 rows on 13.0 and
+// 13.5), take several waves.
+NormForm norm_form(bool backward, uint64_t rows, uint32_t cols, int v) {
     if (cols < (uint32_t)v) return {1, 0};
-    const int most = kLaneValues / v;
-    for (int w : {1, 4, 16}) {
+    for (int w : {1, 4}) {
         const int n = (int)ceil_div(cols, kWave * w * v);
-        if (n > most || (w == 1 && rows < 1024 && n > 1)) continue;
+        if (n > most_pieces(backward, w, v) || (w == 1 && rows < 1024 && n > 1)) continue;
         return {w, n == 5 ? 6 : n == 7 ? 8 : n};
     }
-    return {16, most};
+    const int n = (int)ceil_div(cols, kWave * 16 * v);
+    return {16, n == 5 ? 6 : n == 7 ? 8 : n};
 }
 
 // Calls f with the form's constants.
-template <typename T, typename F>
+template <typename T, bool BACKWARD, typename F>
 void with_form(NormForm form, F&& f) {
     using std::integral_constant;
-    const std::false_type many;
     auto pieces = [&](auto w) {
-        switch (form.pieces) {
-            case 1: f(w, integral_constant<int, 1>{}, many); break;
-            case 2: f(w, integral_constant<int, 2>{}, many); break;
-            case 3: f(w, integral_constant<int, 3>{}, many); break;
-            case 4: f(w, integral_constant<int, 4>{}, many); break;
-            default:
-                if constexpr (Piece<T>::V == 4) {
-                    if (form.pieces == 6)
-                        f(w, integral_constant<int, 6>{}, many);
-                    else
-                        f(w, integral_constant<int, 8>{}, many);
-                }
-        }
+        constexpr int W = decltype(w)::value, V = Piece<T>::V;
+        auto is = [&](auto n) {
+            constexpr int N = decltype(n)::value;
+            if constexpr (N >= least_pieces(BACKWARD, W, V) && N <= most_pieces(BACKWARD, W, V))
+                if (form.pieces == N) f(w, n, std::false_type{});
+        };
+        is(integral_constant<int, 1>{});
+        is(integral_constant<int, 2>{});
+        is(integral_constant<int, 3>{});
+        is(integral_constant<int, 4>{});
+        is(integral_constant<int, 6>{});
+        is(integral_constant<int, 8>{});
     };
     if (form.pieces == 0)
         f(integral_constant<int, 1>{}, integral_constant<int, 1>{}, std::true_type{});
@@ -327,7 +347,7 @@ int32_t tatara_op_layer_norm_forward(const void* x, int64_t x_stride, const floa
     TATARA_REQUIRE_ALIGNED(y, elem_bytes(dtype));
     if (int32_t st = check_stream(stream)) return st;
     TATARA_FOR_DTYPE(dtype, {
-        with_form<T>(norm_form(rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
+        with_form<T, false>(norm_form(false, rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
             constexpr int W = decltype(w)::value;
             constexpr int N = decltype(n)::value;
             const uint32_t blocks = (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, kMaxGrid);
@@ -371,7 +391,7 @@ int32_t tatara_op_layer_norm_backward(const void* dy, int64_t dy_stride, const v
     uint32_t blocks = 0;
     if (rows) {
         TATARA_FOR_DTYPE(dtype, {
-            with_form<T>(norm_form(rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
+            with_form<T, true>(norm_form(true, rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
                 constexpr int W = decltype(w)::value;
                 constexpr int N = decltype(n)::value;
                 blocks = grad_blocks(W == 1 ? (rows + 3) / 4 : rows);

@@ -21,6 +21,8 @@ EPS32 = 2.0**-24
 
 SHAPES = [(1, 1), (1, 1536), (3, 7), (5, 64), (2, 65), (70, 256), (33, 257), (9, 770), (2100, 96), (2049, 513),
           (4, 2049), (3, 4100), (2, 8193), (2, 32768), (2050, 2048)]
+# either side of the widths where more waves share a row
+SHAPES += [(1100, 1024), (1100, 1025), (1100, 1536), (1100, 1537), (3, 6144), (3, 6145), (3, 7000), (2, 8192), (2, 16385)]
 
 
 def rows_of(g, rows, cols, pad, dtype, scale=1.0, shift=0.0):

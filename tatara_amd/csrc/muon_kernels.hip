@@ -44,10 +44,18 @@ __device__ __forceinline__ uint64_t held_at(uint64_t row, uint32_t col, uint32_t
     return ((row / 4) * (cols / 16) + col / 16) * 128 + row % 4 * 16 + col % 16;
 }
 
+// v less an f16 number, in one instruction of both widths: the factor is hidden from
+// the compiler, which would widen the number and subtract.
+__device__ __forceinline__ float less(float v, f16_t h) {
+    float minus = -1.0f;
+    asm("" : "+s"(minus));
+    return fmaf((float)h, minus, v);
+}
+
 __device__ __forceinline__ void split(float v, f16_t& hi, f16_t& lo) {
     const float s = v * kHeld;
     hi = (f16_t)s;
-    lo = (f16_t)(s - (float)hi);
+    lo = (f16_t)less(s, hi);
 }
 
 // Where a step's U comes from: a gradient alone, or a gradient and the
@@ -126,7 +134,8 @@ __device__ __forceinline__ double block_sum(double x, double (&join)[256 / kWave
 }
 
 // Adds the gradient to the momentum and leaves partial sums of |U|^2.  Squares
-// are summed in 64 bits: no gradient's size overflows or vanishes.
+// are summed in 64 bits: no gradient's size overflows or vanishes.  Bound by memory:
+// 45 of 1629 x 1536 f32 (1.35 GB read and written) 0.23 ms.
 template <typename T>
 __global__ __launch_bounds__(256) void muon_moment_kernel(Source s, double* __restrict__ parts) {
     __shared__ double join[256 / kWave];
@@ -144,7 +153,9 @@ __global__ __launch_bounds__(256) void muon_moment_kernel(Source s, double* __re
     if (threadIdx.x == 0) parts[(uint64_t)b * kNormParts + blockIdx.x] = sum;
 }
 
-// Writes X_0 as U lies (straight, [rows up][cols up]) and transposed, 64 x 64 a workgroup.
+// Writes X_0 as U lies (straight, [rows up][cols up]) and transposed, 64 x 64 a
+// workgroup.  U is formed again from gradient and momentum, which costs no more than
+// to have kept it.  Bound by memory: 45 of 1629 x 1536 f32 (1.82 GB) 0.35 ms.
 template <typename T>
 __global__ __launch_bounds__(256) void muon_split_kernel(Source s, const double* __restrict__ parts, uint32_t n_parts,
                                                          Held straight, Held turned, uint32_t rows_up,
@@ -230,11 +241,10 @@ __device__ __forceinline__ Halves split_held(const floatx4& v) {
     h.hi = to_halves(v);
     floatx4 rest;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) rest[r] = fmaf((float)h.hi[r], -1.0f, v[r]);
+    for (int r = 0; r < 4; ++r) rest[r] = less(v[r], h.hi[r]);
     h.lo = to_halves(rest);
     return h;
 }
-__device__ __forceinline__ Halves split4(const floatx4& v) { return split_held(v * kHeld); }
 
 __device__ __forceinline__ half8 join8(const half4& a, const half4& b) {
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -305,13 +315,16 @@ __device__ __forceinline__ void store4(V* base, uint32_t uniform, uint32_t lane,
 // right operand, so B X needs no rearrangement; X X^T takes the blocks
 // transposed, which a product with the identity gives (exactly: one term a sum).
 // Each wave sums X X^T over its columns, the workgroup adds the waves' sums in
-// order.
+// order.  One launch and one CU a matrix: 9 of 16 x 1536 take 20.4 us, five steps of
+// 2.6 us, each bound by the issue of its conversions and products (270 instructions
+// a wave, four waves a SIMD).
 template <int MB, int NT, typename T>
 __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, uint32_t steps) {
     constexpr int NB = MB * (MB + 1) / 2, CHUNK = NB < 4 ? NB : 4, PITCH = MB * 16 + 4;
     __shared__ __align__(16) float gram[MB * 16][PITCH];
     __shared__ __align__(16) f16_t poly_hi[MB * 16][PITCH], poly_lo[MB * 16][PITCH];
-    __shared__ floatx4 parts[16][CHUNK][kWave];
+    // one more, so that four waves' sums that are read together lie in different banks
+    __shared__ floatx4 parts[16][CHUNK * kWave + 1];
     __shared__ double join[16];
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
     const uint32_t col = lane % 16, row4 = lane / 16 * 4;
@@ -335,7 +348,10 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
     // same for all its blocks, the rest the same for all lanes.
     const uint32_t my_row = lane / 4, my_col = lane % 4 * 4;
     auto moved = [&](int slot, const Halves& h, uint32_t from, uint32_t to) {
-        half8* at = reinterpret_cast<half8*>(parts[wave][slot % CHUNK]);
+        half8* at = reinterpret_cast<half8*>(parts[wave] + slot % CHUNK * kWave);
+        // 16 columns' pieces lie 64 bytes apart; turned, they cover all banks
+        from ^= from / 16;
+        to ^= to / 16;
         at[from] = join8(h.hi, h.lo);
         __builtin_amdgcn_wave_barrier();
         const half8 v = at[to];
@@ -471,7 +487,7 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
         for (int k0 = 0; k0 < NB; k0 += CHUNK) {
 #pragma unroll
             for (int k = 0; k < CHUNK; ++k)
-                if (k0 + k < NB) parts[wave][k][lane] = acc[k0 + k];
+                if (k0 + k < NB) parts[wave][k * kWave + lane] = acc[k0 + k];
             __syncthreads();
             const uint32_t have = (NB - k0 < CHUNK ? NB - k0 : CHUNK) * 256;
             // four lanes an element, four waves' sums a lane
@@ -483,7 +499,7 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
                     v += w0 + i < waves ? reinterpret_cast<const float*>(parts[w0 + i])[e] : 0.0f;
                 v += __shfl_xor(v, 1);
                 v += __shfl_xor(v, 2);
-                v *= kProduct;
+                v *= kUnheld;  // with its factor
                 if (w0) continue;
                 uint32_t k = k0 + e / 256, ib = 0;
                 while (k >= MB - ib) k -= MB - ib, ++ib;
@@ -499,12 +515,12 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
             floatx4 v = zero;
 #pragma unroll
             for (int kb = 0; kb < MB; ++kb)
-                v = product(split4(*reinterpret_cast<const floatx4*>(&gram[ib * 16 + col][kb * 16 + row4])),
-                            split4(*reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][kb * 16 + row4])), v);
+                v = product(split_held(*reinterpret_cast<const floatx4*>(&gram[ib * 16 + col][kb * 16 + row4])),
+                            split_held(*reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][kb * 16 + row4])), v);
             const floatx4 old = *reinterpret_cast<const floatx4*>(&gram[jb * 16 + col][ib * 16 + row4]);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                v[r] = fmaf(kC, v[r] * kProduct, fmaf(kB, old[r], ib == jb && row4 + r == col ? kA : 0.0f));
+                v[r] = fmaf(kC * kProduct, v[r], fmaf(kB * kUnheld, old[r], ib == jb && row4 + r == col ? kA : 0.0f));
             // without the factor, so that B X has X's: of B's entries, up to 3.45, no
             // more than 2^-25 is lost to f16's smallest numbers
             return split_held(v);
@@ -712,6 +728,12 @@ struct Strip {
 
 // P = 2: hi hi + hi lo + lo hi;  P = 1: hi hi alone, with a X added in f32 to the
 // last product of the step instead of a I to B.
+//
+// 45 of 1629 x 1536 f32, a step: X X^T 0.60 ms, B 0.58, B X 1.15 (1.31 into the
+// weights), 930 TFLOP/s of f16 products in tiles of 128.  There the card's power is
+// the bound: matrix cores are busy in 57% of cycles at a clock of about 1.6 GHz,
+// tiles of 256 x 256 and 256 x 128 reach the same rate.  Small ones are bound by
+// latency: 6 to 8 us a launch (5 of 257 x 391).
 template <int EPI, typename T, typename L, int P>
 __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a) {
     constexpr int BM = L::BM, BN = L::BN, TM = L::TM, TN = L::TN;
@@ -1047,7 +1069,9 @@ struct Layout {
 Held held(void* ws, uint64_t offset) { return reinterpret_cast<Held>(static_cast<uint8_t*>(ws) + offset); }
 
 // Columns of blocks that a wave of muon_small_kernel holds, 0 where a workgroup
-// cannot hold the matrix: twelve blocks a wave are 48 of its 128 registers.
+// cannot hold the matrix: twelve blocks a wave are 48 of its 128 registers.  What it
+// can hold is faster there (one of 16 x 1536: 17 us, by products 106; 32 x 1536 38
+// and 107; 64 x 768 74 and 82).
 uint32_t small_blocks(uint32_t rows, uint32_t cols) {
     const uint32_t mb = ceil_div(std::min(rows, cols), 16), nt = ceil_div(std::max(rows, cols), 256);
     if (mb > 4 || nt * mb > 12) return 0;

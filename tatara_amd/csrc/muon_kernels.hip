@@ -315,18 +315,22 @@ __device__ __forceinline__ void store4(V* base, uint32_t uniform, uint32_t lane,
 // right operand, so B X needs no rearrangement; X X^T takes the blocks
 // transposed, which a product with the identity gives (exactly: one term a sum).
 // Each wave sums X X^T over its columns, the workgroup adds the waves' sums in
-// order.  One launch and one CU a matrix: 9 of 16 x 1536 take 20.4 us, five steps of
-// 2.6 us, each bound by the issue of its conversions and products (270 instructions
+// order.  One launch and one CU a matrix: 9 of 16 x 1536 take 19.2 us, five steps of
+// 2.4 us, each bound by the issue of its conversions and products (270 instructions
 // a wave, four waves a SIMD).
+// All 16 waves also where columns do not fill them: they share the sums and B (16 x 16:
+// 8 us, with one wave 22; 64 x 64: 38, with four 75).
+constexpr uint32_t kSmallWaves = 16;
 template <int MB, int NT, typename T>
-__global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, uint32_t steps) {
+__global__ __launch_bounds__(kSmallWaves* kWave) void muon_small_kernel(Source s, Target t, uint32_t steps) {
+    constexpr uint32_t waves = kSmallWaves;
     constexpr int NB = MB * (MB + 1) / 2, CHUNK = NB < 4 ? NB : 4, PITCH = MB * 16 + 4;
     __shared__ __align__(16) float gram[MB * 16][PITCH];
     __shared__ __align__(16) f16_t poly_hi[MB * 16][PITCH], poly_lo[MB * 16][PITCH];
     // one more, so that four waves' sums that are read together lie in different banks
-    __shared__ floatx4 parts[16][CHUNK * kWave + 1];
-    __shared__ double join[16];
-    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
+    __shared__ floatx4 parts[waves][CHUNK * kWave + 1];
+    __shared__ double join[waves];
+    const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const uint32_t col = lane % 16, row4 = lane / 16 * 4;
     const bool flipped = s.rows > s.cols;
     const uint32_t m = flipped ? s.cols : s.rows, n = flipped ? s.rows : s.cols, b = blockIdx.x;
@@ -436,7 +440,7 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
     __syncthreads();
     sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += (uint32_t)i < waves ? join[i] : 0.0;
+    for (int i = 0; i < (int)waves; ++i) sum += join[i];
     const Inverse inv(sum);
     // X as it is held; its f32 values only pass through
     Halves x[MB][NT];
@@ -491,12 +495,12 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
             __syncthreads();
             const uint32_t have = (NB - k0 < CHUNK ? NB - k0 : CHUNK) * 256;
             // four lanes an element, four waves' sums a lane
-            for (uint32_t q = threadIdx.x; q < have * 4; q += blockDim.x) {
+            for (uint32_t q = threadIdx.x; q < have * 4; q += waves * kWave) {
                 const uint32_t e = q / 4, w0 = q % 4 * 4;
                 float v = 0.0f;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; ++i)
-                    v += w0 + i < waves ? reinterpret_cast<const float*>(parts[w0 + i])[e] : 0.0f;
+                    v += reinterpret_cast<const float*>(parts[w0 + i])[e];
                 v += __shfl_xor(v, 1);
                 v += __shfl_xor(v, 2);
                 v *= kUnheld;  // with its factor
@@ -531,8 +535,8 @@ __global__ __launch_bounds__(1024) void muon_small_kernel(Source s, Target t, ui
         if constexpr (MB == 1) {
             only = poly(0, 0);
         } else {
-            for (uint32_t k = wave; k < MB * MB; k += waves) {
-                const uint32_t ib = k / MB, jb = k % MB;
+            if (wave < MB * MB) {
+                const uint32_t ib = wave / MB, jb = wave % MB;
                 const Halves h = poly(ib, jb);
                 *reinterpret_cast<half4*>(&poly_hi[jb * 16 + col][ib * 16 + row4]) = h.hi;
                 *reinterpret_cast<half4*>(&poly_lo[jb * 16 + col][ib * 16 + row4]) = h.lo;
@@ -987,22 +991,31 @@ void launch_tiles(ProductArgs p, uint32_t batch, hipStream_t stream) {
 
 // Tiles of 128, two workgroups a CU that fill each other's waits, from two rounds
 // of the GPU's CUs on.  Below, tiles of 64, with two groups of waves for one
-// workgroup on a CU (5 of 320 x 448: 6.3 us against 12); two stages of them let a
-// second workgroup onto a CU (512 tiles, k 1024: 21 us against 25), three go further
-// where it would have nothing to do (136 tiles, k 2048: 19.5 against 21.7).
+// workgroup on a CU; two stages of them let a second workgroup onto a CU (30 of 200
+// x 200: 130 us, three stages 163), three go further where it would have nothing to
+// do (3 of 512 x 512: 142, two 150).  What bounds such a product is what a CU's loads
+// bring to LDS, so where CUs are left over the tiles are of 64 x 32 (3 of 512 x 512:
+// 137) and 32 x 32, four groups of waves and four stages (512 x 512: 102, tiles of 64
+// 127; 257 x 391: 82 and 103; 3 of 512 x 512 139).
 template <int EPI, typename T, int P>
 void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
     using Wide = Tile<128, 128, 2, 2, 16, 4>;
     using Narrow = Tile<64, 64, 2, 2, 64, 2, 2>;
     using Deep = Tile<64, 64, 2, 2, 64, 3, 2>;
+    using Half = Tile<64, 32, 2, 1, 64, 3, 2>;
+    using Tiny = Tile<32, 32, 1, 1, 64, 4, 4>;
     constexpr uint64_t kCus = 256;
-    const uint64_t b = batch;
-    if (b * count_tiles<EPI, Wide>(p) >= 2 * kCus)
+    const uint64_t narrow = (uint64_t)batch * count_tiles<EPI, Narrow>(p);
+    if ((uint64_t)batch * count_tiles<EPI, Wide>(p) >= 2 * kCus)
         launch_tiles<EPI, T, Wide, P>(p, batch, stream);
-    else if (b * count_tiles<EPI, Narrow>(p) > kCus || p.k <= 512)
+    else if (narrow > kCus)
         launch_tiles<EPI, T, Narrow, P>(p, batch, stream);
-    else
+    else if (narrow > kCus / 2)
         launch_tiles<EPI, T, Deep, P>(p, batch, stream);
+    else if (narrow > kCus * 3 / 8)
+        launch_tiles<EPI, T, Half, P>(p, batch, stream);
+    else
+        launch_tiles<EPI, T, Tiny, P>(p, batch, stream);
 }
 
 struct Step {
@@ -1070,8 +1083,8 @@ Held held(void* ws, uint64_t offset) { return reinterpret_cast<Held>(static_cast
 
 // Columns of blocks that a wave of muon_small_kernel holds, 0 where a workgroup
 // cannot hold the matrix: twelve blocks a wave are 48 of its 128 registers.  What it
-// can hold is faster there (one of 16 x 1536: 17 us, by products 106; 32 x 1536 38
-// and 107; 64 x 768 74 and 82).
+// can hold is faster there (one of 16 x 1536: 16 us, by products 82; 32 x 1536 38
+// and 82; 64 x 512 53 and 66) or as fast on one CU (64 x 768: 73 and 70).
 uint32_t small_blocks(uint32_t rows, uint32_t cols) {
     const uint32_t mb = ceil_div(std::min(rows, cols), 16), nt = ceil_div(std::max(rows, cols), 256);
     if (mb > 4 || nt * mb > 12) return 0;
@@ -1083,9 +1096,8 @@ uint32_t small_blocks(uint32_t rows, uint32_t cols) {
 template <typename T>
 int32_t launch_small(const Source& s, const Target& t, uint32_t batch, uint32_t steps, hipStream_t stream) {
     const uint32_t mb = ceil_div(std::min(s.rows, s.cols), 16), nt = small_blocks(s.rows, s.cols);
-    const uint32_t threads = std::min<uint32_t>(16, ceil_div(std::max(s.rows, s.cols), 16)) * kWave;
     auto go = [&](auto m, auto n) {
-        muon_small_kernel<decltype(m)::value, decltype(n)::value, T><<<batch, threads, 0, stream>>>(s, t, steps);
+        muon_small_kernel<decltype(m)::value, decltype(n)::value, T><<<batch, kSmallWaves * kWave, 0, stream>>>(s, t, steps);
     };
     auto with_columns = [&](auto m) {
         constexpr int MB = decltype(m)::value;

@@ -50,6 +50,9 @@ def matrices(batch, rows, cols, seed, low_rank=False):
 
 SHAPES = [(1, 1, 1), (3, 1, 5), (2, 5, 1), (9, 32, 30), (9, 8, 768), (2, 16, 1536), (1, 64, 64), (2, 65, 64),
           (1, 100, 300), (3, 300, 100), (1, 128, 129), (2, 193, 257), (1, 512, 32), (1, 520, 390), (7, 33, 1000)]
+# batches that take each size of a product's tiles, upright and lying
+TILES = [(14, 150, 130), (18, 130, 150), (25, 130, 150), (60, 150, 130), (300, 140, 150), (300, 150, 140)]
+SHAPES += TILES
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
@@ -115,7 +118,7 @@ def test_zeros_sizes_and_special_values(gpu):
 
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("nesterov", [True, False])
-@pytest.mark.parametrize("batch,rows,cols", [(9, 16, 200), (1, 96, 32), (2, 130, 140)])
+@pytest.mark.parametrize("batch,rows,cols", [(9, 16, 200), (1, 96, 32), (2, 130, 140)] + TILES[:5])
 def test_muon_steps(gpu, batch, rows, cols, nesterov, dtype):
     w = 0.05 * torch.randn(batch, rows, cols, generator=torch.Generator().manual_seed(0))
     m = torch.zeros(batch, rows, cols)

@@ -17,6 +17,7 @@
 // the result.  Errors against 64-bit steps are those of f32 products (1e-6 to
 // 1e-5 of |X|, from the sums' rounding).
 #include "elem.hpp"
+#include "muon_tiles.hpp"
 
 namespace tatara {
 namespace {
@@ -620,20 +621,6 @@ struct ProductArgs {
     int32_t flipped;
 };
 
-// A workgroup's tile BM x BN of p q^T: WR x WC waves, KS values of k a stage, S
-// stages in LDS (KS 16 or more).  KG groups of such waves share a stage's values of k, and their
-// sums are joined in order.
-template <int BM_, int BN_, int WR_, int WC_, int KS_, int S_, int KG_ = 1>
-struct Tile {
-    static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, KS = KS_, S = S_, KG = KG_;
-    static constexpr int THREADS = KG * WR * WC * (int)kWave;
-    static constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 blocks of a wave
-    // with P of hi and lo: 16-byte pieces of the stage, and a thread's loads
-    static constexpr int pieces(int P) { return (BM + BN) * (KS / 8) * P; }
-    static constexpr int loads(int P) { return pieces(P) / THREADS; }
-    static_assert(pieces(1) % THREADS == 0, "every thread loads alike");
-};
-
 // A stage lies in LDS by blocks of 16 columns, in each the rows of p, then of q, four
 // rows' 8 P pieces together as they lie in memory (hi of the four rows, then lo).
 // Within those the place turns with the row, so that 16 rows of one piece cover all
@@ -665,13 +652,9 @@ __device__ __forceinline__ void arrive() {
 // A wave's strip of 32 rows in LDS, f32: filled from MFMA results, read in rows.
 template <typename L>
 struct Strip {
-    static constexpr int DOWN = L::TM < 2 ? L::TM : 2, OVER = L::TN < 2 ? L::TN : 2;  // blocks of a strip
-    static constexpr int PITCH = (DOWN > OVER ? DOWN : OVER) * 32 + 4;
-    static constexpr int BYTES = (int)sizeof(float) * 32 * PITCH * L::WR * L::WC;
+    static constexpr int PITCH = StripShape<L>::PITCH;
     float* base;
     uint32_t lane;
-    __device__ __forceinline__ Strip(void* lds, uint32_t wave, uint32_t lane_)
-        : base(static_cast<float*>(lds) + wave * 32 * PITCH), lane(lane_) {}
 
     // block t of the strip, its rows along the strip's
     __device__ __forceinline__ void put_along(const floatx16& v, int t) const {
@@ -742,13 +725,10 @@ template <int EPI, typename T, typename L, int P>
 __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a) {
     constexpr int BM = L::BM, BN = L::BN, TM = L::TM, TN = L::TN;
     constexpr int S = L::S, LOADS = L::loads(P);
-    constexpr int DOWN = Strip<L>::DOWN, OVER = Strip<L>::OVER;
+    constexpr int DOWN = StripShape<L>::DOWN, OVER = StripShape<L>::OVER;
     constexpr int STAGE = L::pieces(P), BLOCK = (BM + BN) * 2 * P;  // pieces, of a stage and of 16 columns
-    // the stages, then the groups' sums, then the strips
-    constexpr int STAGES_BYTES = S * STAGE * 16, SUMS_BYTES = (L::KG - 1) * BM * BN * 4;
-    constexpr int BYTES0 = STAGES_BYTES > SUMS_BYTES ? STAGES_BYTES : SUMS_BYTES;
-    constexpr int BYTES = BYTES0 > Strip<L>::BYTES ? BYTES0 : Strip<L>::BYTES;
-    __shared__ half8 lds[BYTES / 16];
+    using Lds = ProductLds<L, P>;
+    __shared__ half8 lds[Lds::BYTES / 16];
     // neighbouring tiles on one XCD, so that its L2 holds the panels they share
     const uint32_t bid = xcd_swizzle(blockIdx.x, gridDim.x);
     const uint32_t b = bid / a.tiles, at = bid % a.tiles;
@@ -843,7 +823,6 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
     arrive<0>();
     if constexpr (L::KG > 1) {
         floatx4* sums = reinterpret_cast<floatx4*>(lds);
-        constexpr int WAVES = L::WR * L::WC, QUADS = TM * TN * 4;
         if (group > 0) {
 #pragma unroll
             for (int x = 0; x < TM; ++x)
@@ -851,11 +830,11 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
                 for (int y = 0; y < TN; ++y)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        sums[(((group - 1) * WAVES + wave) * QUADS + (x * TN + y) * 4 + q) * kWave + lane] =
+                        sums[Lds::sum(group, wave, (x * TN + y) * 4 + q, lane)] =
                             floatx4{acc[x][y][q * 4], acc[x][y][q * 4 + 1], acc[x][y][q * 4 + 2], acc[x][y][q * 4 + 3]};
         }
         __syncthreads();
-        if (group > 0) return;  // no barrier follows
+        if (group > 0) return;  // no barrier follows: a wave's strip holds none of the sums
 #pragma unroll
         for (int x = 0; x < TM; ++x)
 #pragma unroll
@@ -863,13 +842,13 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
 #pragma unroll
-                    for (int o = 0; o < L::KG - 1; ++o) {
-                        const floatx4 v = sums[((o * WAVES + wave) * QUADS + (x * TN + y) * 4 + q) * kWave + lane];
+                    for (int o = 1; o < L::KG; ++o) {
+                        const floatx4 v = sums[Lds::sum(o, wave, (x * TN + y) * 4 + q, lane)];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[x][y][q * 4 + r] += v[r];
                     }
     }
-    const Strip<L> strip{lds, wave, lane};
+    const Strip<L> strip{reinterpret_cast<float*>(lds) + Lds::strip(wave) / 4, lane};
     const uint64_t first = 2ull * b * a.m * a.n;
 #pragma unroll
     for (int x = 0; x < TM; ++x) {
@@ -999,11 +978,6 @@ void launch_tiles(ProductArgs p, uint32_t batch, hipStream_t stream) {
 // 127; 257 x 391: 82 and 103; 3 of 512 x 512 139).
 template <int EPI, typename T, int P>
 void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
-    using Wide = Tile<128, 128, 2, 2, 16, 4>;
-    using Narrow = Tile<64, 64, 2, 2, 64, 2, 2>;
-    using Deep = Tile<64, 64, 2, 2, 64, 3, 2>;
-    using Half = Tile<64, 32, 2, 1, 64, 3, 2>;
-    using Tiny = Tile<32, 32, 1, 1, 64, 4, 4>;
     constexpr uint64_t kCus = 256;
     const uint64_t narrow = (uint64_t)batch * count_tiles<EPI, Narrow>(p);
     if ((uint64_t)batch * count_tiles<EPI, Wide>(p) >= 2 * kCus)

@@ -1130,18 +1130,21 @@ int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32
     return kOk;
 }
 
-// First steps that multiply hi parts alone (11 bits; X itself keeps its 22).  Their
-// rounding is an error of X that later steps see as part of X: the steps that
-// follow in full move it along with the rest, so it fades.  Five steps end with an
-// error of X, from the products, of 2e-3 to 4e-3 (none full), 2e-4 to 3e-3 (two,
-// the less the larger the matrix: up to 8e-4 from a short side of 256 on) or 3e-5
-// to 7e-4 (three).  A result of 16 bits is rounded to 1.7e-3 (bf16) or 2e-4 (f16),
-// so bf16 takes two full steps from 256 on and three below, f16 three: 9 or 11
-// products of 15.  f32 results take full products throughout.
+// First steps of a bf16 result that multiply hi parts alone (11 bits; X itself keeps
+// its 22).  Their rounding is an error of X that later steps see as part of X.  It
+// stays small while the values of X are far from 1, so it is their number that counts,
+// not that of the full steps behind them.  Left of it after five steps, the most over
+// full-rank, nearly low-rank, graded and heavy-tailed matrices (64-bit model of this
+// arithmetic): one rough step 2e-4 to 7e-4 at short sides of 33 to 66, 1e-4 from 128
+// on; two 8e-4 at 128 to 300, 4e-4 from 384, 2e-4 from 640 on; three 2e-3 at 512, 8e-4
+// at 1024.  More steps spread it: after 16 two leave 1e-3 at 512, after 32 one 4e-4 at
+// 256.  Rounding to bf16 itself is 1.7e-3 of the result: what is chosen leaves at most
+// a quarter of that.  Rounding to f16 is 2e-4 and f32's 2^-24, which no rough step
+// leaves alone, so those take full products throughout.
 template <typename T>
 uint32_t rough_steps(uint32_t steps, uint32_t side) {
-    const uint32_t full = sizeof(T) == 4 ? steps : std::is_same<T, bf16_t>::value && side >= 256 ? 2 : 3;
-    return steps > full ? steps - full : 0;
+    if (!std::is_same<T, bf16_t>::value || side < 128) return 0;
+    return std::min(side >= 512 && steps <= 5 ? 2u : 1u, steps - 1);
 }
 
 template <typename T>

@@ -56,6 +56,8 @@ TATARA_API const char* tatara_version(void);
 TATARA_API int32_t tatara_device_count(int32_t* count);
 /* Selects the device for subsequent calls on this thread. */
 TATARA_API int32_t tatara_set_device(int32_t device);
+/* The device that is current on this thread. */
+TATARA_API int32_t tatara_get_device(int32_t* device);
 /* Device name and compute-unit count (DeviceOccupancy::query). */
 TATARA_API int32_t tatara_device_info(int32_t device, char* name, int32_t name_len, int32_t* cu_count);
 /* DeviceBuffer::zeroed / from_host / to_host_vec / memset_d8_async. */

@@ -203,6 +203,7 @@ SIGNATURES = {
     "tatara_version": (C.c_char_p, []),
     "tatara_device_count": (C.c_int32, [c_i32p]),
     "tatara_set_device": (C.c_int32, [C.c_int32]),
+    "tatara_get_device": (C.c_int32, [c_i32p]),
     "tatara_device_info": (C.c_int32, [C.c_int32, C.c_char_p, C.c_int32, c_i32p]),
     "tatara_malloc": (C.c_int32, [C.POINTER(C.c_void_p), C.c_uint64]),
     "tatara_free": (C.c_int32, [C.c_void_p]),

@@ -164,6 +164,14 @@ int32_t tatara_set_device(int32_t device) {
     return kOk;
 }
 
+int32_t tatara_get_device(int32_t* device) {
+    TATARA_REQUIRE(device, "device is null");
+    int current = 0;
+    TATARA_HIP(hipGetDevice(&current), "hipGetDevice");
+    *device = current;
+    return kOk;
+}
+
 int32_t tatara_device_info(int32_t device, char* name, int32_t name_len, int32_t* cu_count) {
     hipDeviceProp_t prop;
     TATARA_HIP(hipGetDeviceProperties(&prop, device), "hipGetDeviceProperties");

@@ -14,11 +14,14 @@ dimension is contiguous; rows may lie inside wider ones.  An operator's element
 type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16.  Calls queue
 their work on `stream` (a runtime.Stream; None is the null stream) and return;
 one operator's calls belong on one stream at a time, since they share the
-workspace.  Wrong shapes and types raise ValueError, device errors TataraError.
+workspace.  All tensors of a call lie on the thread's current device, where the first
+call that needs it makes the workspace.  Wrong shapes, types and devices raise
+ValueError, device errors TataraError.
 """
 from __future__ import annotations
 
 import ctypes as C
+import sys
 
 from . import _lib
 from ._lib import check
@@ -40,8 +43,38 @@ class _TypeNames(dict):
 _TYPE = _TypeNames()
 
 
+_torch_device = None  # torch.cuda.current_device, once torch has met the GPU
+
+
+def _here() -> int:
+    """The thread's current device, which every tensor of a call lies on."""
+    global _torch_device
+    if _torch_device is not None:
+        return _torch_device()
+    torch = sys.modules.get("torch")
+    if torch is not None and torch.cuda.is_initialized():  # else no tensor of its lies on a GPU
+        _torch_device = torch.cuda.current_device
+        return _torch_device()
+    device = C.c_int32()
+    if _lib.load().tatara_get_device(C.byref(device)):
+        return -2  # no GPU, as the call will say; -1 is what a host tensor gives
+    return device.value
+
+
+class _Workspaces(dict):
+    """Device memory that an operator keeps for its calls, by device."""
+
+    def __init__(self, nbytes: int):
+        super().__init__()
+        self.nbytes = nbytes
+
+    def __missing__(self, device: int):  # the current one
+        self[device] = w = _Workspace(self.nbytes)
+        return w
+
+
 class _Workspace:
-    """Device memory that an operator keeps for its calls."""
+    """Memory of the current device."""
 
     def __init__(self, nbytes: int):
         p = C.c_void_p()
@@ -66,8 +99,19 @@ def _dtype(dtype: str) -> int:
 
 
 def _wrong(name: str, x, shape, dtype: str):
+    if getattr(x, "is_cuda", False) and x.get_device() != _here():
+        raise ValueError(f"{name} is on device {x.get_device()}, the current device is {_here()}")
     raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on the device with a contiguous last "
                      f"dimension, not {getattr(x, 'dtype', type(x).__name__)} {tuple(getattr(x, 'shape', ()))}")
+
+
+def _count(name: str, x, cols: int, dtype: str) -> int:
+    """The rows of a [rows, cols] tensor."""
+    try:
+        rows, _ = x.shape
+        return rows
+    except (AttributeError, TypeError, ValueError):
+        _wrong(name, x, ("rows", cols), dtype)
 
 
 def _owned(name: str, x, shape: tuple, dtype: str) -> int:
@@ -81,20 +125,20 @@ def _owned(name: str, x, shape: tuple, dtype: str) -> int:
 # tensor's attributes once, and everything that is not a right tensor goes on to
 # _owned, which takes a DeviceArray and refuses the rest.
 
-def _dense(name: str, x, shape: tuple, dtype: str) -> int:
+def _dense(name: str, x, shape: tuple, dtype: str, here: int) -> int:
     """The address of a contiguous tensor of this shape."""
     try:
-        if x.shape == shape and _TYPE[x.dtype] == dtype and x.is_cuda and x.is_contiguous():
+        if x.shape == shape and _TYPE[x.dtype] == dtype and x.get_device() == here and x.is_contiguous():
             return x.data_ptr()
     except AttributeError:
         pass
     return _owned(name, x, shape, dtype)
 
 
-def _rows(name: str, x, shape: tuple, dtype: str):
+def _rows(name: str, x, shape: tuple, dtype: str, here: int):
     """Address and row stride of a [rows, cols] tensor."""
     try:
-        if x.shape == shape and _TYPE[x.dtype] == dtype and x.is_cuda:
+        if x.shape == shape and _TYPE[x.dtype] == dtype and x.get_device() == here:
             stride, one = x.stride()
             if one == 1 or shape[1] == 1:
                 return x.data_ptr(), stride if shape[0] > 1 else shape[1]  # one row's stride says nothing
@@ -103,10 +147,10 @@ def _rows(name: str, x, shape: tuple, dtype: str):
     return _owned(name, x, shape, dtype), shape[1]
 
 
-def _matrices(name: str, x, shape: tuple, dtype: str):
+def _matrices(name: str, x, shape: tuple, dtype: str, here: int):
     """Address, row stride and matrix stride of a [batch, rows, cols] tensor."""
     try:
-        if x.shape == shape and _TYPE[x.dtype] == dtype and x.is_cuda:
+        if x.shape == shape and _TYPE[x.dtype] == dtype and x.get_device() == here:
             batch, stride, one = x.stride()
             if one == 1 or shape[2] == 1:
                 return x.data_ptr(), stride if shape[1] > 1 else shape[2], batch
@@ -129,42 +173,40 @@ class LayerNorm:
         if not self.eps >= 0.0:
             raise ValueError(f"eps must not be negative, not {eps}")
         self._lib = _lib.load()
-        self._ws = None
+        n = C.c_uint64()
+        check(self._lib.tatara_op_layer_norm_backward_workspace(self.cols, C.byref(n)))
+        self._ws = _Workspaces(n.value)
 
     def forward(self, x, weight, bias, y, mean=None, rstd=None, stream=None) -> None:
         """Writes y, and mean and rstd [rows] for the backward pass if given."""
-        cols, dtype = self.cols, self.dtype
-        rows = x.shape[0]
+        cols, dtype, here = self.cols, self.dtype, _here()
+        rows = _count("x", x, cols, dtype)
         shape, vec, param = (rows, cols), (rows,), (cols,)
-        xp, xs = _rows("x", x, shape, dtype)
-        yp, ys = _rows("y", y, shape, dtype)
+        xp, xs = _rows("x", x, shape, dtype, here)
+        yp, ys = _rows("y", y, shape, dtype, here)
         status = self._lib.tatara_op_layer_norm_forward(
-            xp, xs, None if weight is None else _dense("weight", weight, param, "f32"),
-            None if bias is None else _dense("bias", bias, param, "f32"), yp, ys,
-            None if mean is None else _dense("mean", mean, vec, "f32"),
-            None if rstd is None else _dense("rstd", rstd, vec, "f32"), rows, cols, self.eps, self._code,
+            xp, xs, None if weight is None else _dense("weight", weight, param, "f32", here),
+            None if bias is None else _dense("bias", bias, param, "f32", here), yp, ys,
+            None if mean is None else _dense("mean", mean, vec, "f32", here),
+            None if rstd is None else _dense("rstd", rstd, vec, "f32", here), rows, cols, self.eps, self._code,
             None if stream is None else stream.handle)
         if status:
             check(status)
 
     def backward(self, dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, stream=None) -> None:
         """Writes dx, and the weight's and bias's gradients [cols] if given (overwritten)."""
-        cols, dtype = self.cols, self.dtype
-        rows = x.shape[0]
+        cols, dtype, here = self.cols, self.dtype, _here()
+        rows = _count("x", x, cols, dtype)
         shape, vec, param = (rows, cols), (rows,), (cols,)
-        if self._ws is None:
-            n = C.c_uint64()
-            check(self._lib.tatara_op_layer_norm_backward_workspace(cols, C.byref(n)))
-            self._ws = _Workspace(n.value)
-        dyp, dys = _rows("dy", dy, shape, dtype)
-        xp, xs = _rows("x", x, shape, dtype)
-        dxp, dxs = _rows("dx", dx, shape, dtype)
+        dyp, dys = _rows("dy", dy, shape, dtype, here)
+        xp, xs = _rows("x", x, shape, dtype, here)
+        dxp, dxs = _rows("dx", dx, shape, dtype, here)
         status = self._lib.tatara_op_layer_norm_backward(
-            dyp, dys, xp, xs, None if weight is None else _dense("weight", weight, param, "f32"),
-            _dense("mean", mean, vec, "f32"), _dense("rstd", rstd, vec, "f32"), dxp, dxs,
-            None if dweight is None else _dense("dweight", dweight, param, "f32"),
-            None if dbias is None else _dense("dbias", dbias, param, "f32"), rows, cols, self._code, self._ws.ptr,
-            self._ws.nbytes, None if stream is None else stream.handle)
+            dyp, dys, xp, xs, None if weight is None else _dense("weight", weight, param, "f32", here),
+            _dense("mean", mean, vec, "f32", here), _dense("rstd", rstd, vec, "f32", here), dxp, dxs,
+            None if dweight is None else _dense("dweight", dweight, param, "f32", here),
+            None if dbias is None else _dense("dbias", dbias, param, "f32", here), rows, cols, self._code,
+            (ws := self._ws[here]).ptr, ws.nbytes, None if stream is None else stream.handle)
         if status:
             check(status)
 
@@ -187,38 +229,40 @@ class BucketGate:
         if not 1 <= self.top_k <= min(16, self.buckets):
             raise ValueError(f"top_k must be 1 to 16 and no more than buckets, not {top_k}")
         self._lib = _lib.load()
-        self._ws = None
+        n = C.c_uint64()
+        check(self._lib.tatara_op_bucket_gate_workspace(self.buckets, C.byref(n)))
+        self._ws = _Workspaces(n.value)
 
     def forward(self, logits, bucket, gate, count, prob_sum, counted, loss, valid=None, stream=None) -> None:
         """Writes bucket (int32) and gate (f32) [positions, top_k], count (int32)
         and prob_sum (f32) [buckets], counted (int32) and loss (f32) [1]."""
-        n = logits.shape[0]
-        if self._ws is None:
-            b = C.c_uint64()
-            check(self._lib.tatara_op_bucket_gate_workspace(self.buckets, C.byref(b)))
-            self._ws = _Workspace(b.value)
-        lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype)
+        here = _here()
+        n = _count("logits", logits, self.buckets, self.dtype)
+        lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype, here)
         chosen = (n, self.top_k)
         check(self._lib.tatara_op_bucket_gate_forward(
-            lp, ls, None if valid is None else _dense("valid", valid, (n,), "u8"), n, self.buckets, self.top_k,
-            self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32"),
-            _dense("gate", gate, chosen, "f32"), _dense("count", count, (self.buckets,), "i32"),
-            _dense("prob_sum", prob_sum, (self.buckets,), "f32"), _dense("counted", counted, (1,), "i32"),
-            _dense("loss", loss, (1,), "f32"), self._ws.ptr, self._ws.nbytes, None if stream is None else stream.handle))
+            lp, ls, None if valid is None else _dense("valid", valid, (n,), "u8", here), n, self.buckets, self.top_k,
+            self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32", here),
+            _dense("gate", gate, chosen, "f32", here), _dense("count", count, (self.buckets,), "i32", here),
+            _dense("prob_sum", prob_sum, (self.buckets,), "f32", here), _dense("counted", counted, (1,), "i32", here),
+            _dense("loss", loss, (1,), "f32", here), (ws := self._ws[here]).ptr, ws.nbytes,
+            None if stream is None else stream.handle))
 
     def backward(self, logits, bucket, count, counted, dlogits, dgate=None, dloss: float = 1.0, valid=None,
                  stream=None) -> None:
         """Writes dlogits from dgate (f32 [positions, top_k], None: no gradient) and
         dloss; bucket, count and counted are the forward call's."""
-        n = logits.shape[0]
-        lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype)
-        dp, ds = _rows("dlogits", dlogits, (n, self.buckets), self.dtype)
+        here = _here()
+        n = _count("logits", logits, self.buckets, self.dtype)
+        lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype, here)
+        dp, ds = _rows("dlogits", dlogits, (n, self.buckets), self.dtype, here)
         chosen = (n, self.top_k)
         check(self._lib.tatara_op_bucket_gate_backward(
-            lp, ls, None if valid is None else _dense("valid", valid, (n,), "u8"), n, self.buckets, self.top_k,
-            self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32"),
-            _dense("count", count, (self.buckets,), "i32"), _dense("counted", counted, (1,), "i32"),
-            None if dgate is None else _dense("dgate", dgate, chosen, "f32"), dloss, dp, ds, None if stream is None else stream.handle))
+            lp, ls, None if valid is None else _dense("valid", valid, (n,), "u8", here), n, self.buckets, self.top_k,
+            self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32", here),
+            _dense("count", count, (self.buckets,), "i32", here), _dense("counted", counted, (1,), "i32", here),
+            None if dgate is None else _dense("dgate", dgate, chosen, "f32", here), dloss, dp, ds,
+            None if stream is None else stream.handle))
 
 
 class Orthogonaliser:
@@ -242,18 +286,14 @@ class Orthogonaliser:
         self._lib = _lib.load()
         n = C.c_uint64()
         check(self._lib.tatara_op_orthogonalise_workspace(self.batch, self.rows, self.cols, self._code, C.byref(n)))
-        self._bytes, self._ws = n.value, None
-
-    def _workspace(self) -> int:
-        if self._ws is None:
-            self._ws = _Workspace(self._bytes)
-        return self._ws.ptr
+        self._ws = _Workspaces(n.value)
 
     def __call__(self, x, out, stream=None) -> None:
-        xp, xr, xb = _matrices("x", x, self.shape, self.dtype)
-        op, orow, ob = _matrices("out", out, self.shape, self.dtype)
+        here = _here()
+        xp, xr, xb = _matrices("x", x, self.shape, self.dtype, here)
+        op, orow, ob = _matrices("out", out, self.shape, self.dtype, here)
         check(self._lib.tatara_op_orthogonalise(xp, xr, xb, op, orow, ob, self.batch, self.rows, self.cols,
-                                                self._code, self.steps, self._workspace(), self._bytes,
+                                                self._code, self.steps, (ws := self._ws[here]).ptr, ws.nbytes,
                                                 None if stream is None else stream.handle))
 
 
@@ -279,9 +319,9 @@ class Muon:
         self.weight_decay, self.min_w, self.max_w = float(weight_decay), float(min_w), float(max_w)
 
     def step(self, weights, momentum, grad, lr: float, scale: float = 1.0, stream=None) -> None:
-        o, shape = self._ortho, self.shape
+        o, shape, here = self._ortho, self.shape, _here()
         check(o._lib.tatara_op_muon_step(
-            _dense("weights", weights, shape, "f32"), _dense("momentum", momentum, shape, "f32"),
-            _dense("grad", grad, shape, self.grad_dtype), o.batch, o.rows, o.cols, self._grad_code, self.beta,
-            self.nesterov, lr, self.weight_decay, scale, self.min_w, self.max_w, o.steps, o._workspace(), o._bytes,
-            None if stream is None else stream.handle))
+            _dense("weights", weights, shape, "f32", here), _dense("momentum", momentum, shape, "f32", here),
+            _dense("grad", grad, shape, self.grad_dtype, here), o.batch, o.rows, o.cols, self._grad_code, self.beta,
+            self.nesterov, lr, self.weight_decay, scale, self.min_w, self.max_w, o.steps,
+            (ws := o._ws[here]).ptr, ws.nbytes, None if stream is None else stream.handle))

@@ -9,7 +9,8 @@ tatara_op_bucket_gate_*, tatara_op_orthogonalise, tatara_op_muon_step).
 
 An operator is made once for a layer's shape and holds its workspace.  Tensors
 are device memory: a `DeviceArray`, or any object with data_ptr(), shape,
-stride(), dtype and element_size() (a torch tensor on the GPU).  The last
+stride(), dtype, get_device() and is_contiguous() (a torch tensor on the GPU; torch is
+imported before the library is loaded, so that both run on one HIP runtime).  The last
 dimension is contiguous; rows may lie inside wider ones.  An operator's element
 type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16.  Calls queue
 their work on `stream` (a runtime.Stream; None is the null stream) and return;
@@ -46,18 +47,29 @@ _TYPE = _TypeNames()
 _torch_device = None  # torch.cuda.current_device, once torch has met the GPU
 
 
+def _one_runtime() -> bool:
+    """Whether this library and torch run on one HIP runtime.  torch brings its own and
+    the library takes the one that is loaded, or the system's if none is: loaded ahead
+    of torch they have two, whose streams know nothing of each other."""
+    with open("/proc/self/maps") as maps:
+        return len({line.split()[-1] for line in maps if "/libamdhip64.so" in line}) < 2
+
+
 def _here() -> int:
-    """The thread's current device, which every tensor of a call lies on."""
+    """The thread's current device, which every tensor of a call lies on.  Below zero
+    where no torch tensor can be taken, one number a device."""
     global _torch_device
     if _torch_device is not None:
-        return _torch_device()
-    torch = sys.modules.get("torch")
-    if torch is not None and torch.cuda.is_initialized():  # else no tensor of its lies on a GPU
-        _torch_device = torch.cuda.current_device
         return _torch_device()
     device = C.c_int32()
     if _lib.load().tatara_get_device(C.byref(device)):
         return -2  # no GPU, as the call will say; -1 is what a host tensor gives
+    torch = sys.modules.get("torch")
+    if torch is not None and torch.cuda.is_initialized():  # else no tensor of its lies on a GPU
+        if not _one_runtime():
+            return -3 - device.value
+        _torch_device = torch.cuda.current_device
+        return _torch_device()
     return device.value
 
 
@@ -100,6 +112,9 @@ def _dtype(dtype: str) -> int:
 
 def _wrong(name: str, x, shape, dtype: str):
     if getattr(x, "is_cuda", False) and x.get_device() != _here():
+        if _here() < -2:
+            raise RuntimeError("torch and tatara_amd's library run on two HIP runtimes, which cannot order each "
+                               "other's work: import torch before the library is loaded")
         raise ValueError(f"{name} is on device {x.get_device()}, the current device is {_here()}")
     raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on the device with a contiguous last "
                      f"dimension, not {getattr(x, 'dtype', type(x).__name__)} {tuple(getattr(x, 'shape', ()))}")

@@ -98,6 +98,11 @@ TATARA_API int32_t tatara_device_compute_capability(int32_t device, int32_t* maj
  * (native_backend.rs:54-60, :105-112). */
 TATARA_API int32_t tatara_stream_create(int32_t device, TataraStream** out);
 TATARA_API int32_t tatara_stream_destroy(TataraStream* stream);
+/* A handle of another library's stream of that device (a hipStream_t; NULL is the
+ * device's null stream).  The stream stays the other library's: destroying the
+ * handle leaves it alone, and it must outlive the handle's use.  Makes no device
+ * current. */
+TATARA_API int32_t tatara_stream_wrap(int32_t device, void* native, TataraStream** out);
 TATARA_API int32_t tatara_stream_synchronize(TataraStream* stream);
 TATARA_API int32_t tatara_stream_wait_event(TataraStream* stream, TataraEvent* event);
 /* CudaContext::new_event / CudaEvent::record / CudaEvent::synchronize

@@ -216,6 +216,7 @@ SIGNATURES = {
     "tatara_device_compute_capability": (C.c_int32, [C.c_int32, c_i32p, c_i32p]),
     "tatara_stream_create": (C.c_int32, [C.c_int32, C.POINTER(C.c_void_p)]),
     "tatara_stream_destroy": (C.c_int32, [C.c_void_p]),
+    "tatara_stream_wrap": (C.c_int32, [C.c_int32, C.c_void_p, C.POINTER(C.c_void_p)]),
     "tatara_stream_synchronize": (C.c_int32, [C.c_void_p]),
     "tatara_stream_wait_event": (C.c_int32, [C.c_void_p, C.c_void_p]),
     "tatara_event_create": (C.c_int32, [C.c_int32, C.c_uint32, C.POINTER(C.c_void_p)]),

@@ -13,6 +13,7 @@
 
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 
@@ -84,15 +85,27 @@ int32_t tatara_stream_create(int32_t device, TataraStream** out) {
     TATARA_HIP(hipSetDevice(device), "hipSetDevice");
     hipStream_t s = nullptr;
     TATARA_HIP(hipStreamCreateWithFlags(&s, hipStreamNonBlocking), "hipStreamCreateWithFlags");
-    *out = new TataraStream{s, device};
+    *out = new TataraStream{s, device, false};
     return kOk;
 }
 
 int32_t tatara_stream_destroy(TataraStream* stream) {
     if (!stream) return kOk;
-    const hipError_t e = hipStreamDestroy(stream->s);
+    const hipError_t e = stream->wrapped ? hipSuccess : hipStreamDestroy(stream->s);
     delete stream;
     TATARA_HIP(e, "hipStreamDestroy");
+    return kOk;
+}
+
+int32_t tatara_stream_wrap(int32_t device, void* native, TataraStream** out) {
+    TATARA_REQUIRE(out, "out is null");
+    *out = nullptr;
+    TATARA_REQUIRE(device >= 0, "no such device");
+    *out = new (std::nothrow) TataraStream{static_cast<hipStream_t>(native), device, true};
+    if (!*out) {
+        set_error("out of host memory");
+        return kErrOutOfMemory;
+    }
     return kOk;
 }
 

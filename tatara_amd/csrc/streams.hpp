@@ -8,6 +8,7 @@
 struct TataraStream {
     hipStream_t s;
     int device;
+    bool wrapped;  // another library's stream
 };
 
 struct TataraEvent {

@@ -13,7 +13,8 @@ stride(), dtype, get_device() and is_contiguous() (a torch tensor on the GPU; to
 imported before the library is loaded, so that both run on one HIP runtime).  The last
 dimension is contiguous; rows may lie inside wider ones.  An operator's element
 type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16.  Calls queue
-their work on `stream` (a runtime.Stream; None is the null stream) and return;
+their work on `stream` (a runtime.Stream or a torch.cuda.Stream; None is torch's
+current stream where the call's first tensor is torch's, else the null stream) and return;
 one operator's calls belong on one stream at a time, since they share the
 workspace.  All tensors of a call lie on the thread's current device, where the first
 call that needs it makes the workspace.  Wrong shapes, types and devices raise
@@ -44,7 +45,9 @@ class _TypeNames(dict):
 _TYPE = _TypeNames()
 
 
-_torch_device = None  # torch.cuda.current_device, once torch has met the GPU
+# torch.cuda.current_device and the hipStream_t of its current stream on a device, once
+# torch has met the GPU
+_torch_device = _torch_stream = None
 
 
 def _one_runtime() -> bool:
@@ -55,10 +58,15 @@ def _one_runtime() -> bool:
         return len({line.split()[-1] for line in maps if "/libamdhip64.so" in line}) < 2
 
 
+def _two_runtimes():
+    raise RuntimeError("torch and tatara_amd's library run on two HIP runtimes, which cannot order each other's work: "
+                       "import torch before the library is loaded")
+
+
 def _here() -> int:
     """The thread's current device, which every tensor of a call lies on.  Below zero
     where no torch tensor can be taken, one number a device."""
-    global _torch_device
+    global _torch_device, _torch_stream
     if _torch_device is not None:
         return _torch_device()
     device = C.c_int32()
@@ -68,9 +76,44 @@ def _here() -> int:
     if torch is not None and torch.cuda.is_initialized():  # else no tensor of its lies on a GPU
         if not _one_runtime():
             return -3 - device.value
-        _torch_device = torch.cuda.current_device
+        # what torch.cuda.current_stream and current_device ask, without a Stream object for
+        # the answer: 0.6 us less of a call's 7
+        _torch_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                                lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _torch_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         return _torch_device()
     return device.value
+
+
+class _Handles(dict):
+    """(device, hipStream_t) -> the library's handle of that stream of torch's."""
+
+    def __missing__(self, key) -> int:
+        h = C.c_void_p()
+        check(_lib.load().tatara_stream_wrap(*key, C.byref(h)))
+        self[key] = h.value  # 16 bytes, for as long as the process
+        return h.value
+
+
+_HANDLES = _Handles()
+
+
+def _place(x, stream):
+    """The current device, as _here() gives it, and the handle of the stream that a call
+    goes to whose first tensor is x."""
+    here = _here() if _torch_device is None else _torch_device()
+    if stream is None:
+        if here < 0 or not hasattr(x, "get_device"):
+            return here, None
+        native = _torch_stream(here)
+        return here, _HANDLES[here, native] if native else None  # the default one is the null stream
+    if hasattr(stream, "cuda_stream"):
+        if here < -2:
+            _two_runtimes()
+        return here, _HANDLES[stream.device_index, stream.cuda_stream]
+    if not stream.handle:
+        raise ValueError("the stream is closed")
+    return here, stream.handle
 
 
 class _Workspaces(dict):
@@ -113,8 +156,7 @@ def _dtype(dtype: str) -> int:
 def _wrong(name: str, x, shape, dtype: str):
     if getattr(x, "is_cuda", False) and x.get_device() != _here():
         if _here() < -2:
-            raise RuntimeError("torch and tatara_amd's library run on two HIP runtimes, which cannot order each "
-                               "other's work: import torch before the library is loaded")
+            _two_runtimes()
         raise ValueError(f"{name} is on device {x.get_device()}, the current device is {_here()}")
     raise ValueError(f"{name} must be a {dtype} tensor of shape {tuple(shape)} on the device with a contiguous last "
                      f"dimension, not {getattr(x, 'dtype', type(x).__name__)} {tuple(getattr(x, 'shape', ()))}")
@@ -194,7 +236,8 @@ class LayerNorm:
 
     def forward(self, x, weight, bias, y, mean=None, rstd=None, stream=None) -> None:
         """Writes y, and mean and rstd [rows] for the backward pass if given."""
-        cols, dtype, here = self.cols, self.dtype, _here()
+        cols, dtype = self.cols, self.dtype
+        here, queue = _place(x, stream)
         rows = _count("x", x, cols, dtype)
         shape, vec, param = (rows, cols), (rows,), (cols,)
         xp, xs = _rows("x", x, shape, dtype, here)
@@ -204,13 +247,14 @@ class LayerNorm:
             None if bias is None else _dense("bias", bias, param, "f32", here), yp, ys,
             None if mean is None else _dense("mean", mean, vec, "f32", here),
             None if rstd is None else _dense("rstd", rstd, vec, "f32", here), rows, cols, self.eps, self._code,
-            None if stream is None else stream.handle)
+            queue)
         if status:
             check(status)
 
     def backward(self, dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, stream=None) -> None:
         """Writes dx, and the weight's and bias's gradients [cols] if given (overwritten)."""
-        cols, dtype, here = self.cols, self.dtype, _here()
+        cols, dtype = self.cols, self.dtype
+        here, queue = _place(x, stream)
         rows = _count("x", x, cols, dtype)
         shape, vec, param = (rows, cols), (rows,), (cols,)
         dyp, dys = _rows("dy", dy, shape, dtype, here)
@@ -221,7 +265,7 @@ class LayerNorm:
             _dense("mean", mean, vec, "f32", here), _dense("rstd", rstd, vec, "f32", here), dxp, dxs,
             None if dweight is None else _dense("dweight", dweight, param, "f32", here),
             None if dbias is None else _dense("dbias", dbias, param, "f32", here), rows, cols, self._code,
-            (ws := self._ws[here]).ptr, ws.nbytes, None if stream is None else stream.handle)
+            (ws := self._ws[here]).ptr, ws.nbytes, queue)
         if status:
             check(status)
 
@@ -251,7 +295,7 @@ class BucketGate:
     def forward(self, logits, bucket, gate, count, prob_sum, counted, loss, valid=None, stream=None) -> None:
         """Writes bucket (int32) and gate (f32) [positions, top_k], count (int32)
         and prob_sum (f32) [buckets], counted (int32) and loss (f32) [1]."""
-        here = _here()
+        here, queue = _place(logits, stream)
         n = _count("logits", logits, self.buckets, self.dtype)
         lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype, here)
         chosen = (n, self.top_k)
@@ -261,13 +305,13 @@ class BucketGate:
             _dense("gate", gate, chosen, "f32", here), _dense("count", count, (self.buckets,), "i32", here),
             _dense("prob_sum", prob_sum, (self.buckets,), "f32", here), _dense("counted", counted, (1,), "i32", here),
             _dense("loss", loss, (1,), "f32", here), (ws := self._ws[here]).ptr, ws.nbytes,
-            None if stream is None else stream.handle))
+            queue))
 
     def backward(self, logits, bucket, count, counted, dlogits, dgate=None, dloss: float = 1.0, valid=None,
                  stream=None) -> None:
         """Writes dlogits from dgate (f32 [positions, top_k], None: no gradient) and
         dloss; bucket, count and counted are the forward call's."""
-        here = _here()
+        here, queue = _place(logits, stream)
         n = _count("logits", logits, self.buckets, self.dtype)
         lp, ls = _rows("logits", logits, (n, self.buckets), self.dtype, here)
         dp, ds = _rows("dlogits", dlogits, (n, self.buckets), self.dtype, here)
@@ -277,7 +321,7 @@ class BucketGate:
             self.renormalise, self.balance, self._code, _dense("bucket", bucket, chosen, "i32", here),
             _dense("count", count, (self.buckets,), "i32", here), _dense("counted", counted, (1,), "i32", here),
             None if dgate is None else _dense("dgate", dgate, chosen, "f32", here), dloss, dp, ds,
-            None if stream is None else stream.handle))
+            queue))
 
 
 class Orthogonaliser:
@@ -304,12 +348,12 @@ class Orthogonaliser:
         self._ws = _Workspaces(n.value)
 
     def __call__(self, x, out, stream=None) -> None:
-        here = _here()
+        here, queue = _place(x, stream)
         xp, xr, xb = _matrices("x", x, self.shape, self.dtype, here)
         op, orow, ob = _matrices("out", out, self.shape, self.dtype, here)
         check(self._lib.tatara_op_orthogonalise(xp, xr, xb, op, orow, ob, self.batch, self.rows, self.cols,
                                                 self._code, self.steps, (ws := self._ws[here]).ptr, ws.nbytes,
-                                                None if stream is None else stream.handle))
+                                                queue))
 
 
 class Muon:
@@ -334,9 +378,10 @@ class Muon:
         self.weight_decay, self.min_w, self.max_w = float(weight_decay), float(min_w), float(max_w)
 
     def step(self, weights, momentum, grad, lr: float, scale: float = 1.0, stream=None) -> None:
-        o, shape, here = self._ortho, self.shape, _here()
+        o, shape = self._ortho, self.shape
+        here, queue = _place(weights, stream)
         check(o._lib.tatara_op_muon_step(
             _dense("weights", weights, shape, "f32", here), _dense("momentum", momentum, shape, "f32", here),
             _dense("grad", grad, shape, self.grad_dtype, here), o.batch, o.rows, o.cols, self._grad_code, self.beta,
             self.nesterov, lr, self.weight_decay, scale, self.min_w, self.max_w, o.steps,
-            (ws := o._ws[here]).ptr, ws.nbytes, None if stream is None else stream.handle))
+            (ws := o._ws[here]).ptr, ws.nbytes, queue))

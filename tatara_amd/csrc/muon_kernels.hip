@@ -669,12 +669,20 @@ struct Strip {
             *reinterpret_cast<float4*>(base + lane % 32 * PITCH + t * 32 + g * 8 + lane / 32 * 4) = q;
         }
     }
+    // Between filling a strip and reading it, and before the next filling: lanes read what
+    // others wrote.  The wave's LDS accesses are done in their order, which the compiler
+    // has to keep; no instruction.
+    __device__ __forceinline__ static void exchange() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
     // the strip as rows of a held matrix from (row, col) on, of which `left`
     // columns exist (a multiple of 32: the side is one of 64, a strip starts at one of 32)
     template <int WIDTH>
     __device__ __forceinline__ void store(Held to, uint32_t row, uint32_t col, uint32_t cols, int32_t left) const {
         constexpr int LANES = WIDTH / 8;  // of a row
         const uint32_t c = lane % LANES * 8;
+        exchange();
 #pragma unroll
         for (int r0 = 0; r0 < 32; r0 += (int)kWave / LANES) {
             const uint32_t r = r0 + lane / LANES;
@@ -692,6 +700,7 @@ struct Strip {
                 *reinterpret_cast<half8*>(at + kLow) = lo;
             }
         }
+        exchange();
     }
     // its values one by one, a batch's loads ahead of its stores:
     // store(row, column, value, load(row, column))
@@ -699,6 +708,7 @@ struct Strip {
     __device__ __forceinline__ void each(F&& load, G&& store) const {
         constexpr int ROWS = (int)kWave / WIDTH, BATCH = 8;
         const uint32_t c = lane % WIDTH;
+        exchange();
 #pragma unroll
         for (int r0 = 0; r0 < 32; r0 += BATCH * ROWS) {
             float old[BATCH];
@@ -710,6 +720,7 @@ struct Strip {
                 store(r, c, base[r * PITCH + c], old[q]);
             }
         }
+        exchange();
     }
 };
 

@@ -264,9 +264,13 @@ __global__ __launch_bounds__(kThreads) void gate_forward_kernel(
     for (int w = 0; w < WAVES; ++w) n += sum_n[w];
     if (gridDim.x > 1) {
         // The last workgroup to get here joins all partial sums, in their order.
-        // They are written past the XCD's L2 and waited for before the workgroup is
-        // counted, and read past it: what a fence would do for them alone, which
-        // would write back all of the L2 (512 workgroups: 47 us instead of 15).
+        // They are atomic stores of agent scope, which gfx950 writes through the XCD's
+        // L2 (sc1) and whose vmcnt falls when they have arrived; each wave waits for
+        // its own ahead of the barrier, and a thread behind it counts the workgroup.
+        // The last one reads them by atomic loads of that scope, past its L2.  That is
+        // the sequence that a release and an acquire of agent scope become on this chip
+        // less the write-back and invalidation of the whole L2, which they need for
+        // plain stores alone (65536 x 9 with them: 12.2 us instead of 8.7).
         for (uint32_t e = threadIdx.x; e <= buckets; e += kThreads)
             put_partial(ws, blockIdx.x, e, buckets, e < buckets ? sum_p[0][e] : 0.0f, e < buckets ? sum_c[0][e] : n);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

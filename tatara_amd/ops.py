@@ -16,8 +16,9 @@ type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16.  Calls queue
 their work on `stream` (a runtime.Stream or a torch.cuda.Stream; None is torch's
 current stream where the call's first tensor is torch's, else the null stream) and return;
 one operator's calls belong on one stream at a time, since they share the
-workspace.  All tensors of a call lie on the thread's current device, where the first
-call that needs it makes the workspace.  Wrong shapes, types and devices raise
+workspace.  All tensors of a call lie on the thread's current device.  The first call
+there that needs the workspace makes it, which waits for the device and cannot be
+recorded into a graph; prepare() makes it ahead.  Wrong shapes, types and devices raise
 ValueError, device errors TataraError.
 """
 from __future__ import annotations
@@ -147,6 +148,14 @@ class _Workspace:
             pass
 
 
+class _Operator:
+    _ws: _Workspaces
+
+    def prepare(self) -> None:
+        """Makes the workspace on the current device, if it has none yet."""
+        self._ws[_here()]
+
+
 def _dtype(dtype: str) -> int:
     if dtype not in DTYPES:
         raise ValueError(f"dtype must be one of {', '.join(DTYPES)}, not {dtype!r}")
@@ -216,7 +225,7 @@ def _matrices(name: str, x, shape: tuple, dtype: str, here: int):
     return _owned(name, x, shape, dtype), shape[2], shape[1] * shape[2]
 
 
-class LayerNorm:
+class LayerNorm(_Operator):
     """y = (x - mean) * rstd * weight + bias over rows of `cols` values.
 
     x, y, dy and dx are [rows, cols] of `dtype`; weight, bias, mean, rstd and the
@@ -270,7 +279,7 @@ class LayerNorm:
             check(status)
 
 
-class BucketGate:
+class BucketGate(_Operator):
     """The best top_k of `buckets` for each position by its logits, with the loss
     that keeps them balanced: balance * buckets / (top_k * counted^2) *
     sum_e count[e] * prob_sum[e], which is `balance` when all are taken alike.
@@ -324,7 +333,7 @@ class BucketGate:
             queue))
 
 
-class Orthogonaliser:
+class Orthogonaliser(_Operator):
     """Newton-Schulz orthogonalisation of `batch` matrices [rows, cols]: called
     with input and output [batch, rows, cols] of `dtype` (out may be the input).
 
@@ -356,7 +365,7 @@ class Orthogonaliser:
                                                 queue))
 
 
-class Muon:
+class Muon(_Operator):
     """Muon updates of `batch` weight matrices [rows, cols]: momentum of the
     gradient, orthogonalised, subtracted from the weights.
 
@@ -374,6 +383,7 @@ class Muon:
             raise ValueError(f"min_w {min_w} exceeds max_w {max_w}")
         self.grad_dtype, self._grad_code = grad_dtype, _dtype(grad_dtype)
         self._ortho = Orthogonaliser(batch, rows, cols, "f32", steps)
+        self._ws = self._ortho._ws
         self.shape, self.beta, self.nesterov = self._ortho.shape, float(beta), int(bool(nesterov))
         self.weight_decay, self.min_w, self.max_w = float(weight_decay), float(min_w), float(max_w)
 
@@ -384,4 +394,4 @@ class Muon:
             _dense("weights", weights, shape, "f32", here), _dense("momentum", momentum, shape, "f32", here),
             _dense("grad", grad, shape, self.grad_dtype, here), o.batch, o.rows, o.cols, self._grad_code, self.beta,
             self.nesterov, lr, self.weight_decay, scale, self.min_w, self.max_w, o.steps,
-            (ws := o._ws[here]).ptr, ws.nbytes, queue))
+            (ws := self._ws[here]).ptr, ws.nbytes, queue))

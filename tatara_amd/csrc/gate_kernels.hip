@@ -376,7 +376,8 @@ __global__ __launch_bounds__(kThreads) void gate_backward_kernel(
         for (int j0 = 0; j0 < V; j0 += Piece<T>::V) {
             Piece<T> out;
 #pragma unroll
-            for (int j = 0; j < Piece<T>::V; ++j) out.v[j] = (T)(row.p[j0 + j] * (h[j0 + j] - s));
+            for (int j = 0; j < Piece<T>::V; ++j)
+                out.v[j] = (T)(row.counts ? row.p[j0 + j] * (h[j0 + j] - s) : 0.0f);  // 0 also where h is infinite
             out.store(to + j0, left - j0);
         }
     }

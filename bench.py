@@ -87,7 +87,7 @@ def hbm_traffic(workload: str, kernel: str):
 
     profiles/hbm_traffic.md holds FETCH_SIZE / WRITE_SIZE per dispatch from
     two rocprofv3 --pmc passes of this script, scaled by a plain-copy
-    calibration, with the commit and the `source_digest` of the kernels
+    calibration, with the commit and the `step_digest` of the kernels
     measured; (None, None, None) when the kernel was not profiled.
     """
     path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "profiles", "hbm_traffic.md")
@@ -909,9 +909,9 @@ def main() -> int:
     if achieved > HBM_PEAK_GBS:
         raise SystemExit(f"{dom}: compulsory bytes / launch time = {achieved:.0f} GB/s exceeds the HBM peak")
     traffic, traffic_commit, traffic_digest = hbm_traffic(args.workload, dom)
-    from tatara_amd.build import source_digest
+    from tatara_amd.build import step_digest
 
-    digest = source_digest()
+    digest = step_digest()
     roofline = {
         "bound": "hbm",
         "kernel": dom,
@@ -929,8 +929,9 @@ def main() -> int:
         "traffic_over_compulsory": round(traffic / byts, 3) if traffic else None,
         "logical_GBps": round(logical / (ms * 1e-3) / 1e9, 1) if ms > 0 else None,
         "traffic_source": "profiles/hbm_traffic.md (rocprofv3 --pmc FETCH_SIZE, WRITE_SIZE; copy-calibrated)",
-        # the commit and kernel-source digest the traffic row was measured
-        # with, beside this run's: a stale row shows as traffic_current false
+        # the commit and the digest of the step's kernel sources the traffic row
+        # was measured with, beside this run's: a stale row shows as
+        # traffic_current false
         "traffic_commit": traffic_commit,
         "traffic_source_digest": traffic_digest,
         "source_digest": digest,

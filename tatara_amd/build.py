@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -45,14 +46,38 @@ def source_digest() -> str:
     """A short SHA-256 over the kernel sources (every csrc file and the C
     header, by name and content): it names the kernels a measurement was
     taken with where no git metadata travels with the tree."""
+    return _digest(list(CSRC.glob("*.hip")) + list(CSRC.glob("*.hpp")) + [PKG.parent / "include" / "tatara_hip.h"])
+
+
+def _digest(files: list[Path]) -> str:
     import hashlib
 
     h = hashlib.sha256()
-    files = sorted(list(CSRC.glob("*.hip")) + list(CSRC.glob("*.hpp")) + [PKG.parent / "include" / "tatara_hip.h"])
-    for f in files:
+    for f in sorted(files):
         h.update(f.name.encode() + b"\0")
         h.update(f.read_bytes())
     return h.hexdigest()[:12]
+
+
+def step_sources() -> list[Path]:
+    """The sources of a training step's kernels: the trainers', every file that one of
+    them includes, and the .hip beside a header that is included."""
+    todo, seen = [CSRC / "trainer.hip", CSRC / "simple_trainer.hip"], set()
+    while todo:
+        f = todo.pop()
+        if f in seen or not f.exists():
+            continue
+        seen.add(f)
+        todo += [CSRC / name for name in re.findall(r'^#include "([\w.]+)"', f.read_text(), re.M)]
+        if f.suffix == ".hpp":
+            todo.append(f.with_suffix(".hip"))
+    return sorted(seen)
+
+
+def step_digest() -> str:
+    """As source_digest, of step_sources alone: what a step's kernels were measured
+    with, whatever other operators the library has."""
+    return _digest(step_sources())
 
 
 def build(jobs: int | None = None) -> Path:

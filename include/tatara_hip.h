@@ -265,8 +265,8 @@ TATARA_API int32_t tatara_op_quantise_ft_noalloc(const float* w, uint64_t rows, 
  *
  * These calls queue their work on `stream` (NULL: the device's null stream) and
  * return; nothing is allocated and nothing waits.  The stream must be of the
- * thread's current device.  Tensors are device memory;
- * `dtype` is the element type of the tensors that are void*, strides count
+ * thread's current device (tatara_stream_wrap takes another library's).  Tensors
+ * are device memory; `dtype` is the element type of the tensors that are void*, strides count
  * elements from one row (or matrix) to the next and rows may start at any
  * element.  Inputs and outputs must not overlap unless stated.  `workspace` has
  * at least the bytes that the call's *_workspace function gives, aligned to 16
@@ -337,7 +337,7 @@ TATARA_API int32_t tatara_op_bucket_gate_backward(const void* logits, int64_t st
  *   A = X X^T,  X = 3.4445 X + (-4.7750 A + 2.0315 A^2) X
  * on the matrix's shorter side.  Every singular value that is not tiny beside
  * the largest ends between about 0.7 and 1.2.  A matrix of zeros stays zero; one
- * with a NaN or an infinity becomes NaN.  out may be in.
+ * with a NaN or an infinity becomes NaN.  out may be in, with the same strides.
  * Products take operands of 22 bits and sum in f32.  A bf16 result whose shorter
  * side is 128 or more takes 11 bits in the first step (from 512 on, with five steps
  * or fewer, in the first two): no more than 4e-4 of the result, whose own rounding

@@ -164,8 +164,11 @@ __device__ __forceinline__ void write_totals(const float* prob, const int32_t* c
 
 // One launch: a lane holds eight buckets of a position, so that most positions need
 // one to eight lanes and few joins.  Bound by latency, not bytes (65536 x 9 f32, 2.9
-// MB: 8.9 us): a load, the softmax and the choice, then the partial sums' way past
-// the L2 and back.  As two launches it took 11.4 us.
+// MB: 8.7 us a call, 9.3 the kernel under a profiler): a load, the softmax and the
+// choice, then the partial sums' way past the L2 and back.  As two launches it took
+// 11.4 us.  With many buckets the choice and the join, four buckets a round, are most
+// of it: 65536 x 64 32 us, 65536 x 256 117, 16384 x 1024 with two choices 321, where the
+// backward pass, which has neither, takes 14, 40 and 70 for twice the bytes.
 // scale = balance E / k.  K: at least top_k, for registers without an index.
 template <typename T, int V, int G, int K>
 __global__ __launch_bounds__(kThreads) void gate_forward_kernel(
@@ -309,7 +312,9 @@ __global__ __launch_bounds__(kThreads) void gate_forward_kernel(
 }
 
 // The softmax again from the logits, which costs less than to have kept it.  Bound by
-// latency: 65536 x 9 f32 (5.2 MB) 5.5 us, 16381 x 64 bf16 with four choices 7.5.
+// latency: 65536 x 9 f32 (5.2 MB) 5.5 us, 16381 x 64 bf16 with four choices 7.5; with
+// many buckets by its loads and joins: 65536 x 64 f32 13.6 us (7 of bytes), 65536 x 256
+// 40 (27), 16384 x 1024 with two choices 70 (27).
 // scale = dloss balance E / k
 template <typename T, int V, int G, int K>
 __global__ __launch_bounds__(kThreads) void gate_backward_kernel(

@@ -1067,9 +1067,11 @@ struct Layout {
 Held held(void* ws, uint64_t offset) { return reinterpret_cast<Held>(static_cast<uint8_t*>(ws) + offset); }
 
 // Columns of blocks that a wave of muon_small_kernel holds, 0 where a workgroup
-// cannot hold the matrix: twelve blocks a wave are 48 of its 128 registers.  What it
-// can hold is faster there (one of 16 x 1536: 16 us, by products 82; 32 x 1536 38
-// and 82; 64 x 512 53 and 66) or as fast on one CU (64 x 768: 73 and 70).
+// cannot hold the matrix: twelve blocks a wave are 48 of its 128 registers.  From eight
+// blocks on they do not last beside a step's sums, and 40 to 330 bytes a lane go to
+// scratch.  What it can hold is faster there all the same (one of
+// 16 x 1536: 16 us, by products 82; 32 x 1536, 12 blocks, 38 and 82; 64 x 512, 8 blocks,
+// 53 and 66) or as fast on one CU (64 x 768, 12 blocks: 73 and 70).
 uint32_t small_blocks(uint32_t rows, uint32_t cols) {
     const uint32_t mb = ceil_div(std::min(rows, cols), 16), nt = ceil_div(std::max(rows, cols), 256);
     if (mb > 4 || nt * mb > 12) return 0;

@@ -11,9 +11,12 @@
 // in registers gives without a second read.
 //
 // Both passes read and write each value once and are bound by memory: 65536 x 1536
-// take 153 us forward in f32 (5.3 TB/s; a copy of 2 GiB runs at 4.9) and 121 us
-// backward in bf16 (5.0 TB/s).  Small ones are bound by their launches: 6.4 us
-// forward, 9.8 backward (two launches) up to 512 x 1536.
+// take 152 us forward in f32 (5.3 TB/s; a copy of 2 GiB runs at 4.9) and 122 us
+// backward in bf16 (4.9 TB/s).  Small ones are bound by their launches: 3.7 us
+// forward, 6.7 backward (two launches) at 64 x 1536.  From 8193 columns on the backward
+// pass's sixteen waves hold more than their registers (40 to 700 bytes a lane in
+// scratch): 16384 x 12288 f32 469 us (5.2 TB/s), x 16384 1035 (3.1), 8192 x 32768 3068.
+// (Calls of the C entry points, back to back.)
 #include "elem.hpp"
 
 namespace tatara {
@@ -24,8 +27,8 @@ namespace {
 constexpr int kLaneValues = 32;
 constexpr uint32_t kMaxCols = 16 * kWave * kLaneValues;
 // Workgroups of the backward pass, each of which leaves a partial sum of dw and db:
-// two a CU (65536 x 1536 bf16: 121 us, with four 130), one where rows are few
-// (1009 x 769 f32: 8.9 us, with two 9.8).
+// two a CU (65536 x 1536 bf16: 122 us, with four 130), one where rows are few
+// (1009 x 769 f32: 8.8 us, with two 9.5).
 constexpr uint32_t kGradBlocks = 512;
 uint32_t grad_blocks(uint64_t units) {
     return (uint32_t)std::min<uint64_t>(units, units >= 2048 ? kGradBlocks : kGradBlocks / 2);

@@ -338,10 +338,8 @@ TATARA_API int32_t tatara_op_bucket_gate_backward(const void* logits, int64_t st
  * on the matrix's shorter side.  Every singular value that is not tiny beside
  * the largest ends between about 0.7 and 1.2.  A matrix of zeros stays zero; one
  * with a NaN or an infinity becomes NaN.  out may be in, with the same strides.
- * Products take operands of 22 bits and sum in f32.  A bf16 result whose shorter
- * side is 128 or more takes 11 bits in the first step (from 512 on, with five steps
- * or fewer, in the first two): no more than 4e-4 of the result, whose own rounding
- * is 1.7e-3. */
+ * Products take operands of 22 bits and sum in f32, whatever the type; the result is
+ * rounded to it once. */
 TATARA_API int32_t tatara_op_orthogonalise_workspace(uint32_t batch, uint32_t rows, uint32_t cols, int32_t dtype,
                                                      uint64_t* bytes);
 TATARA_API int32_t tatara_op_orthogonalise(const void* in, int64_t in_row_stride, int64_t in_batch_stride, void* out,

@@ -37,7 +37,7 @@ using floatx16 = float __attribute__((ext_vector_type(16)));
 
 // Where a held matrix has the hi of (row, col); lo lies kLow further.  Four rows'
 // 16 columns of hi fill a 128-byte line, the next line has their lo: a stage's
-// loads take whole lines, also where they take hi alone or 16 columns.  Loads of
+// loads take whole lines, also where a stage is of 16 columns.  Loads of
 // half lines ran at 22 to 27 bytes a clock and CU, of whole ones at 35.
 using Held = f16_t*;
 constexpr uint32_t kLow = 64;
@@ -613,7 +613,7 @@ struct ProductArgs {
     Held p, q;           // [m][k] and [n][k]: the product is p q^T
     uint32_t m, n, k;    // multiples of kPad
     uint32_t tiles_m, tiles_n, tiles;  // of one matrix's product
-    Held old;            // kPoly: A; kApply and later with hi alone: X transposed
+    Held old;            // kPoly: A
     Held to, turned;     // results as they lie and (kApply) transposed
     // kOut, kUpdate: the caller's matrices, [rows][cols]; flipped: X is their transpose
     Target target;
@@ -622,16 +622,14 @@ struct ProductArgs {
 };
 
 // A stage lies in LDS by blocks of 16 columns, in each the rows of p, then of q, four
-// rows' 8 P pieces together as they lie in memory (hi of the four rows, then lo).
+// rows' 16 pieces together as they lie in memory (hi of the four rows, then lo).
 // Within those the place turns with the row, so that 16 rows of one piece cover all
 // of LDS's banks.
-template <int P>
 __device__ __forceinline__ uint32_t turn(uint32_t row) {
-    return P == 2 ? (row / 4 & 1) | (row / 4 & 2) << 2 : row / 8 & 1;
+    return (row / 4 & 1) | (row / 4 & 2) << 2;
 }
-template <int P>
 __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t low, uint32_t half) {
-    return row / 4 * (8 * P) + ((low * 8 + row % 4 * 2 + half) ^ turn<P>(row));
+    return row / 4 * 16 + ((low * 8 + row % 4 * 2 + half) ^ turn(row));
 }
 
 // 16 bytes a lane from global memory to LDS, the wave's 64 in a row from `to`.
@@ -724,21 +722,25 @@ struct Strip {
     }
 };
 
-// P = 2: hi hi + hi lo + lo hi;  P = 1: hi hi alone, with a X added in f32 to the
-// last product of the step instead of a I to B.
+// hi hi + hi lo + lo hi of every product, whatever the result's type (T, of kOut alone).
+// Early steps that multiply hi alone (11 bits) would take a fifth off a bf16 result
+// (2048 x 1024: three of five 209 us, none 267) and are not taken: what they leave of it
+// has no bound near its own rounding of 1.7e-3.  One of five leaves 3e-6 of a full-rank
+// matrix of 256, but 2e-3 of one whose rows are all alike: its one singular value is at
+// 1 from the start, and what rounding puts beside it grows in the steps that follow.
 //
 // 45 of 1629 x 1536 f32, a step: X X^T 0.60 ms, B 0.58, B X 1.15 (1.31 into the
 // weights), 930 TFLOP/s of f16 products in tiles of 128.  There the card's power is
 // the bound: matrix cores are busy in 57% of cycles at a clock of about 1.6 GHz,
 // tiles of 256 x 256 and 256 x 128 reach the same rate.  Small ones are bound by
 // latency: 6 to 8 us a launch (5 of 257 x 391).
-template <int EPI, typename T, typename L, int P>
+template <int EPI, typename T, typename L>
 __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a) {
     constexpr int BM = L::BM, BN = L::BN, TM = L::TM, TN = L::TN;
-    constexpr int S = L::S, LOADS = L::loads(P);
+    constexpr int S = L::S, LOADS = L::LOADS;
     constexpr int DOWN = StripShape<L>::DOWN, OVER = StripShape<L>::OVER;
-    constexpr int STAGE = L::pieces(P), BLOCK = (BM + BN) * 2 * P;  // pieces, of a stage and of 16 columns
-    using Lds = ProductLds<L, P>;
+    constexpr int STAGE = L::PIECES, BLOCK = (BM + BN) * 4;  // pieces, of a stage and of 16 columns
+    using Lds = ProductLds<L>;
     __shared__ half8 lds[Lds::BYTES / 16];
     // neighbouring tiles on one XCD, so that its L2 holds the panels they share
     const uint32_t bid = xcd_swizzle(blockIdx.x, gridDim.x);
@@ -770,8 +772,8 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
     const f16_t* from[LOADS];
 #pragma unroll
     for (int s = 0; s < LOADS; ++s) {
-        const uint32_t e = s * L::THREADS + tid, at = e % BLOCK, four = at / (8 * P);
-        const uint32_t piece = at % (8 * P) ^ turn<P>(four * 4), row = four * 4 + piece % 8 / 2;
+        const uint32_t e = s * L::THREADS + tid, at = e % BLOCK, four = at / 16;
+        const uint32_t piece = at % 16 ^ turn(four * 4), row = four * 4 + piece % 8 / 2;
         // rows past the matrix (its side is a multiple of 64, not of the tile) are not stored
         const uint32_t r = row < BM ? min(i0 + row, a.m - 1) : min(j0 + row - BM, a.n - 1);
         from[s] = (row < BM ? a.p + p_at : a.q + q_at) + held_at(r, e / BLOCK * 16 + piece % 2 * 8, a.k) +
@@ -794,21 +796,21 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
         if (it + S - 1 < stages) fetch(buf == 0 ? S - 1 : buf - 1, (it + S - 1) * L::KS);
         // the next 16 values of k are read while these are multiplied
         constexpr int STEPS = L::KS / 16 / L::KG;
-        half8 fp[2][P][TM], fq[2][P][TN];  // [this, next][hi, lo][block]
+        half8 fp[2][2][TM], fq[2][2][TN];  // [this, next][hi, lo][block]
         auto read = [&](int kk) {
             const half8* from_lds = lds + buf * STAGE + (kk * L::KG + group) * BLOCK;
 #pragma unroll
-            for (int lo = 0; lo < P; ++lo) {
+            for (int lo = 0; lo < 2; ++lo) {
                 // in the order of the products below
 #pragma unroll
                 for (int x = 0; x < TM; ++x) {
                     const uint32_t row = wi + x * 32 + lane % 32;
-                    fp[kk % 2][P - 1 - lo][x] = from_lds[place<P>(row, P - 1 - lo, lane / 32)];
+                    fp[kk % 2][1 - lo][x] = from_lds[place(row, 1 - lo, lane / 32)];
                 }
 #pragma unroll
                 for (int y = 0; y < TN; ++y) {
                     const uint32_t row = BM + wj + y * 32 + lane % 32;
-                    fq[kk % 2][lo][y] = from_lds[place<P>(row, lo, lane / 32)];
+                    fq[kk % 2][lo][y] = from_lds[place(row, lo, lane / 32)];
                 }
             }
         };
@@ -818,7 +820,7 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
             if (kk + 1 < STEPS) read(kk + 1);
             const int c = kk % 2;
 #pragma unroll
-            for (int pass = P == 2 ? 2 : 0; pass >= 0; --pass)  // lo hi, hi lo, hi hi
+            for (int pass = 2; pass >= 0; --pass)  // lo hi, hi lo, hi hi
 #pragma unroll
                 for (int x = 0; x < TM; ++x)
 #pragma unroll
@@ -864,8 +866,8 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
 #pragma unroll
     for (int x = 0; x < TM; ++x) {
         const uint32_t i = i0 + wi + x * 32;
-        if ((EPI == kPoly || (P == 1 && EPI != kGram)) && i < a.m) {
-            // A, which is symmetric, or X transposed: four rows of a column are four columns of a row
+        if (EPI == kPoly && i < a.m) {
+            // A is symmetric: four rows of a column are four columns of a row
             half4 hi[TN][4], lo[TN][4];
 #pragma unroll
             for (int y = 0; y < TN; ++y)
@@ -884,10 +886,8 @@ __global__ __launch_bounds__(L::THREADS) void muon_product_kernel(ProductArgs a)
                     for (int r = 0; r < 4; ++r) {
                         const float o = ((float)hi[y][g][r] + (float)lo[y][g][r]) * kUnheld;
                         const float v = acc[x][y][g * 4 + r] * kProduct;
-                        const bool diagonal =
-                            P == 2 && i + g * 8 + lane / 32 * 4 + r == j0 + wj + y * 32 + lane % 32;
-                        acc[x][y][g * 4 + r] =
-                            EPI == kPoly ? fmaf(kC, v, fmaf(kB, o, diagonal ? kA : 0.0f)) : fmaf(kA, o, v);
+                        const bool diagonal = i + g * 8 + lane / 32 * 4 + r == j0 + wj + y * 32 + lane % 32;
+                        acc[x][y][g * 4 + r] = fmaf(kC, v, fmaf(kB, o, diagonal ? kA : 0.0f));
                     }
         } else {
 #pragma unroll
@@ -973,10 +973,10 @@ uint32_t count_tiles(ProductArgs& p) {
     return p.tiles;
 }
 
-template <int EPI, typename T, typename L, int P>
+template <int EPI, typename T, typename L>
 void launch_tiles(ProductArgs p, uint32_t batch, hipStream_t stream) {
     const uint32_t tiles = count_tiles<EPI, L>(p);
-    muon_product_kernel<EPI, T, L, P><<<tiles * batch, L::THREADS, 0, stream>>>(p);
+    muon_product_kernel<EPI, T, L><<<tiles * batch, L::THREADS, 0, stream>>>(p);
 }
 
 // Tiles of 128, two workgroups a CU that fill each other's waits, from two rounds
@@ -987,20 +987,20 @@ void launch_tiles(ProductArgs p, uint32_t batch, hipStream_t stream) {
 // bring to LDS, so where CUs are left over the tiles are of 64 x 32 (3 of 512 x 512:
 // 137) and 32 x 32, four groups of waves and four stages (512 x 512: 102, tiles of 64
 // 127; 257 x 391: 82 and 103; 3 of 512 x 512 139).
-template <int EPI, typename T, int P>
+template <int EPI, typename T>
 void launch_product(ProductArgs p, uint32_t batch, hipStream_t stream) {
     constexpr uint64_t kCus = 256;
     const uint64_t narrow = (uint64_t)batch * count_tiles<EPI, Narrow>(p);
     if ((uint64_t)batch * count_tiles<EPI, Wide>(p) >= 2 * kCus)
-        launch_tiles<EPI, T, Wide, P>(p, batch, stream);
+        launch_tiles<EPI, T, Wide>(p, batch, stream);
     else if (narrow > kCus)
-        launch_tiles<EPI, T, Narrow, P>(p, batch, stream);
+        launch_tiles<EPI, T, Narrow>(p, batch, stream);
     else if (narrow > kCus / 2)
-        launch_tiles<EPI, T, Deep, P>(p, batch, stream);
+        launch_tiles<EPI, T, Deep>(p, batch, stream);
     else if (narrow > kCus * 3 / 8)
-        launch_tiles<EPI, T, Half, P>(p, batch, stream);
+        launch_tiles<EPI, T, Half>(p, batch, stream);
     else
-        launch_tiles<EPI, T, Tiny, P>(p, batch, stream);
+        launch_tiles<EPI, T, Tiny>(p, batch, stream);
 }
 
 struct Step {
@@ -1009,20 +1009,20 @@ struct Step {
     bool last;
 };
 
-template <typename T, int P>
+template <typename T>
 void launch_step(const Step& s, const Source& from, const Target& t, uint32_t batch, hipStream_t stream) {
     ProductArgs p{};
     p.p = p.q = s.x;
     p.m = p.n = s.m;
     p.k = s.n;
     p.to = s.gram;
-    launch_product<kGram, T, P>(p, batch, stream);
+    launch_product<kGram, float>(p, batch, stream);
     p.p = p.q = p.old = s.gram;
     p.k = s.m;
     p.to = s.poly;
-    launch_product<kPoly, T, P>(p, batch, stream);
+    launch_product<kPoly, float>(p, batch, stream);
     p.p = s.poly;
-    p.q = p.old = s.xt;
+    p.q = s.xt;
     p.n = s.n;
     p.to = s.x;
     p.turned = s.next_xt;
@@ -1031,11 +1031,11 @@ void launch_step(const Step& s, const Source& from, const Target& t, uint32_t ba
     p.cols = from.cols;
     p.flipped = from.rows > from.cols;
     if (!s.last)
-        launch_product<kApply, T, P>(p, batch, stream);
+        launch_product<kApply, float>(p, batch, stream);
     else if (t.weights)
-        launch_product<kUpdate, T, P>(p, batch, stream);
+        launch_product<kUpdate, float>(p, batch, stream);
     else
-        launch_product<kOut, T, P>(p, batch, stream);
+        launch_product<kOut, T>(p, batch, stream);
 }
 
 uint32_t up(uint32_t n) { return (n + kPad - 1) / kPad * kPad; }
@@ -1112,8 +1112,8 @@ int32_t launch_small(const Source& s, const Target& t, uint32_t batch, uint32_t 
 }
 
 template <typename T>
-int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws, hipStream_t stream,
-                        uint32_t rough) {
+int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32_t steps, void* ws,
+                        hipStream_t stream) {
     const Layout l(batch, s.rows, s.cols);
     const bool flipped = s.rows > s.cols;
     double* parts = reinterpret_cast<double*>(static_cast<uint8_t*>(ws) + l.parts);
@@ -1134,30 +1134,10 @@ int32_t launch_products(const Source& s, const Target& t, uint32_t batch, uint32
         step.m = l.m;
         step.n = l.n;
         step.last = i + 1 == steps;
-        if (i < rough)
-            launch_step<T, 1>(step, s, t, batch, stream);
-        else
-            launch_step<T, 2>(step, s, t, batch, stream);
+        launch_step<T>(step, s, t, batch, stream);
         TATARA_LAUNCHED("muon_product");
     }
     return kOk;
-}
-
-// First steps of a bf16 result that multiply hi parts alone (11 bits; X itself keeps
-// its 22).  Their rounding is an error of X that later steps see as part of X.  It
-// stays small while the values of X are far from 1, so it is their number that counts,
-// not that of the full steps behind them.  Left of it after five steps, the most over
-// full-rank, nearly low-rank, graded and heavy-tailed matrices (64-bit model of this
-// arithmetic): one rough step 2e-4 to 7e-4 at short sides of 33 to 66, 1e-4 from 128
-// on; two 8e-4 at 128 to 300, 4e-4 from 384, 2e-4 from 640 on; three 2e-3 at 512, 8e-4
-// at 1024.  More steps spread it: after 16 two leave 1e-3 at 512, after 32 one 4e-4 at
-// 256.  Rounding to bf16 itself is 1.7e-3 of the result: what is chosen leaves at most
-// a quarter of that.  Rounding to f16 is 2e-4 and f32's 2^-24, which no rough step
-// leaves alone, so those take full products throughout.
-template <typename T>
-uint32_t rough_steps(uint32_t steps, uint32_t side) {
-    if (!std::is_same<T, bf16_t>::value || side < 128) return 0;
-    return std::min(side >= 512 && steps <= 5 ? 2u : 1u, steps - 1);
 }
 
 template <typename T>
@@ -1165,8 +1145,7 @@ int32_t launch_steps(const Source& s, const Target& t, uint32_t batch, uint32_t 
     // its offsets within a matrix are of 32 bits
     const bool near = (uint64_t)s.rows * std::max(s.row_stride, t.row_stride) < (1u << 29);
     if (near && small_blocks(s.rows, s.cols)) return launch_small<T>(s, t, batch, steps, stream);
-    const uint32_t rough = t.weights ? 0 : rough_steps<T>(steps, std::min(s.rows, s.cols));
-    return launch_products<T>(s, t, batch, steps, ws, stream, rough);
+    return launch_products<T>(s, t, batch, steps, ws, stream);
 }
 
 int32_t check_matrices(uint32_t batch, uint32_t rows, uint32_t cols, int32_t dtype) {

@@ -13,10 +13,9 @@ struct Tile {
     static constexpr int BM = BM_, BN = BN_, WR = WR_, WC = WC_, KS = KS_, S = S_, KG = KG_;
     static constexpr int THREADS = KG * WR * WC * 64;
     static constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 blocks of a wave
-    // with P of hi and lo: 16-byte pieces of the stage, and a thread's loads
-    static constexpr int pieces(int P) { return (BM + BN) * (KS / 8) * P; }
-    static constexpr int loads(int P) { return pieces(P) / THREADS; }
-    static_assert(pieces(1) % THREADS == 0, "every thread loads alike");
+    static constexpr int PIECES = (BM + BN) * (KS / 8) * 2;  // of 16 bytes, of a stage's hi and lo
+    static constexpr int LOADS = PIECES / THREADS;            // of a thread
+    static_assert(PIECES % THREADS == 0, "every thread loads alike");
 };
 
 using Wide = Tile<128, 128, 2, 2, 16, 4>;
@@ -36,10 +35,10 @@ struct StripShape {
 // LDS holds the stages; when all are multiplied, the sums of the groups but the
 // first and, behind them, a strip a wave.  Sums and strips overlap nowhere: one wave
 // may fill its strip while another still reads its sums.
-template <typename L, int P>
+template <typename L>
 struct ProductLds {
     static constexpr int WAVES = L::WR * L::WC, QUADS = L::TM * L::TN * 4;  // of a group; four values a lane
-    static constexpr int STAGES_BYTES = L::S * L::pieces(P) * 16;
+    static constexpr int STAGES_BYTES = L::S * L::PIECES * 16;
     static constexpr int SUMS_BYTES = (L::KG - 1) * WAVES * QUADS * 64 * 16;
     static constexpr int LATER_BYTES = SUMS_BYTES + WAVES * StripShape<L>::BYTES;
     static constexpr int BYTES = STAGES_BYTES > LATER_BYTES ? STAGES_BYTES : LATER_BYTES;

@@ -337,9 +337,8 @@ class Orthogonaliser(_Operator):
     """Newton-Schulz orthogonalisation of `batch` matrices [rows, cols]: called
     with input and output [batch, rows, cols] of `dtype` (out may be the input).
 
-    Products take operands of 22 bits and sum in f32; the first one or two steps of
-    a bf16 result with sides of 128 or more take 11 bits (at most 4e-4 of the result,
-    whose own rounding is 1.7e-3)."""
+    Products take operands of 22 bits and sum in f32, whatever the type; the result is
+    rounded to it once."""
 
     def __init__(self, batch: int, rows: int, cols: int, dtype: str = "f32", steps: int = 5):
         self.batch, self.rows, self.cols = int(batch), int(rows), int(cols)

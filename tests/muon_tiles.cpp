@@ -11,9 +11,9 @@ using namespace tatara;
 namespace {
 int failures = 0;
 
-template <typename L, int P>
+template <typename L>
 void check(const char* name) {
-    using Lds = ProductLds<L, P>;
+    using Lds = ProductLds<L>;
     constexpr int waves = L::WR * L::WC;
     std::vector<int> reader(Lds::BYTES, -1);  // the wave that reads the byte as a sum
     for (int g = 1; g < L::KG; ++g)
@@ -22,7 +22,7 @@ void check(const char* name) {
                 for (int lane = 0; lane < 64; ++lane)
                     for (uint32_t at = 16 * Lds::sum(g, w, q, lane), i = 0; i < 16; ++i) {
                         if (at + i >= reader.size() || reader[at + i] != -1) {
-                            std::printf("%s P=%d: sum byte %u outside or held twice\n", name, P, at + i);
+                            std::printf("%s: sum byte %u outside or held twice\n", name, at + i);
                             ++failures;
                             return;
                         }
@@ -39,26 +39,20 @@ void check(const char* name) {
                                     : reader[at] != -1 && reader[at] != w     ? "read by another wave"
                                                                               : nullptr;
                 if (wrong) {
-                    std::printf("%s P=%d: byte %u of wave %d's strip is %s\n", name, P, at, w, wrong);
+                    std::printf("%s: byte %u of wave %d's strip is %s\n", name, at, w, wrong);
                     ++failures;
                     return;
                 }
                 writer[at] = w;
             }
 }
-
-template <typename L>
-void both(const char* name) {
-    check<L, 1>(name);
-    check<L, 2>(name);
-}
 }  // namespace
 
 int main() {
-    both<Wide>("Wide");
-    both<Narrow>("Narrow");
-    both<Deep>("Deep");
-    both<Half>("Half");
-    both<Tiny>("Tiny");
+    check<Wide>("Wide");
+    check<Narrow>("Narrow");
+    check<Deep>("Deep");
+    check<Half>("Half");
+    check<Tiny>("Tiny");
     return failures != 0;
 }

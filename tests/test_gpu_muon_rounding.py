@@ -1,10 +1,9 @@
 """16-bit results of the Newton-Schulz steps carry their type's rounding and little more.
 
 The result's own rounding, norm-wise, is that of the exact result rounded to the
-type.  Beside it f16 may have what full products leave, e (1 + a + ... + a^4) with
-e = 2^-20 of a step (operands of 22 bits and f32 sums) and a = 3.4445 the most that a
-later step multiplies it by; bf16 a quarter of its rounding, 2^-8 * 0.43 / 4 = 4.2e-4,
-which its first steps of 11 bits may leave.
+type.  Beside it stands what products leave, e (1 + a + ... + a^4) with e = 2^-20 of
+a step (operands of 22 bits and f32 sums) and a = 3.4445 the most that a later step
+multiplies it by.
 """
 import pytest
 import torch
@@ -17,8 +16,8 @@ TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
 A, B, C = 3.4445, -4.7750, 2.0315
 
 
-def left_over(dtype, steps):
-    return 2.0**-8 * 0.43 / 4 if dtype == "bf16" else 2.0**-20 * sum(A**i for i in range(steps))
+def left_over(steps):
+    return 2.0**-20 * sum(A**i for i in range(steps))
 
 
 def exact(u, steps):
@@ -46,6 +45,17 @@ def graded(batch, rows, cols, g):
     return torch.randn(batch, rows, cols, generator=g) * torch.logspace(0, -3, rows)[:, None]
 
 
+def alike(batch, rows, cols, g):
+    """One singular value, which is at 1 from the start."""
+    return torch.full((batch, rows, cols), 3.0)
+
+
+def low_rank(batch, rows, cols, g):
+    """Whole numbers of rank 3, exact in 16 bits."""
+    return (torch.randint(-2, 3, (batch, rows, 3), generator=g) @ torch.randint(-2, 3, (batch, 3, cols),
+                                                                              generator=g)).float()
+
+
 def check(dtype, batch, rows, cols, kind, steps, seed):
     u = kind(batch, rows, cols, torch.Generator().manual_seed(seed)).to(TYPES[dtype])
     out = torch.empty_like(u, device="cuda")
@@ -54,11 +64,11 @@ def check(dtype, batch, rows, cols, kind, steps, seed):
     for got, want in zip(out.double().cpu(), e):
         rounding = float((want.to(TYPES[dtype]).double() - want).norm() / want.norm())
         off = float((got - want).norm() / want.norm())
-        assert off <= rounding + left_over(dtype, steps), (off, rounding)
+        assert off <= rounding + left_over(steps), (off, rounding)
 
 
 @pytest.mark.parametrize("dtype", list(TYPES))
-@pytest.mark.parametrize("kind", [full_rank, nearly_low_rank, graded])
+@pytest.mark.parametrize("kind", [full_rank, nearly_low_rank, graded, alike, low_rank])
 @pytest.mark.parametrize("batch,rows,cols", [(2, 65, 66), (1, 65, 100), (1, 100, 72), (1, 66, 1000), (1, 33, 1100),
                                              (3, 129, 127), (1, 128, 512), (2, 257, 256), (1, 511, 600),
                                              (1, 512, 513)])

@@ -379,7 +379,7 @@ def _operator(kind: str, dtype: str, *shape):
     if kind == "dropout":
         return ops.Dropout(cols=shape[0], p=shape[1], dtype=dtype, seed=shape[2])
     if kind == "embed":
-        return ops.Embedding(vocab=shape[0], cols=shape[1], dtype=dtype, scale=shape[2])
+        return ops.Embedding(vocab=shape[0], cols=shape[1], positions=shape[2], dtype=dtype, scale=shape[3])
     return ops.BucketRows(buckets=shape[0], cols=shape[1], top_k=shape[2], dtype=dtype, capacity=shape[3])
 
 
@@ -401,14 +401,16 @@ def _own(s: dict) -> dict:
     elif kind == "dropout_grad":
         _operator("dropout", dtype, cols, c["p"], s["seed"]).backward(s["x"], o["y"], step=s["step"])
     elif kind == "embed":
-        _operator("embed", dtype, c["vocab"], cols, s["scale"]).forward(s["token"], s["table"], o["y"])
+        op = _operator("embed", dtype, c["vocab"], cols, c["rows"], s["scale"])
+        op.forward(s["token"], s["table"], o["y"])
     elif kind == "embed_grad":
-        _operator("embed", dtype, c["vocab"], cols, s["scale"]).backward(s["dy"], s["token"], o["dtable"])
+        op = _operator("embed", dtype, c["vocab"], cols, c["rows"], s["scale"])
+        op.backward(s["dy"], s["token"], o["dtable"])
     else:
         op = _operator("rows", dtype, c["buckets"], cols, c["top"], _room(c))
         if kind == "gather":
             op.sort(s["bucket"], o["slot"], o["source"], o["offset"])
-            op.gather(s["x"], o["source"], o["rows"])
+            op.gather(s["x"], o["slot"], o["source"], o["rows"])
         elif kind == "gather_grad":
             op.gather_backward(s["rows"], s["slot"], o["y"])
         elif kind == "combine":

@@ -359,6 +359,116 @@ TATARA_API int32_t tatara_op_muon_step(float* weights, float* momentum, const vo
                                        TataraStream* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Around a learned choice's bucket layers                                   */
+/* ------------------------------------------------------------------------ */
+
+/* No counterparts in the reference: a root-mean-square norm with the residual's
+ * addition, dropout, the rows of each bucket side by side and back, and an
+ * embedding.  What stands above of streams, tensors, strides and workspaces holds
+ * for them too; none of their workspaces has to be cleared. */
+
+/* Root-mean-square norm of rows of 1..32768 columns:
+ *   s = x + residual (rounded to the element type; residual may be NULL: s = x),
+ *   y = s * rstd * weight,  rstd = 1 / sqrt(sum(s^2) / cols + eps).
+ * weight is f32 and may be NULL (1).  total takes s and may be NULL, and may be x or
+ * residual, with the same stride; it needs a residual.  rstd, f32 per row, is what the
+ * backward pass reads and may be NULL. */
+TATARA_API int32_t tatara_op_rms_norm_forward(const void* x, int64_t x_stride, const void* residual,
+                                              int64_t residual_stride, const float* weight, void* total,
+                                              int64_t total_stride, void* y, int64_t y_stride, float* rstd,
+                                              uint64_t rows, uint32_t cols, float eps, int32_t dtype,
+                                              TataraStream* stream);
+/* The same with y in 8 bits, q [rows][cols] (a byte each, q_stride bytes from row to
+ * row) and scale [rows][groups], f32: y is about q * scale.  A scale stands for `group`
+ * columns (32, 64 or 128; groups = cols / group rounded up) or for the whole row (0;
+ * groups = 1):
+ *   scale = max(largest |y| of the group, 2^-100) / M,  q = y / scale rounded to nearest,
+ * M = 448 for TATARA_E4M3 (4 bits of exponent, 3 of fraction, no infinity), 127 for
+ * TATARA_I8.  A group with a y that is not finite gets the scale NaN and q 0. */
+#define TATARA_E4M3 0
+#define TATARA_I8 1
+TATARA_API int32_t tatara_op_rms_norm_forward_8bit(const void* x, int64_t x_stride, const void* residual,
+                                                   int64_t residual_stride, const float* weight, void* total,
+                                                   int64_t total_stride, void* q, int64_t q_stride, float* scale,
+                                                   float* rstd, uint64_t rows, uint32_t cols, uint32_t group,
+                                                   float eps, int32_t dtype, int32_t format, TataraStream* stream);
+/* With s the forward call's, h = s * rstd and g = dy * weight:
+ *   dx = rstd * (g - h * sum(g * h) / cols) + dtotal,  dweight = sum over rows of dy * h.
+ * dx is the gradient of x and of the residual alike.  dtotal, the gradient that reaches
+ * s by itself, may be NULL; dx may be dtotal, with the same stride.  dweight (f32,
+ * overwritten) may be NULL, and then no workspace is needed.  No rows: it becomes 0. */
+TATARA_API int32_t tatara_op_rms_norm_backward_workspace(uint32_t cols, uint64_t* bytes);
+TATARA_API int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride, const void* total,
+                                               int64_t total_stride, const float* weight, const float* rstd,
+                                               const void* dtotal, int64_t dtotal_stride, void* dx,
+                                               int64_t dx_stride, float* dweight, uint64_t rows, uint32_t cols,
+                                               int32_t dtype, void* workspace, uint64_t workspace_bytes,
+                                               TataraStream* stream);
+
+/* Dropout of rows of 1..2^24 columns:
+ *   y = u >= round(p * 2^32) ? x / (1 - p) : 0, plus residual (may be NULL),
+ * u of row r and column c: word c % 4 of Philox4x32-10 at the counter (c / 4,
+ * first_row + r, low and high half of the step) with seed's halves as the key, so no mask is
+ * stored.  The step is `step`, plus *more_steps if that is given (device memory, read
+ * when the call runs: a captured graph's replays take other masks by it).  p in [0, 1).
+ * A dropped value is 0 whatever it was.  The gradient of x is the same call on dy with
+ * no residual. */
+TATARA_API int32_t tatara_op_dropout(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                     void* y, int64_t y_stride, uint64_t rows, uint32_t cols, double p, uint64_t seed,
+                                     uint64_t step, const uint64_t* more_steps, uint32_t first_row, int32_t dtype,
+                                     TataraStream* stream);
+
+/* The choices (t, j) of positions' buckets, bucket [positions][top_k] (top_k 1..16),
+ * by bucket, and in a bucket by t and j:
+ *   slot[t][j] = the row of choice (t, j), -1 if it has none,
+ *   source[r]  = t * top_k + j of row r's choice, -1 if it has none,
+ *   offset[e]  = choices of buckets below e, [buckets] of all.
+ * A bucket outside 0..buckets - 1 is no choice.  With capacity 0 rows follow each
+ * other (positions * top_k of them, the last ones without a choice); with another,
+ * bucket e has rows e * capacity to (e + 1) * capacity - 1, and choices that do not
+ * fit have no row. */
+TATARA_API int32_t tatara_op_bucket_rows_workspace(uint32_t buckets, uint64_t* bytes);
+TATARA_API int32_t tatara_op_bucket_rows_sort(const int32_t* bucket, uint64_t positions, uint32_t buckets,
+                                              uint32_t top_k, uint32_t capacity, int32_t* slot, int32_t* source,
+                                              int32_t* offset, void* workspace, uint64_t workspace_bytes,
+                                              TataraStream* stream);
+/* rows[slot[t][j]] = x[t], and zeros in rows without a choice; 1..32768 columns. */
+TATARA_API int32_t tatara_op_bucket_rows_gather(const void* x, int64_t x_stride, const int32_t* slot,
+                                                const int32_t* source, uint64_t positions, uint32_t top_k, void* rows,
+                                                int64_t rows_stride, uint64_t n_rows, uint32_t cols, int32_t dtype,
+                                                TataraStream* stream);
+/* y[t] = sum over j of gate[t][j] * rows[slot[t][j]], of the choices that have a row
+ * (gate, f32, may be NULL: 1, which is also the gradient of the gather call). */
+TATARA_API int32_t tatara_op_bucket_rows_combine(const void* rows, int64_t rows_stride, uint64_t n_rows,
+                                                 const int32_t* slot, const float* gate, uint64_t positions,
+                                                 uint32_t top_k, void* y, int64_t y_stride, uint32_t cols,
+                                                 int32_t dtype, TataraStream* stream);
+/* drows[slot[t][j]] = gate[t][j] * dy[t], zeros in rows without a choice, and
+ * dgate[t][j] = sum(dy[t] * rows[slot[t][j]]), 0 for a choice without a row.  dgate may be
+ * NULL, and then rows may be too. */
+TATARA_API int32_t tatara_op_bucket_rows_combine_backward(const void* dy, int64_t dy_stride, const void* rows,
+                                                          int64_t rows_stride, uint64_t n_rows, const int32_t* slot,
+                                                          const int32_t* source, const float* gate,
+                                                          uint64_t positions, uint32_t top_k, void* drows,
+                                                          int64_t drows_stride, float* dgate, uint32_t cols,
+                                                          int32_t dtype, TataraStream* stream);
+
+/* Rows of a table [vocab][cols] (1..2^28 rows, 1..32768 columns) by token:
+ *   y[i] = scale * table[token[i]], zeros where the token is outside 0..vocab - 1. */
+TATARA_API int32_t tatara_op_embedding_forward(const int32_t* token, uint64_t positions, const void* table,
+                                               int64_t table_stride, uint32_t vocab, uint32_t cols, float scale,
+                                               void* y, int64_t y_stride, int32_t dtype, TataraStream* stream);
+/* dtable[v] = scale * sum of dy[i] over the positions i with token v, in f32 and in their
+ * order, for every v (0 where there is none); dtable is f32 [vocab][cols].  The workspace is for
+ * `positions` of them or fewer. */
+TATARA_API int32_t tatara_op_embedding_backward_workspace(uint64_t positions, uint32_t vocab, uint32_t cols,
+                                                          int32_t dtype, uint64_t* bytes);
+TATARA_API int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const int32_t* token,
+                                                uint64_t positions, uint32_t vocab, uint32_t cols, float scale,
+                                                float* dtable, int32_t dtype, void* workspace,
+                                                uint64_t workspace_bytes, TataraStream* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Dataloader: PSV records -> batch (Batch::push_decoded + BucketMode)       */
 /* ------------------------------------------------------------------------ */
 

@@ -294,6 +294,59 @@ SIGNATURES = {
         [C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_int32, C.c_float, C.c_int32]
         + [C.c_void_p] * 4 + [C.c_float, C.c_void_p, C.c_int64, C.c_void_p],
     ),
+    "tatara_op_rms_norm_forward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+         C.c_void_p, C.c_uint64, C.c_uint32, C.c_float, C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_rms_norm_forward_8bit": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+         C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_float, C.c_int32, C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_rms_norm_backward_workspace": (C.c_int32, [C.c_uint32, c_u64p]),
+    "tatara_op_rms_norm_backward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p,
+         C.c_int64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p],
+    ),
+    "tatara_op_dropout": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_uint64, C.c_uint32, C.c_double,
+         C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint32, C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_bucket_rows_workspace": (C.c_int32, [C.c_uint32, c_u64p]),
+    "tatara_op_bucket_rows_sort": (
+        C.c_int32,
+        [C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32] + [C.c_void_p] * 4 + [C.c_uint64, C.c_void_p],
+    ),
+    "tatara_op_bucket_rows_gather": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_int64, C.c_uint64,
+         C.c_uint32, C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_bucket_rows_combine": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p, C.c_int64,
+         C.c_uint32, C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_bucket_rows_combine_backward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_uint64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64,
+         C.c_uint32, C.c_void_p, C.c_int64, C.c_void_p, C.c_uint32, C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_embedding_forward": (
+        C.c_int32,
+        [C.c_void_p, C.c_uint64, C.c_void_p, C.c_int64, C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_int64,
+         C.c_int32, C.c_void_p],
+    ),
+    "tatara_op_embedding_backward_workspace": (
+        C.c_int32, [C.c_uint64, C.c_uint32, C.c_uint32, C.c_int32, c_u64p]),
+    "tatara_op_embedding_backward": (
+        C.c_int32,
+        [C.c_void_p, C.c_int64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_int32,
+         C.c_void_p, C.c_uint64, C.c_void_p],
+    ),
     "tatara_op_orthogonalise_workspace": (C.c_int32, [C.c_uint32, C.c_uint32, C.c_uint32, C.c_int32, c_u64p]),
     "tatara_op_orthogonalise": (
         C.c_int32,

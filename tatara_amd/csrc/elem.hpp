@@ -99,14 +99,20 @@ __device__ __forceinline__ uint32_t partner(uint32_t x) {
 
 // Joins over groups of G lanes (a power of two), the same in all lanes of a group.
 template <int G, typename F>
-__device__ __forceinline__ float group_join(float x, F&& f) {
-    if constexpr (G > 1) x = f(x, __uint_as_float(partner<0>(__float_as_uint(x))));
-    if constexpr (G > 2) x = f(x, __uint_as_float(partner<1>(__float_as_uint(x))));
-    if constexpr (G > 4) x = f(x, __uint_as_float(partner<2>(__float_as_uint(x))));
-    if constexpr (G > 8) x = f(x, __uint_as_float(partner<3>(__float_as_uint(x))));
-    if constexpr (G > 16) x = f(x, __uint_as_float(partner<4>(__float_as_uint(x))));
-    if constexpr (G > 32) x = f(x, __uint_as_float(partner<5>(__float_as_uint(x))));
+__device__ __forceinline__ uint32_t group_join_u(uint32_t x, F&& f) {
+    if constexpr (G > 1) x = f(x, partner<0>(x));
+    if constexpr (G > 2) x = f(x, partner<1>(x));
+    if constexpr (G > 4) x = f(x, partner<2>(x));
+    if constexpr (G > 8) x = f(x, partner<3>(x));
+    if constexpr (G > 16) x = f(x, partner<4>(x));
+    if constexpr (G > 32) x = f(x, partner<5>(x));
     return x;
+}
+template <int G, typename F>
+__device__ __forceinline__ float group_join(float x, F&& f) {
+    return __uint_as_float(group_join_u<G>(__float_as_uint(x), [&](uint32_t a, uint32_t b) {
+        return __float_as_uint(f(__uint_as_float(a), __uint_as_float(b)));
+    }));
 }
 template <int G>
 __device__ __forceinline__ float group_sum(float x) {

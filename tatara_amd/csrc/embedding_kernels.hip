@@ -1,0 +1,331 @@
+// Rows of a table by a position's token, scaled, and the table's gradient.
+//
+//   y_i = scale table_{token_i},   dtable_v = scale sum over i with token_i = v of dy_i
+//
+// A token outside 0..V - 1 stands for none: its row is zeros, and it has no gradient.
+//
+// The gradient sorts the positions by token (a stable radix sort of up to three digits)
+// and adds each token's rows in the positions' order, in f32: no atomics, and every row
+// of dtable is written once.  The sorted positions are cut into chunks of equal length, so
+// that a token that nearly all positions have costs no more than others.  A chunk's
+// first and last token may reach into its neighbours: their sums go to `partial` and are
+// joined in order by a last launch.
+#include "key_sort.hpp"
+#include "row_moves.hpp"
+
+namespace tatara {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr uint32_t kMaxVocab = 1u << 28;
+constexpr uint32_t kClearRows = 64;  // rows of the table that a workgroup looks up, and clears where no position has one
+constexpr int kBatch = 8;            // rows that a lane has in hand
+constexpr uint32_t kMostChunks = 1024;  // of rows as wide as a wave
+constexpr uint32_t kLeastChunk = 8;     // positions
+
+// A pass of the radix sort.  The first one reads the tokens, of which those that stand
+// for none become `vocab`, behind the others.
+struct Digit {
+    const int32_t* token;
+    const uint32_t* in_key;
+    const uint32_t* in_at;
+    uint32_t vocab, shift, mask;
+    uint32_t* out_key;
+    uint32_t* out_at;
+
+    __device__ __forceinline__ uint32_t whole(uint64_t i) const {
+        return token ? min((uint32_t)token[i], vocab) : in_key[i];
+    }
+    __device__ __forceinline__ uint32_t key(uint64_t i) const { return whole(i) >> shift & mask; }
+    __device__ __forceinline__ void put(uint64_t i, uint32_t, uint32_t first, uint32_t rank) const {
+        out_key[first + rank] = whole(i);
+        out_at[first + rank] = token ? (uint32_t)i : in_at[i];
+    }
+    __device__ __forceinline__ void drop(uint64_t) const {}
+    __device__ __forceinline__ void finish(const uint32_t*, uint32_t) const {}
+};
+
+struct Sorted {
+    const uint32_t* key;  // [n] tokens
+    const uint32_t* at;   // [n] their positions
+    uint32_t n, chunk, chunks;
+};
+
+// A group of G lanes adds the rows of a chunk, V columns a lane; rows wider than a wave
+// are cut into `slabs`.  The first `clear` workgroups write the rows of the table that no
+// position has.
+template <typename T, int G, bool FEW>
+__global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __restrict__ dy, int64_t dy_stride, Sorted s,
+                                                                 uint32_t vocab, uint32_t cols, float scale,
+                                                                 float* __restrict__ dtable,
+                                                                 float* __restrict__ partial, uint32_t clear,
+                                                                 uint32_t slabs) {
+    constexpr int V = Piece<T>::V;
+    if (blockIdx.x < clear) {
+        __shared__ bool none[kClearRows];
+        const uint32_t per_row = (cols + 3) / 4;
+        for (uint64_t first = (uint64_t)blockIdx.x * kClearRows; first < vocab; first += (uint64_t)clear * kClearRows) {
+            __syncthreads();
+            if (threadIdx.x < kClearRows) {
+                const uint64_t v = first + threadIdx.x;
+                uint32_t lo = 0, hi = s.n;  // the first place with a key of v or above
+                while (lo < hi) {
+                    const uint32_t mid = lo + (hi - lo) / 2;
+                    if (s.key[mid] < v)
+                        lo = mid + 1;
+                    else
+                        hi = mid;
+                }
+                none[threadIdx.x] = v < vocab && !(lo < s.n && s.key[lo] == v);
+            }
+            __syncthreads();
+            Piece<float> zero;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zero.v[e] = 0.0f;
+            for (uint32_t i = threadIdx.x; i < kClearRows * per_row; i += kThreads) {
+                const uint32_t r = i / per_row, c = (i - r * per_row) * 4;
+                if (none[r]) zero.store(dtable + (first + r) * cols + c, (int)(cols - c));
+            }
+        }
+        return;
+    }
+    uint32_t unit = (blockIdx.x - clear) * (kThreads / G) + threadIdx.x / G;
+    if (G == kWave) unit = __builtin_amdgcn_readfirstlane(unit);
+    const uint32_t chunk = unit / slabs;
+    if (chunk >= s.chunks) return;
+    const int c = (int)((unit - chunk * slabs) * kWave + threadIdx.x % G) * V, left = (int)cols - c;
+    if (left <= 0) return;
+    const uint32_t begin = chunk * s.chunk, end = min(begin + s.chunk, s.n);
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+    // whether the token's first row lies in the chunk
+    bool began = begin == 0 || s.key[begin - 1] != s.key[begin];
+    bool open = false;
+    auto flush = [&](float* to, float by) {
+#pragma unroll
+        for (int h = 0; h < V / 4; ++h) {
+            Piece<float> out;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) out.v[e] = acc[4 * h + e] * by;
+            out.store(to + c + 4 * h, left - 4 * h);
+        }
+    };
+    for (uint32_t i0 = begin; i0 < end; i0 += kBatch) {
+        uint32_t key[kBatch + 1], at[kBatch];
+#pragma unroll
+        for (int j = 0; j <= kBatch; ++j) {
+            const uint32_t i = min(i0 + j, s.n - 1);
+            key[j] = s.key[i];
+            if (j < kBatch) at[j] = s.at[min(i, end - 1)];
+        }
+        Piece<T> p[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (FEW)
+                p[j].load_few(dy + (int64_t)at[j] * dy_stride, (int)cols);
+            else
+                p[j].load(dy + (int64_t)at[j] * dy_stride, c, (int)cols);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (i0 + j >= end || key[j] >= vocab) break;
+            if (!FEW) p[j].fix(left);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += (float)p[j].v[e];
+            open = i0 + j + 1 < s.n && key[j + 1] == key[j];
+            if (!open) {
+                if (began)
+                    flush(dtable + (uint64_t)key[j] * cols, scale);
+                else
+                    flush(partial + (uint64_t)chunk * 2 * cols, 1.0f);
+#pragma unroll
+                for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+                began = true;
+            }
+        }
+    }
+    if (open) flush(partial + ((uint64_t)chunk * 2 + began) * cols, 1.0f);
+}
+
+// The rows of tokens that reach over several chunks: a workgroup a chunk in which one
+// begins and 256 columns, four waves that each add a quarter of the chunks.
+__global__ __launch_bounds__(kThreads) void embedding_join_kernel(Sorted s, uint32_t vocab, uint32_t cols, float scale,
+                                                                  const float* __restrict__ partial,
+                                                                  float* __restrict__ dtable, uint32_t slabs) {
+    constexpr uint32_t WAVES = kThreads / kWave;
+    __shared__ float join[WAVES - 1][kWave * 4];
+    const uint32_t chunk = blockIdx.x / slabs, begin = chunk * s.chunk, next = begin + s.chunk;
+    if (next >= s.n) return;
+    const uint32_t key = s.key[next];
+    if (key >= vocab || s.key[next - 1] != key || (begin > 0 && s.key[begin - 1] == key)) return;
+    // chunks behind this one that begin with the token
+    uint32_t more = 0;
+    for (;;) {
+        const uint64_t place = (uint64_t)next + (uint64_t)(more + threadIdx.x) * s.chunk;
+        const uint32_t got = (uint32_t)__syncthreads_count(place < s.n && s.key[place < s.n ? place : 0] == key);
+        more += got;
+        if (got < kThreads) break;
+    }
+    const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const int c = (int)((blockIdx.x - chunk * slabs) * kWave + lane) * 4, left = (int)cols - c;
+    const uint32_t terms = more + 1, from = (uint32_t)((uint64_t)terms * wave / WAVES),
+                   to = (uint32_t)((uint64_t)terms * (wave + 1) / WAVES);
+    float acc[4] = {};
+    const bool few = cols < 4;
+#pragma unroll 8
+    for (uint32_t t = from; t < to; ++t) {
+        const float* row = partial + ((uint64_t)(chunk + t) * 2 + (t == 0)) * cols;
+        Piece<float> p;
+        if (few) {
+            p.load_few(row, left);
+        } else {
+            p.load(row, min(c, (int)cols), (int)cols);
+            p.fix(left);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += p.v[e];
+    }
+    if (wave) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) join[wave - 1][lane * 4 + e] = acc[e];
+    }
+    __syncthreads();
+    if (wave || left <= 0) return;
+    Piece<float> out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES - 1; ++w) acc[e] += join[w][lane * 4 + e];
+        out.v[e] = acc[e] * scale;
+    }
+    out.store(dtable + (uint64_t)key * cols + c, left);
+}
+
+// Lanes of a row.
+uint32_t sum_lanes(uint32_t cols, int v) {
+    const uint32_t pieces = ceil_div(cols, v);
+    return pieces <= 4 ? 4 : pieces <= 16 ? 16 : kWave;
+}
+
+struct Plan {
+    int passes, bits;  // of the sort
+    uint32_t keys;
+    uint32_t chunk, chunks;
+    uint64_t counts, list, partial, bytes;  // where the workspace's parts begin; four lists
+};
+
+uint64_t whole_lines(uint64_t bytes) { return (bytes + 127) / 128 * 128; }
+
+Plan plan(uint64_t n, uint32_t vocab, uint32_t cols, int32_t dtype) {
+    Plan p;
+    int bits = 0;
+    while (bits < 32 && (uint64_t)vocab >> bits) ++bits;  // the largest key is vocab itself
+    p.passes = (bits + 9) / 10;
+    p.bits = (bits + p.passes - 1) / p.passes;
+    p.keys = p.passes == 1 ? vocab + 1 : 1u << p.bits;
+    // chunks enough to fill the GPU, of rows enough that few of them are joined
+    const uint64_t most = (uint64_t)kMostChunks * (kWave / sum_lanes(cols, 16 / elem_bytes(dtype)));
+    p.chunk = kLeastChunk;
+    while ((n + p.chunk - 1) / p.chunk > most) p.chunk *= 2;
+    p.chunks = (uint32_t)((n + p.chunk - 1) / p.chunk);
+    p.counts = 0;
+    p.list = whole_lines(sort_bytes(p.keys));
+    p.partial = p.list + 4 * whole_lines(4 * n);
+    // of any smaller number of positions too
+    const uint64_t some = std::min<uint64_t>((n + kLeastChunk - 1) / kLeastChunk, most);
+    p.bytes = std::max<uint64_t>(p.partial + 8 * some * cols, 128);
+    return p;
+}
+
+int32_t check_embedding(uint64_t positions, uint32_t vocab, uint32_t cols, int32_t dtype) {
+    TATARA_REQUIRE_DTYPE(dtype);
+    TATARA_REQUIRE(vocab >= 1 && vocab <= kMaxVocab, "a table has 1 to 2^28 rows");
+    TATARA_REQUIRE(cols >= 1 && cols <= kMaxRowCols, "rows have 1 to 32768 columns");
+    TATARA_REQUIRE(positions < (1ull << 31), "too many positions");
+    return kOk;
+}
+
+}  // namespace
+}  // namespace tatara
+
+using namespace tatara;
+
+extern "C" {
+
+int32_t tatara_op_embedding_forward(const int32_t* token, uint64_t positions, const void* table, int64_t table_stride,
+                                    uint32_t vocab, uint32_t cols, float scale, void* y, int64_t y_stride,
+                                    int32_t dtype, TataraStream* stream) {
+    if (int32_t st = check_embedding(positions, vocab, cols, dtype)) return st;
+    if (positions == 0) return kOk;
+    TATARA_REQUIRE(token && table && y, "null tensor");
+    TATARA_REQUIRE(table_stride >= (int64_t)cols && y_stride >= (int64_t)cols, "a row stride is smaller than the row");
+    TATARA_REQUIRE_ALIGNED(table, elem_bytes(dtype));
+    TATARA_REQUIRE_ALIGNED(y, elem_bytes(dtype));
+    if (int32_t st = check_stream(stream)) return st;
+    return launch_rows_back(RowsBack{table, table_stride, vocab, token, nullptr, scale, y, y_stride, positions, 1, cols},
+                            dtype, raw(stream));
+}
+
+int32_t tatara_op_embedding_backward_workspace(uint64_t positions, uint32_t vocab, uint32_t cols, int32_t dtype,
+                                               uint64_t* bytes) {
+    TATARA_REQUIRE(bytes, "null output");
+    if (int32_t st = check_embedding(positions, vocab, cols, dtype)) return st;
+    *bytes = plan(positions, vocab, cols, dtype).bytes;
+    return kOk;
+}
+
+int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const int32_t* token, uint64_t positions,
+                                     uint32_t vocab, uint32_t cols, float scale, float* dtable, int32_t dtype,
+                                     void* workspace, uint64_t workspace_bytes, TataraStream* stream) {
+    if (int32_t st = check_embedding(positions, vocab, cols, dtype)) return st;
+    TATARA_REQUIRE(dtable && (!positions || (dy && token)), "null tensor");
+    TATARA_REQUIRE(!positions || dy_stride >= (int64_t)cols, "the row stride is smaller than the row");
+    TATARA_REQUIRE_ALIGNED(dy, elem_bytes(dtype));
+    const Plan p = plan(positions, vocab, cols, dtype);
+    TATARA_REQUIRE(workspace && workspace_bytes >= p.bytes, "workspace too small");
+    TATARA_REQUIRE_ALIGNED(workspace, 16);
+    if (int32_t st = check_stream(stream)) return st;
+    char* base = static_cast<char*>(workspace);
+    auto list = [&](int i) { return reinterpret_cast<uint32_t*>(base + p.list + i * whole_lines(4 * positions)); };
+    float* partial = reinterpret_cast<float*>(base + p.partial);
+    for (int i = 0; positions && i < p.passes; ++i) {
+        const int to = i % 2 * 2, from = 2 - to;
+        const Digit digit{i ? nullptr : token, list(from), list(from + 1), vocab, (uint32_t)(i * p.bits),
+                          p.passes == 1 ? ~0u : p.keys - 1, list(to), list(to + 1)};
+        if (int32_t st = launch_sort(digit, positions, p.keys, reinterpret_cast<uint32_t*>(base + p.counts), raw(stream)))
+            return st;
+    }
+    const int last = (p.passes - 1) % 2 * 2;
+    const Sorted s{list(last), list(last + 1), (uint32_t)positions, p.chunk, p.chunks};
+    const uint32_t clear = std::min(ceil_div(vocab, kClearRows), 1u << 20);
+    TATARA_FOR_DTYPE(dtype, {
+        constexpr int V = Piece<T>::V;
+        const uint32_t lanes = sum_lanes(cols, V), slabs = ceil_div(cols, lanes * V);
+        auto launch = [&](auto g, auto few) {
+            constexpr int G = decltype(g)::value;
+            const uint32_t blocks = clear + ceil_div((uint64_t)p.chunks * slabs, kThreads / G);
+            embedding_sum_kernel<T, G, decltype(few)::value><<<blocks, kThreads, 0, raw(stream)>>>(
+                static_cast<const T*>(dy), dy_stride, s, vocab, cols, scale, dtable, partial, clear, slabs);
+        };
+        using std::integral_constant;
+        if (cols < (uint32_t)V)
+            launch(integral_constant<int, 4>{}, std::true_type{});
+        else if (lanes == 4)
+            launch(integral_constant<int, 4>{}, std::false_type{});
+        else if (lanes == 16)
+            launch(integral_constant<int, 16>{}, std::false_type{});
+        else
+            launch(integral_constant<int, 64>{}, std::false_type{});
+    });
+    TATARA_LAUNCHED("embedding_sum");
+    if (p.chunks > 1) {
+        const uint32_t slabs = ceil_div(cols, kWave * 4);
+        embedding_join_kernel<<<(p.chunks - 1) * slabs, kThreads, 0, raw(stream)>>>(s, vocab, cols, scale, partial,
+                                                                                  dtable, slabs);
+        TATARA_LAUNCHED("embedding_join");
+    }
+    return kOk;
+}
+
+}  // extern "C"

@@ -1,0 +1,475 @@
+// Root-mean-square norm of rows with the residual's addition, with an output in 8
+// bits, and its gradient.
+//
+//   s = x + residual, rounded to the element type (as it is stored),
+//   rstd_r = 1 / sqrt(sum_c s^2 / C + eps),  y = s rstd w
+//   8 bits: of each group of a row's columns, scale = max(max |y|, 2^-100) / M and
+//           q = round(y / scale), M = 448 (e4m3) or 127 (whole numbers)
+//   backward: h = s rstd,  g = dy w,
+//             ds = rstd (g - h sum_c (g h) / C) + dtotal,  dw = sum_r dy h
+//
+// Every sum is f32 and in a fixed order (no atomics).
+#include "norm_rows.hpp"
+
+namespace tatara {
+namespace {
+
+// The largest of what the W waves of a row hold.
+template <int W>
+__device__ __forceinline__ uint32_t row_max(uint32_t x, uint32_t (*part)[W], int slot) {
+    x = group_join_u<(int)kWave>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+    if constexpr (W > 1) {
+        if (threadIdx.x % kWave == 0) part[slot][threadIdx.x / kWave] = x;
+        __syncthreads();
+        x = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) x = max(x, part[slot][i]);
+    }
+    return x;
+}
+
+// V values as 8-bit ones, of which the first `left` are stored.
+template <int V>
+__device__ __forceinline__ void store_8bit(uint8_t* to, const float* v, bool e4m3, int left) {
+    uint32_t word[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        if (e4m3) {
+            const int low = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
+            word[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], low, true);
+        } else {
+            word[i] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) word[i] |= ((uint32_t)(int32_t)rintf(v[4 * i + j]) & 0xffu) << (8 * j);
+        }
+    }
+    if (left >= V) {
+        __builtin_memcpy(to, word, V);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < left) to[j] = (uint8_t)(word[j / 4] >> (8 * (j % 4)));
+    }
+}
+
+// Where y goes.
+struct RmsOut {
+    void* y;  // of the element type, or of 8 bits
+    int64_t stride;
+    float* scale;     // 8 bits: [rows][groups]
+    uint32_t groups;  // of a row
+    uint32_t lanes;   // that a group lies in; 0: the whole row
+    bool e4m3;
+};
+
+// FEW: rows of fewer elements than a piece has.  BITS8: an output in 8 bits.
+// total may be x or residual: a row's loads stand ahead of its sum, and its stores
+// behind.
+template <typename T, int W, int N, bool FEW, bool ADD, bool BITS8>
+__global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
+    const T* x, int64_t x_stride, const T* residual, int64_t residual_stride, const float* __restrict__ weight,
+    T* total, int64_t total_stride, RmsOut out, float* __restrict__ rstd, uint64_t rows, uint32_t cols, float eps) {
+    constexpr int V = Piece<T>::V;
+    __shared__ float part[2][W];
+    __shared__ uint32_t part_max[2][W];
+    const uint32_t lane = threadIdx.x % (kWave * W);
+    auto column = [&](int i) { return (int)(i * kWave * W + lane) * V; };
+    auto read = [&](auto& piece, const auto* from, int i) {
+        if (FEW)
+            piece.load_few(from, (int)cols - column(i));
+        else
+            piece.load(from, column(i), (int)cols);
+    };
+    auto fix = [&](auto& piece, int i) {
+        if (!FEW) piece.fix((int)cols - column(i));
+    };
+    // more rows than the grid has room for are taken in turn
+    constexpr int G = W == 1 ? 4 : 1;
+    const uint64_t step = (uint64_t)gridDim.x * G;
+    int slot = 0;
+    for (uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / (kWave * W); row < rows; row += step, slot ^= 1) {
+        Piece<T> in[N], more[ADD ? N : 1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            read(in[i], x + (int64_t)row * x_stride, i);
+            if constexpr (ADD) read(more[i], residual + (int64_t)row * residual_stride, i);
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            fix(in[i], i);
+            if constexpr (ADD) fix(more[i], i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if constexpr (ADD) in[i].v[j] = (T)((float)in[i].v[j] + (float)more[i].v[j]);
+                const float v = (float)in[i].v[j];
+                s = fmaf(v, v, s);
+            }
+        }
+        const float r = 1.0f / sqrtf(row_sum<W>(s, part, slot) / (float)cols + eps);
+        if (lane == 0 && rstd) rstd[row] = r;
+        if constexpr (ADD) {
+            if (total) {
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    in[i].store(total + (int64_t)row * total_stride + column(i), (int)cols - column(i));
+            }
+        }
+        auto normed = [&](int i, float* y) {
+            Floats<V> w;
+            if (weight) {
+                read(w, weight, i);
+                fix(w, i);
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) y[j] = (float)in[i].v[j] * r * (weight ? w[j] : 1.0f);
+        };
+        if constexpr (!BITS8) {
+            T* to = static_cast<T*>(out.y) + (int64_t)row * out.stride;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int left = (int)cols - column(i);
+                if (left <= 0) break;
+                float y[V];
+                normed(i, y);
+                Piece<T> piece;
+#pragma unroll
+                for (int j = 0; j < V; ++j) piece.v[j] = (T)y[j];
+                piece.store(to + column(i), left);
+            }
+        } else {
+            // magnitudes as whole numbers, which order as they do, with infinity and
+            // NaN above the rest
+            float y[N][V];
+            uint32_t top[N], all = 0;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                normed(i, y[i]);
+                top[i] = 0;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const bool in_row = column(i) + j < (int)cols;  // past it a NaN of rstd shows too
+                    top[i] = max(top[i], in_row ? __float_as_uint(y[i][j]) & 0x7fffffffu : 0u);
+                }
+                all = max(all, top[i]);
+            }
+            if (out.lanes == 0) {
+                all = row_max<W>(all, part_max, slot);
+#pragma unroll
+                for (int i = 0; i < N; ++i) top[i] = all;
+            } else {
+                auto join = [&](auto s) {
+                    constexpr int S = decltype(s)::value;
+                    if (out.lanes >> S > 1) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i) top[i] = max(top[i], partner<S>(top[i]));
+                    }
+                };
+                join(std::integral_constant<int, 0>{});
+                join(std::integral_constant<int, 1>{});
+                join(std::integral_constant<int, 2>{});
+                join(std::integral_constant<int, 3>{});
+                join(std::integral_constant<int, 4>{});
+            }
+            uint8_t* to = static_cast<uint8_t*>(out.y) + (int64_t)row * out.stride;
+            const float most = out.e4m3 ? 448.0f : 127.0f;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int left = (int)cols - column(i);
+                if (left <= 0) break;
+                // a group with a value that is not finite has the scale NaN, and zeros
+                const bool finite = top[i] < 0x7f800000u;
+                const float scale = finite ? fmaxf(__uint_as_float(top[i]), 0x1p-100f) / most : __uint_as_float(0x7fc00000u);
+                // one division a group: a product is an ulp of f32 off y / scale, which
+                // shows where that lies on the border of two results; the largest, M and
+                // two ulps at most, rounds to M
+                const float inv = 1.0f / scale;
+                float v[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[j] = finite ? y[i][j] * inv : 0.0f;
+                store_8bit<V>(to + column(i), v, out.e4m3, left);
+                const uint32_t in_group = out.lanes ? lane % out.lanes : lane + i;
+                if (in_group == 0)
+                    out.scale[row * out.groups + (out.lanes ? (uint32_t)column(i) / (out.lanes * V) : 0)] = scale;
+            }
+        }
+    }
+}
+
+// dx may be dtotal, as total above.
+template <typename T, int W, int N, bool FEW, bool ADD>
+__global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_backward_kernel(
+    const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ total, int64_t total_stride,
+    const float* __restrict__ weight, const float* __restrict__ rstd, const T* dtotal, int64_t dtotal_stride, T* dx,
+    int64_t dx_stride, float* __restrict__ partial, uint64_t rows, uint32_t cols) {
+    constexpr int V = Piece<T>::V;
+    constexpr int G = W == 1 ? 4 : 1;  // rows that the workgroup has in hand
+    __shared__ float part[2][W];
+    __shared__ float join[G == 1 ? 1 : (G - 1) * kWave * N * V];
+    const uint32_t lane = threadIdx.x % (kWave * W), group = threadIdx.x / (kWave * W);
+    auto column = [&](int i) { return (int)(i * kWave * W + lane) * V; };
+    auto read = [&](auto& piece, const auto* from, int i) {
+        if (FEW)
+            piece.load_few(from, (int)cols - column(i));
+        else
+            piece.load(from, column(i), (int)cols);
+    };
+    auto fix = [&](auto& piece, int i) {
+        if (!FEW) piece.fix((int)cols - column(i));
+    };
+    // the weight stays in registers where they last
+    constexpr bool KEEP = N * V <= 24;
+    float dw[N * V];
+    Floats<V> kept[KEEP ? N : 1];
+#pragma unroll
+    for (int i = 0; i < N * V; ++i) dw[i] = 0.0f;
+    auto weights = [&](int i) {
+        Floats<V> w;
+        if (weight) {
+            read(w, weight, i);
+            fix(w, i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w.p[j / 4].v[j % 4] = 1.0f;
+        }
+        return w;
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) kept[i] = weights(i);
+    }
+    Piece<T> ps[N], pd[N], pt[ADD ? N : 1];
+    float r = 0.0f;
+    auto read_row = [&](uint64_t row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            read(ps[i], total + (int64_t)row * total_stride, i);
+            read(pd[i], dy + (int64_t)row * dy_stride, i);
+            if constexpr (ADD) read(pt[i], dtotal + (int64_t)row * dtotal_stride, i);
+        }
+        r = rstd[row];
+    };
+    int slot = 0;
+    const uint64_t step = (uint64_t)gridDim.x * G;
+    uint64_t row = (uint64_t)blockIdx.x * G + group;
+    if (row < rows) read_row(row);
+    for (; row < rows; row += step, slot ^= 1) {
+        float h[N * V], g[N * V];
+        Piece<T> add[ADD ? N : 1];
+        float sgh = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            fix(ps[i], i);
+            fix(pd[i], i);
+            if constexpr (ADD) {
+                fix(pt[i], i);
+                add[i] = pt[i];
+            }
+            const Floats<V> w = KEEP ? kept[KEEP ? i : 0] : weights(i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int e = i * V + j;
+                // past the row's end dy and s are zero; a rstd that is not finite shows there
+                const float d = (float)pd[i].v[j];
+                h[e] = column(i) + j < (int)cols ? (float)ps[i].v[j] * r : 0.0f;
+                g[e] = d * w[j];
+                sgh = fmaf(g[e], h[e], sgh);
+                dw[e] = fmaf(d, h[e], dw[e]);
+            }
+        }
+        const float scale = r;
+        // the next row's values are on their way while this one's sum is joined (behind the
+        // last row nothing uses what is read)
+        const uint64_t next = row + step;
+        read_row(next < rows ? next : row);
+        const float b = row_sum<W>(sgh, part, slot) / (float)cols;
+        T* to = dx + (int64_t)row * dx_stride;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            Piece<T> out;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float d = (g[i * V + j] - h[i * V + j] * b) * scale;
+                if constexpr (ADD)
+                    out.v[j] = (T)(d + (float)add[i].v[j]);
+                else
+                    out.v[j] = (T)d;
+            }
+            out.store(to + column(i), (int)cols - column(i));
+        }
+    }
+    if (!partial) return;
+    float* to = partial + (uint64_t)blockIdx.x * cols;
+    if constexpr (G > 1) {
+        if (group > 0) {
+#pragma unroll
+            for (int i = 0; i < N * V; ++i) join[((group - 1) * N * V + i) * kWave + lane] = dw[i];
+        }
+        __syncthreads();
+        if (group == 0) {
+#pragma unroll
+            for (int i = 0; i < N * V; ++i)
+#pragma unroll
+                for (int o = 0; o < G - 1; ++o) dw[i] += join[(o * N * V + i) * kWave + lane];
+        }
+    }
+    if (group == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = (i * kWave * W + lane) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (c + j < (int)cols) to[c + j] = dw[i * V + j];
+        }
+    }
+}
+
+uint64_t partial_bytes(uint32_t cols) { return 4ull * kGradBlocks * cols; }
+
+int32_t check_forward(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                      const void* total, int64_t total_stride, const void* y, int64_t y_stride, uint64_t rows,
+                      uint32_t cols, float eps, int32_t dtype) {
+    TATARA_REQUIRE_DTYPE(dtype);
+    TATARA_REQUIRE(cols >= 1 && cols <= kMaxCols, "RMS norm takes 1 to 32768 columns");
+    TATARA_REQUIRE(rows < (1ull << 31), "too many rows");
+    TATARA_REQUIRE(eps >= 0.0f, "eps must not be negative");
+    TATARA_REQUIRE(residual || !total, "a sum is asked for, and no residual given");
+    if (rows == 0) return kOk;
+    TATARA_REQUIRE(x && y, "null tensor");
+    TATARA_REQUIRE(x_stride >= (int64_t)cols && y_stride >= (int64_t)cols &&
+                       (!residual || residual_stride >= (int64_t)cols) && (!total || total_stride >= (int64_t)cols),
+                   "a row stride is smaller than the row");
+    TATARA_REQUIRE_ALIGNED(x, elem_bytes(dtype));
+    TATARA_REQUIRE_ALIGNED(residual, elem_bytes(dtype));
+    TATARA_REQUIRE_ALIGNED(total, elem_bytes(dtype));
+    return kOk;
+}
+
+template <bool BITS8>
+void launch_forward(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                    const float* weight, void* total, int64_t total_stride, const RmsOut& out, float* rstd,
+                    uint64_t rows, uint32_t cols, float eps, int32_t dtype, hipStream_t stream) {
+    TATARA_FOR_DTYPE(dtype, {
+        with_form<T, false>(norm_form(false, rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
+            constexpr int W = decltype(w)::value;
+            constexpr int N = decltype(n)::value;
+            constexpr bool FEW = decltype(few)::value;
+            const uint32_t blocks = (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, kMaxGrid);
+            const uint32_t threads = W == 16 ? 1024 : 256;
+            if (residual)
+                rms_forward_kernel<T, W, N, FEW, true, BITS8><<<blocks, threads, 0, stream>>>(
+                    static_cast<const T*>(x), x_stride, static_cast<const T*>(residual), residual_stride, weight,
+                    static_cast<T*>(total), total_stride, out, rstd, rows, cols, eps);
+            else
+                rms_forward_kernel<T, W, N, FEW, false, BITS8><<<blocks, threads, 0, stream>>>(
+                    static_cast<const T*>(x), x_stride, nullptr, 0, weight, nullptr, 0, out, rstd, rows, cols, eps);
+        });
+    });
+}
+
+}  // namespace
+}  // namespace tatara
+
+using namespace tatara;
+
+extern "C" {
+
+int32_t tatara_op_rms_norm_forward(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                   const float* weight, void* total, int64_t total_stride, void* y, int64_t y_stride,
+                                   float* rstd, uint64_t rows, uint32_t cols, float eps, int32_t dtype,
+                                   TataraStream* stream) {
+    if (int32_t st = check_forward(x, x_stride, residual, residual_stride, total, total_stride, y, y_stride, rows,
+                                   cols, eps, dtype))
+        return st;
+    TATARA_REQUIRE_ALIGNED(y, elem_bytes(dtype));
+    if (rows == 0) return kOk;
+    if (int32_t st = check_stream(stream)) return st;
+    launch_forward<false>(x, x_stride, residual, residual_stride, weight, total, total_stride,
+                          RmsOut{y, y_stride, nullptr, 0, 0, false}, rstd, rows, cols, eps, dtype, raw(stream));
+    TATARA_LAUNCHED("rms_forward");
+    return kOk;
+}
+
+int32_t tatara_op_rms_norm_forward_8bit(const void* x, int64_t x_stride, const void* residual,
+                                        int64_t residual_stride, const float* weight, void* total,
+                                        int64_t total_stride, void* q, int64_t q_stride, float* scale, float* rstd,
+                                        uint64_t rows, uint32_t cols, uint32_t group, float eps, int32_t dtype,
+                                        int32_t format, TataraStream* stream) {
+    TATARA_REQUIRE(format == TATARA_E4M3 || format == TATARA_I8, "unknown 8-bit format");
+    TATARA_REQUIRE(group == 0 || group == 32 || group == 64 || group == 128,
+                   "a scale stands for 32, 64 or 128 columns, or for a row (0)");
+    if (int32_t st = check_forward(x, x_stride, residual, residual_stride, total, total_stride, q, q_stride, rows,
+                                   cols, eps, dtype))
+        return st;
+    if (rows == 0) return kOk;
+    TATARA_REQUIRE(scale, "null tensor");
+    if (int32_t st = check_stream(stream)) return st;
+    const uint32_t v = 16 / elem_bytes(dtype);
+    launch_forward<true>(x, x_stride, residual, residual_stride, weight, total, total_stride,
+                         RmsOut{q, q_stride, scale, group ? ceil_div(cols, group) : 1, group / v,
+                                format == TATARA_E4M3},
+                         rstd, rows, cols, eps, dtype, raw(stream));
+    TATARA_LAUNCHED("rms_forward_8bit");
+    return kOk;
+}
+
+int32_t tatara_op_rms_norm_backward_workspace(uint32_t cols, uint64_t* bytes) {
+    TATARA_REQUIRE(bytes, "null output");
+    TATARA_REQUIRE(cols >= 1 && cols <= kMaxCols, "RMS norm takes 1 to 32768 columns");
+    *bytes = partial_bytes(cols);
+    return kOk;
+}
+
+int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride, const void* total, int64_t total_stride,
+                                    const float* weight, const float* rstd, const void* dtotal,
+                                    int64_t dtotal_stride, void* dx, int64_t dx_stride, float* dweight, uint64_t rows,
+                                    uint32_t cols, int32_t dtype, void* workspace, uint64_t workspace_bytes,
+                                    TataraStream* stream) {
+    TATARA_REQUIRE_DTYPE(dtype);
+    TATARA_REQUIRE(cols >= 1 && cols <= kMaxCols, "RMS norm takes 1 to 32768 columns");
+    TATARA_REQUIRE(rows < (1ull << 31), "too many rows");
+    TATARA_REQUIRE(!dweight || (workspace && workspace_bytes >= partial_bytes(cols)), "workspace too small");
+    TATARA_REQUIRE_ALIGNED(workspace, 16);
+    if (rows) {
+        TATARA_REQUIRE(dy && total && rstd && dx, "null tensor");
+        TATARA_REQUIRE(dy_stride >= (int64_t)cols && total_stride >= (int64_t)cols && dx_stride >= (int64_t)cols &&
+                           (!dtotal || dtotal_stride >= (int64_t)cols),
+                       "a row stride is smaller than the row");
+        TATARA_REQUIRE_ALIGNED(dy, elem_bytes(dtype));
+        TATARA_REQUIRE_ALIGNED(total, elem_bytes(dtype));
+        TATARA_REQUIRE_ALIGNED(dtotal, elem_bytes(dtype));
+        TATARA_REQUIRE_ALIGNED(dx, elem_bytes(dtype));
+    }
+    if (int32_t st = check_stream(stream)) return st;
+    float* partial = dweight ? static_cast<float*>(workspace) : nullptr;
+    uint32_t blocks = 0;
+    if (rows) {
+        TATARA_FOR_DTYPE(dtype, {
+            with_form<T, true>(norm_form(true, rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
+                constexpr int W = decltype(w)::value;
+                constexpr int N = decltype(n)::value;
+                constexpr bool FEW = decltype(few)::value;
+                blocks = grad_blocks(W == 1 ? (rows + 3) / 4 : rows);
+                const uint32_t threads = W == 16 ? 1024 : 256;
+                if (dtotal)
+                    rms_backward_kernel<T, W, N, FEW, true><<<blocks, threads, 0, raw(stream)>>>(
+                        static_cast<const T*>(dy), dy_stride, static_cast<const T*>(total), total_stride, weight, rstd,
+                        static_cast<const T*>(dtotal), dtotal_stride, static_cast<T*>(dx), dx_stride, partial, rows,
+                        cols);
+                else
+                    rms_backward_kernel<T, W, N, FEW, false><<<blocks, threads, 0, raw(stream)>>>(
+                        static_cast<const T*>(dy), dy_stride, static_cast<const T*>(total), total_stride, weight, rstd,
+                        nullptr, 0, static_cast<T*>(dx), dx_stride, partial, rows, cols);
+            });
+        });
+        TATARA_LAUNCHED("rms_backward");
+    }
+    if (dweight) {
+        norm_param_grad_kernel<<<ceil_div(cols, kWave), 1024, 0, raw(stream)>>>(partial, blocks, cols, cols, dweight,
+                                                                                nullptr);
+        TATARA_LAUNCHED("rms_weight_grad");
+    }
+    return kOk;
+}
+
+}  // extern "C"

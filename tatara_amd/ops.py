@@ -7,12 +7,18 @@ balanced (`BucketGate`), and Newton-Schulz orthogonalised updates of weight
 matrices (`Orthogonaliser`, `Muon`), over the C ABI (tatara_op_layer_norm_*,
 tatara_op_bucket_gate_*, tatara_op_orthogonalise, tatara_op_muon_step).
 
+Around the layers that are chosen stand an embedding of a position's discrete values
+(`Embedding`), dropout (`Dropout`), a root-mean-square norm with the residual's addition
+and an output in 8 bits (`RMSNorm`), and the rows of each bucket side by side and
+back (`BucketRows`): tatara_op_embedding_*, tatara_op_dropout, tatara_op_rms_norm_*,
+tatara_op_bucket_rows_*.
+
 An operator is made once for a layer's shape and holds its workspace.  Tensors
 are device memory: a `DeviceArray`, or any object with data_ptr(), shape,
 stride(), dtype, get_device() and is_contiguous() (a torch tensor on the GPU; torch is
 imported before the library is loaded, so that both run on one HIP runtime).  The last
 dimension is contiguous; rows may lie inside wider ones.  An operator's element
-type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16.  Calls queue
+type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16 (and e4m3 as uint8).  Calls queue
 their work on `stream` (a runtime.Stream or a torch.cuda.Stream; None is torch's
 current stream where the call's first tensor is torch's, else the null stream) and return;
 one operator's calls belong on one stream at a time, since they share the
@@ -32,7 +38,11 @@ from ._lib import check
 DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
 # names of array types -> the element type that they hold
 _HOLDS = {"float32": "f32", "torch.float32": "f32", "float16": "f16", "torch.float16": "f16", "uint16": "bf16",
-          "torch.bfloat16": "bf16", "int32": "i32", "torch.int32": "i32", "uint8": "u8", "torch.uint8": "u8"}
+          "torch.bfloat16": "bf16", "int32": "i32", "torch.int32": "i32", "uint8": "u8", "torch.uint8": "u8",
+          "int8": "i8", "torch.int8": "i8", "torch.float8_e4m3fn": "e4m3", "uint64": "u64", "torch.uint64": "u64",
+          "int64": "u64", "torch.int64": "u64"}
+# DeviceArray types that stand in for one that numpy lacks
+_STANDS_FOR = {"u8": "e4m3"}
 
 
 class _TypeNames(dict):
@@ -182,7 +192,8 @@ def _count(name: str, x, cols: int, dtype: str) -> int:
 
 def _owned(name: str, x, shape: tuple, dtype: str) -> int:
     """The address of a DeviceArray of this shape."""
-    if hasattr(x, "data_ptr") or not hasattr(x, "ptr") or tuple(x.shape) != shape or _TYPE[x.dtype] != dtype:
+    if hasattr(x, "data_ptr") or not hasattr(x, "ptr") or tuple(x.shape) != shape or not (
+            _TYPE[x.dtype] == dtype or _STANDS_FOR.get(_TYPE[x.dtype]) == dtype):
         _wrong(name, x, shape, dtype)
     return x.ptr
 
@@ -394,3 +405,293 @@ class Muon(_Operator):
             _dense("grad", grad, shape, self.grad_dtype, here), o.batch, o.rows, o.cols, self._grad_code, self.beta,
             self.nesterov, lr, self.weight_decay, scale, self.min_w, self.max_w, o.steps,
             (ws := self._ws[here]).ptr, ws.nbytes, queue))
+
+
+class RMSNorm(_Operator):
+    """y = s * rstd * weight over rows of `cols` values, with s = x + residual.
+
+    x, residual, total (s as it is stored, which is what is normalised), y, dy,
+    dtotal and dx are [rows, cols] of `dtype`; weight, rstd and dweight are f32, and
+    weight may be None.  forward_8bit writes y as q [rows, cols] of `out8` ("e4m3" or
+    "i8") and scale f32 [rows, groups], y being about q * scale; a scale stands for
+    `group` columns (32, 64 or 128), or for the row (0)."""
+
+    def __init__(self, cols: int, dtype: str = "f32", eps: float = 1e-6, out8: str = "e4m3", group: int = 0):
+        self.cols, self.dtype, self.eps, self.out8, self.group = int(cols), dtype, float(eps), out8, int(group)
+        self._code = _dtype(dtype)
+        if not 1 <= self.cols <= 32768:
+            raise ValueError(f"cols must be 1 to 32768, not {cols}")
+        if not self.eps >= 0.0:
+            raise ValueError(f"eps must not be negative, not {eps}")
+        if out8 not in ("e4m3", "i8"):
+            raise ValueError(f"out8 must be e4m3 or i8, not {out8!r}")
+        if self.group not in (0, 32, 64, 128):
+            raise ValueError(f"group must be 0, 32, 64 or 128, not {group}")
+        self.groups = -(-self.cols // self.group) if self.group else 1
+        self._format = ("e4m3", "i8").index(out8)
+        self._lib = _lib.load()
+        n = C.c_uint64()
+        check(self._lib.tatara_op_rms_norm_backward_workspace(self.cols, C.byref(n)))
+        self._ws = _Workspaces(n.value)
+
+    def _sum(self, shape, residual, total, here):
+        """Addresses and strides of residual and total."""
+        if residual is None:
+            if total is not None:
+                raise ValueError("total needs a residual")
+            return None, 0, None, 0
+        rp, rs = _rows("residual", residual, shape, self.dtype, here)
+        return (rp, rs, None, 0) if total is None else (rp, rs, *_rows("total", total, shape, self.dtype, here))
+
+    def forward(self, x, weight, y, rstd=None, residual=None, total=None, stream=None) -> None:
+        """Writes y, rstd [rows] for the backward pass if given, and the sum of x and
+        residual into total if given (which may be x or residual)."""
+        cols = self.cols
+        here, queue = _place(x, stream)
+        rows = _count("x", x, cols, self.dtype)
+        shape = (rows, cols)
+        xp, xs = _rows("x", x, shape, self.dtype, here)
+        yp, ys = _rows("y", y, shape, self.dtype, here)
+        rp, rs, tp, ts = self._sum(shape, residual, total, here)
+        status = self._lib.tatara_op_rms_norm_forward(
+            xp, xs, rp, rs, None if weight is None else _dense("weight", weight, (cols,), "f32", here), tp, ts, yp, ys,
+            None if rstd is None else _dense("rstd", rstd, (rows,), "f32", here), rows, cols, self.eps, self._code,
+            queue)
+        if status:
+            check(status)
+
+    def forward_8bit(self, x, weight, q, scale, rstd=None, residual=None, total=None, stream=None) -> None:
+        """forward() with y as q and scale."""
+        cols = self.cols
+        here, queue = _place(x, stream)
+        rows = _count("x", x, cols, self.dtype)
+        shape = (rows, cols)
+        xp, xs = _rows("x", x, shape, self.dtype, here)
+        qp, qs = _rows("q", q, shape, self.out8, here)
+        rp, rs, tp, ts = self._sum(shape, residual, total, here)
+        status = self._lib.tatara_op_rms_norm_forward_8bit(
+            xp, xs, rp, rs, None if weight is None else _dense("weight", weight, (cols,), "f32", here), tp, ts, qp, qs,
+            _dense("scale", scale, (rows, self.groups), "f32", here),
+            None if rstd is None else _dense("rstd", rstd, (rows,), "f32", here), rows, cols, self.group, self.eps,
+            self._code, self._format, queue)
+        if status:
+            check(status)
+
+    def backward(self, dy, total, weight, rstd, dx, dweight=None, dtotal=None, stream=None) -> None:
+        """Writes dx, the gradient of x and residual alike, from dy and, if given, the
+        gradient dtotal that reaches the sum by itself (dx may be dtotal), and the
+        weight's gradient [cols] if given (overwritten)."""
+        cols, dtype = self.cols, self.dtype
+        here, queue = _place(total, stream)
+        rows = _count("total", total, cols, dtype)
+        shape = (rows, cols)
+        dyp, dys = _rows("dy", dy, shape, dtype, here)
+        tp, ts = _rows("total", total, shape, dtype, here)
+        dxp, dxs = _rows("dx", dx, shape, dtype, here)
+        dtp, dts = (None, 0) if dtotal is None else _rows("dtotal", dtotal, shape, dtype, here)
+        status = self._lib.tatara_op_rms_norm_backward(
+            dyp, dys, tp, ts, None if weight is None else _dense("weight", weight, (cols,), "f32", here),
+            _dense("rstd", rstd, (rows,), "f32", here), dtp, dts, dxp, dxs,
+            None if dweight is None else _dense("dweight", dweight, (cols,), "f32", here), rows, cols, self._code,
+            (ws := self._ws[here]).ptr, ws.nbytes, queue)
+        if status:
+            check(status)
+
+
+class Dropout:
+    """y = x / (1 - p) where a number of the counter-based generator says so, else 0,
+    plus a residual: [rows, cols] of `dtype`.
+
+    The number of a value goes by `seed`, the call's step, its row (from first_row on, for
+    a part of a batch) and its column alone, so backward() makes the mask again.  A layer
+    has a seed of its own, and a training step a step of its own."""
+
+    def __init__(self, cols: int, p: float, dtype: str = "f32", seed: int = 0):
+        self.cols, self.p, self.dtype, self.seed = int(cols), float(p), dtype, int(seed)
+        self._code = _dtype(dtype)
+        if not 1 <= self.cols <= 1 << 24:
+            raise ValueError(f"cols must be 1 to 2^24, not {cols}")
+        if not 0.0 <= self.p < 1.0:
+            raise ValueError(f"p must be in [0, 1), not {p}")
+        if not 0 <= self.seed < 1 << 64:
+            raise ValueError(f"seed must be 0 to 2^64 - 1, not {seed}")
+        self._lib = _lib.load()
+
+    def forward(self, x, y, step: int = 0, residual=None, more_steps=None, first_row: int = 0, stream=None) -> None:
+        """Writes y.  The step is `step` plus more_steps ([1], int64) if that is given,
+        which is read when the call runs."""
+        here, queue = _place(x, stream)
+        rows = _count("x", x, self.cols, self.dtype)
+        shape = (rows, self.cols)
+        if not 0 <= step < 1 << 64:
+            raise ValueError(f"step must be 0 to 2^64 - 1, not {step}")
+        if not 0 <= first_row <= (1 << 32) - 1:
+            raise ValueError(f"first_row must be 0 to 2^32 - 1, not {first_row}")
+        xp, xs = _rows("x", x, shape, self.dtype, here)
+        yp, ys = _rows("y", y, shape, self.dtype, here)
+        rp, rs = (None, 0) if residual is None else _rows("residual", residual, shape, self.dtype, here)
+        status = self._lib.tatara_op_dropout(
+            xp, xs, rp, rs, yp, ys, rows, self.cols, self.p, self.seed, step,
+            None if more_steps is None else _dense("more_steps", more_steps, (1,), "u64", here), first_row,
+            self._code, queue)
+        if status:
+            check(status)
+
+    def backward(self, dy, dx, step: int = 0, more_steps=None, first_row: int = 0, stream=None) -> None:
+        """Writes dx of the forward call with the same step (the residual's gradient is
+        dy itself)."""
+        self.forward(dy, dx, step, None, more_steps, first_row, stream)
+
+
+class BucketRows(_Operator):
+    """The rows of each of `buckets` side by side, for its layers, and back in the
+    positions' order.
+
+    sort() takes a gate's choices, bucket [positions, top_k], and gives each a row:
+    slot [positions, top_k], source [rows(positions)] (position * top_k + choice) and
+    offset [buckets + 1] (choices of buckets below), all int32.  Packed (capacity None), bucket e
+    has rows offset[e] to offset[e + 1] - 1; with a capacity it has rows e * capacity
+    to (e + 1) * capacity - 1, and choices that do not fit have none.  -1 stands in slot for
+    a choice without a row (a bucket of -1 is none) and in source for a row without a
+    choice.  Rows and positions are [.., cols] of `dtype`; gate and dgate are f32."""
+
+    def __init__(self, buckets: int, cols: int, top_k: int = 1, dtype: str = "f32", capacity: int | None = None):
+        self.buckets, self.cols, self.top_k, self.dtype = int(buckets), int(cols), int(top_k), dtype
+        self.capacity = None if capacity is None else int(capacity)
+        self._code = _dtype(dtype)
+        if not 1 <= self.buckets <= 1024:
+            raise ValueError(f"buckets must be 1 to 1024, not {buckets}")
+        if not 1 <= self.cols <= 32768:
+            raise ValueError(f"cols must be 1 to 32768, not {cols}")
+        if not 1 <= self.top_k <= 16:
+            raise ValueError(f"top_k must be 1 to 16, not {top_k}")
+        if self.capacity is not None and not 1 <= self.capacity * self.buckets < 1 << 31:
+            raise ValueError(f"capacity must be at least 1 and buckets * capacity below 2^31, not {capacity}")
+        self._lib = _lib.load()
+        n = C.c_uint64()
+        check(self._lib.tatara_op_bucket_rows_workspace(self.buckets, C.byref(n)))
+        self._ws = _Workspaces(n.value)
+
+    def rows(self, positions: int) -> int:
+        """The rows of so many positions, those without a choice among them."""
+        return positions * self.top_k if self.capacity is None else self.buckets * self.capacity
+
+    def sort(self, bucket, slot, source, offset, stream=None) -> None:
+        """Writes slot, source and offset."""
+        here, queue = _place(bucket, stream)
+        n = _count("bucket", bucket, self.top_k, "i32")
+        chosen = (n, self.top_k)
+        ws = self._ws[here]
+        status = self._lib.tatara_op_bucket_rows_sort(
+            _dense("bucket", bucket, chosen, "i32", here), n, self.buckets, self.top_k, self.capacity or 0,
+            _dense("slot", slot, chosen, "i32", here), _dense("source", source, (self.rows(n),), "i32", here),
+            _dense("offset", offset, (self.buckets + 1,), "i32", here), ws.ptr, ws.nbytes, queue)
+        if status:
+            check(status)
+
+    def gather(self, x, slot, source, rows, stream=None) -> None:
+        """Writes rows: x at its positions' slots, zeros without a choice."""
+        here, queue = _place(x, stream)
+        n = _count("x", x, self.cols, self.dtype)
+        m = self.rows(n)
+        xp, xs = _rows("x", x, (n, self.cols), self.dtype, here)
+        rp, rs = _rows("rows", rows, (m, self.cols), self.dtype, here)
+        status = self._lib.tatara_op_bucket_rows_gather(
+            xp, xs, _dense("slot", slot, (n, self.top_k), "i32", here), _dense("source", source, (m,), "i32", here), n,
+            self.top_k, rp, rs, m, self.cols, self._code, queue)
+        if status:
+            check(status)
+
+    def gather_backward(self, drows, slot, dx, stream=None) -> None:
+        """Writes dx: the sum of drows at each position's slots."""
+        self.combine(drows, slot, None, dx, stream)
+
+    def combine(self, rows, slot, gate, y, stream=None) -> None:
+        """Writes y: the sum of rows at each position's slots, times gate
+        [positions, top_k] unless that is None."""
+        here, queue = _place(rows, stream)
+        n = _count("y", y, self.cols, self.dtype)
+        m = self.rows(n)
+        rp, rs = _rows("rows", rows, (m, self.cols), self.dtype, here)
+        yp, ys = _rows("y", y, (n, self.cols), self.dtype, here)
+        chosen = (n, self.top_k)
+        status = self._lib.tatara_op_bucket_rows_combine(
+            rp, rs, m, _dense("slot", slot, chosen, "i32", here),
+            None if gate is None else _dense("gate", gate, chosen, "f32", here), n, self.top_k, yp, ys, self.cols,
+            self._code, queue)
+        if status:
+            check(status)
+
+    def combine_backward(self, dy, rows, slot, source, gate, drows, dgate=None, stream=None) -> None:
+        """Writes drows, and the gate's gradient if given; rows (the forward call's) may
+        be None without it."""
+        here, queue = _place(dy, stream)
+        n = _count("dy", dy, self.cols, self.dtype)
+        m = self.rows(n)
+        dyp, dys = _rows("dy", dy, (n, self.cols), self.dtype, here)
+        rp, rs = (None, 0) if rows is None and dgate is None else _rows("rows", rows, (m, self.cols), self.dtype, here)
+        drp, drs = _rows("drows", drows, (m, self.cols), self.dtype, here)
+        chosen = (n, self.top_k)
+        status = self._lib.tatara_op_bucket_rows_combine_backward(
+            dyp, dys, rp, rs, m, _dense("slot", slot, chosen, "i32", here),
+            _dense("source", source, (m,), "i32", here), _dense("gate", gate, chosen, "f32", here), n, self.top_k, drp,
+            drs, None if dgate is None else _dense("dgate", dgate, chosen, "f32", here), self.cols, self._code, queue)
+        if status:
+            check(status)
+
+
+class Embedding(_Operator):
+    """y = scale * table[token]: rows of a table [vocab, cols] by a position's token.
+
+    token is int32 [positions]; one outside 0..vocab - 1, such as -1, stands for none: its
+    row is zeros, and it has no gradient.  table, y and dy are of `dtype`, dtable is f32.
+    `positions` is the most that a backward call takes."""
+
+    def __init__(self, vocab: int, cols: int, positions: int, dtype: str = "f32", scale: float = 1.0):
+        self.vocab, self.cols, self.positions, self.dtype = int(vocab), int(cols), int(positions), dtype
+        self.scale = float(scale)
+        self._code = _dtype(dtype)
+        if not 1 <= self.vocab <= 1 << 28:
+            raise ValueError(f"vocab must be 1 to 2^28, not {vocab}")
+        if not 1 <= self.cols <= 32768:
+            raise ValueError(f"cols must be 1 to 32768, not {cols}")
+        if not 0 <= self.positions < 1 << 31:
+            raise ValueError(f"positions must be 0 to 2^31 - 1, not {positions}")
+        self._lib = _lib.load()
+        n = C.c_uint64()
+        check(self._lib.tatara_op_embedding_backward_workspace(self.positions, self.vocab, self.cols, self._code,
+                                                               C.byref(n)))
+        self._ws = _Workspaces(n.value)
+
+    def _tokens(self, token) -> int:
+        try:
+            n, = token.shape
+            return n
+        except (AttributeError, TypeError, ValueError):
+            _wrong("token", token, ("positions",), "i32")
+
+    def forward(self, token, table, y, stream=None) -> None:
+        """Writes y [positions, cols]."""
+        here, queue = _place(token, stream)
+        n = self._tokens(token)
+        tp, ts = _rows("table", table, (self.vocab, self.cols), self.dtype, here)
+        yp, ys = _rows("y", y, (n, self.cols), self.dtype, here)
+        status = self._lib.tatara_op_embedding_forward(
+            _dense("token", token, (n,), "i32", here), n, tp, ts, self.vocab, self.cols, self.scale, yp, ys,
+            self._code, queue)
+        if status:
+            check(status)
+
+    def backward(self, dy, token, dtable, stream=None) -> None:
+        """Writes dtable [vocab, cols] (overwritten)."""
+        here, queue = _place(token, stream)
+        n = self._tokens(token)
+        if n > self.positions:
+            raise ValueError(f"a backward call takes up to {self.positions} positions, not {n}")
+        dp, ds = _rows("dy", dy, (n, self.cols), self.dtype, here)
+        ws = self._ws[here]
+        status = self._lib.tatara_op_embedding_backward(
+            dp, ds, _dense("token", token, (n,), "i32", here), n, self.vocab, self.cols, self.scale,
+            _dense("dtable", dtable, (self.vocab, self.cols), "f32", here), self._code, ws.ptr, ws.nbytes, queue)
+        if status:
+            check(status)

@@ -163,7 +163,13 @@ __global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t 
                     Piece<T> out = p[u];
                     if (a.gate) {
 #pragma unroll
-                        for (int e = 0; e < V; ++e) out.v[e] = (T)(w[j] * (float)p[u].v[e]);
+                        for (int e = 0; e < V; ++e) {
+                            float v = w[j] * (float)p[u].v[e];
+                            // f16: kept from becoming one instruction that rounds once where others
+                            // round twice, so that drows is the same with and without dgate
+                            asm("" : "+v"(v));
+                            out.v[e] = (T)v;
+                        }
                     }
                     out.store(rows + at[j] * a.rows_stride + c, cols - c);
                 }

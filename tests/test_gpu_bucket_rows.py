@@ -1,5 +1,6 @@
-"""Rows by bucket and back on the GPU.  Places are whole numbers and rows copies or one
-rounded product: equal.  Sums are f32, a choice or a column after the other."""
+"""Rows by bucket and back on the GPU.  Places are whole numbers and gathered rows copies:
+equal, as are products, rounded in f32 and then to the type.  Sums are f32, a choice or a column
+after the other."""
 import numpy as np
 import pytest
 import torch

@@ -23,8 +23,10 @@ struct Choices {
     uint64_t n_rows;
     uint32_t capacity;  // 0: packed
 
-    __device__ __forceinline__ uint32_t key(uint64_t i) const { return min((uint32_t)bucket[i], kMaxKeys); }
-    __device__ __forceinline__ void put(uint64_t i, uint32_t e, uint32_t first, uint32_t rank) const {
+    using Item = uint32_t;
+    __device__ __forceinline__ Item load(uint64_t i) const { return (uint32_t)bucket[i]; }
+    __device__ __forceinline__ uint32_t key(Item e) const { return e; }
+    __device__ __forceinline__ void put(uint64_t i, Item, uint32_t e, uint32_t first, uint32_t rank) const {
         const bool fits = !capacity || rank < capacity;
         const uint32_t row = capacity ? e * capacity + rank : first + rank;
         slot[i] = fits ? (int32_t)row : -1;

@@ -33,13 +33,17 @@ struct Digit {
     uint32_t* out_key;
     uint32_t* out_at;
 
-    __device__ __forceinline__ uint32_t whole(uint64_t i) const {
-        return token ? min((uint32_t)token[i], vocab) : in_key[i];
+    struct Item {
+        uint32_t whole, at;
+    };
+    __device__ __forceinline__ Item load(uint64_t i) const {
+        if (token) return {min((uint32_t)token[i], vocab), (uint32_t)i};
+        return {in_key[i], in_at[i]};
     }
-    __device__ __forceinline__ uint32_t key(uint64_t i) const { return whole(i) >> shift & mask; }
-    __device__ __forceinline__ void put(uint64_t i, uint32_t, uint32_t first, uint32_t rank) const {
-        out_key[first + rank] = whole(i);
-        out_at[first + rank] = token ? (uint32_t)i : in_at[i];
+    __device__ __forceinline__ uint32_t key(Item item) const { return item.whole >> shift & mask; }
+    __device__ __forceinline__ void put(uint64_t, Item item, uint32_t, uint32_t first, uint32_t rank) const {
+        out_key[first + rank] = item.whole;
+        out_at[first + rank] = item.at;
     }
     __device__ __forceinline__ void drop(uint64_t) const {}
     __device__ __forceinline__ void finish(const uint32_t*, uint32_t) const {}
@@ -52,8 +56,8 @@ struct Sorted {
 };
 
 // A group of G lanes adds the rows of a chunk, V columns a lane; rows wider than a wave
-// are cut into `slabs`.  The first `clear` workgroups write the rows of the table that no
-// position has.
+// are cut into `slabs`.  `clear` workgroups write the rows of the table that no position
+// has.
 template <typename T, int G, bool FEW>
 __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __restrict__ dy, int64_t dy_stride, Sorted s,
                                                                  uint32_t vocab, uint32_t cols, float scale,
@@ -61,10 +65,13 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
                                                                  float* __restrict__ partial, uint32_t clear,
                                                                  uint32_t slabs) {
     constexpr int V = Piece<T>::V;
-    if (blockIdx.x < clear) {
+    // the workgroups that clear lie evenly among the others, which read where they write
+    const uint32_t cleared = (uint32_t)((uint64_t)blockIdx.x * clear / gridDim.x);
+    const bool clears = cleared != (uint32_t)((uint64_t)(blockIdx.x + 1) * clear / gridDim.x);
+    if (clears) {
         __shared__ bool none[kClearRows];
         const uint32_t per_row = (cols + 3) / 4;
-        for (uint64_t first = (uint64_t)blockIdx.x * kClearRows; first < vocab; first += (uint64_t)clear * kClearRows) {
+        for (uint64_t first = (uint64_t)cleared * kClearRows; first < vocab; first += (uint64_t)clear * kClearRows) {
             __syncthreads();
             if (threadIdx.x < kClearRows) {
                 const uint64_t v = first + threadIdx.x;
@@ -89,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
         }
         return;
     }
-    uint32_t unit = (blockIdx.x - clear) * (kThreads / G) + threadIdx.x / G;
+    uint32_t unit = (blockIdx.x - cleared) * (kThreads / G) + threadIdx.x / G;
     if (G == kWave) unit = __builtin_amdgcn_readfirstlane(unit);
     const uint32_t chunk = unit / slabs;
     if (chunk >= s.chunks) return;
@@ -148,58 +155,82 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
     if (open) flush(partial + ((uint64_t)chunk * 2 + began) * cols, 1.0f);
 }
 
-// The rows of tokens that reach over several chunks: a workgroup a chunk in which one
-// begins and 256 columns, four waves that each add a quarter of the chunks.
+// The rows of tokens that reach over several chunks, of 256 columns.  A wave looks at a
+// chunk: where a token begins in it and goes on, it adds the sums of the chunks that the
+// token is in, and if they are many the workgroup's waves take a quarter of them each.
 __global__ __launch_bounds__(kThreads) void embedding_join_kernel(Sorted s, uint32_t vocab, uint32_t cols, float scale,
                                                                   const float* __restrict__ partial,
                                                                   float* __restrict__ dtable, uint32_t slabs) {
-    constexpr uint32_t WAVES = kThreads / kWave;
+    constexpr uint32_t WAVES = kThreads / kWave, FEW = 16;
     __shared__ float join[WAVES - 1][kWave * 4];
-    const uint32_t chunk = blockIdx.x / slabs, begin = chunk * s.chunk, next = begin + s.chunk;
-    if (next >= s.n) return;
-    const uint32_t key = s.key[next];
-    if (key >= vocab || s.key[next - 1] != key || (begin > 0 && s.key[begin - 1] == key)) return;
-    // chunks behind this one that begin with the token
-    uint32_t more = 0;
-    for (;;) {
-        const uint64_t place = (uint64_t)next + (uint64_t)(more + threadIdx.x) * s.chunk;
-        const uint32_t got = (uint32_t)__syncthreads_count(place < s.n && s.key[place < s.n ? place : 0] == key);
-        more += got;
-        if (got < kThreads) break;
-    }
-    const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const int c = (int)((blockIdx.x - chunk * slabs) * kWave + lane) * 4, left = (int)cols - c;
-    const uint32_t terms = more + 1, from = (uint32_t)((uint64_t)terms * wave / WAVES),
-                   to = (uint32_t)((uint64_t)terms * (wave + 1) / WAVES);
-    float acc[4] = {};
-    const bool few = cols < 4;
+    __shared__ uint32_t many[WAVES];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const uint32_t four = blockIdx.x / slabs * WAVES;
+    const int c = (int)((blockIdx.x % slabs) * kWave + lane) * 4, left = (int)cols - c;
+    // the chunks that the token is in which begins in this one, 0 if it ends there
+    auto chain = [&](uint32_t chunk) {
+        const uint64_t begin = (uint64_t)chunk * s.chunk, next = begin + s.chunk;
+        if (next >= s.n) return 0u;
+        const uint32_t key = s.key[next];
+        if (key >= vocab || s.key[next - 1] != key || (begin > 0 && s.key[begin - 1] == key)) return 0u;
+        uint32_t more = 0, got;
+        do {
+            const uint64_t place = next + (uint64_t)(more + lane) * s.chunk;
+            got = (uint32_t)__popcll(__ballot(place < s.n && s.key[place < s.n ? place : 0] == key));
+            more += got;
+        } while (got == kWave);
+        return more + 1;
+    };
+    float acc[4];
+    auto add = [&](uint32_t chunk, uint32_t from, uint32_t to) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = 0.0f;
 #pragma unroll 8
-    for (uint32_t t = from; t < to; ++t) {
-        const float* row = partial + ((uint64_t)(chunk + t) * 2 + (t == 0)) * cols;
-        Piece<float> p;
-        if (few) {
-            p.load_few(row, left);
-        } else {
-            p.load(row, min(c, (int)cols), (int)cols);
-            p.fix(left);
+        for (uint32_t t = from; t < to; ++t) {
+            const float* row = partial + ((uint64_t)(chunk + t) * 2 + (t == 0)) * cols;
+            Piece<float> p;
+            if (cols < 4) {
+                p.load_few(row, left);
+            } else {
+                p.load(row, min(c, (int)cols), (int)cols);
+                p.fix(left);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += p.v[e];
         }
+    };
+    auto write = [&](uint32_t chunk) {
+        if (left <= 0) return;
+        Piece<float> out;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += p.v[e];
+        for (int e = 0; e < 4; ++e) out.v[e] = acc[e] * scale;
+        out.store(dtable + (uint64_t)s.key[(uint64_t)(chunk + 1) * s.chunk] * cols + c, left);
+    };
+    const uint32_t mine = chain(four + wave);
+    if (mine && mine <= FEW) {
+        add(four + wave, 0, mine);
+        write(four + wave);
     }
-    if (wave) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) join[wave - 1][lane * 4 + e] = acc[e];
-    }
+    if (lane == 0) many[wave] = mine > FEW ? mine : 0;
     __syncthreads();
-    if (wave || left <= 0) return;
-    Piece<float> out;
+    for (uint32_t w = 0; w < WAVES; ++w) {
+        const uint32_t terms = many[w];
+        if (!terms) continue;
+        add(four + w, (uint32_t)((uint64_t)terms * wave / WAVES), (uint32_t)((uint64_t)terms * (wave + 1) / WAVES));
+        if (wave) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 4; ++e) join[wave - 1][lane * 4 + e] = acc[e];
+        }
+        __syncthreads();
+        if (!wave) {
 #pragma unroll
-        for (uint32_t w = 0; w < WAVES - 1; ++w) acc[e] += join[w][lane * 4 + e];
-        out.v[e] = acc[e] * scale;
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (uint32_t o = 0; o < WAVES - 1; ++o) acc[e] += join[o][lane * 4 + e];
+            write(four + w);
+        }
+        __syncthreads();
     }
-    out.store(dtable + (uint64_t)key * cols + c, left);
 }
 
 // Lanes of a row.
@@ -321,7 +352,7 @@ int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const in
     TATARA_LAUNCHED("embedding_sum");
     if (p.chunks > 1) {
         const uint32_t slabs = ceil_div(cols, kWave * 4);
-        embedding_join_kernel<<<(p.chunks - 1) * slabs, kThreads, 0, raw(stream)>>>(s, vocab, cols, scale, partial,
+        embedding_join_kernel<<<ceil_div(p.chunks - 1, kThreads / kWave) * slabs, kThreads, 0, raw(stream)>>>(s, vocab, cols, scale, partial,
                                                                                   dtable, slabs);
         TATARA_LAUNCHED("embedding_join");
     }

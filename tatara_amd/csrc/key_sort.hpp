@@ -17,18 +17,20 @@ namespace {
 constexpr uint32_t kMaxKeys = 1024;
 constexpr uint32_t kSortWaves = 16;
 constexpr uint32_t kSortThreads = kSortWaves * kWave;
+constexpr int kHand = 8;  // items that a lane reads at once
 constexpr uint32_t kMaxRuns = 256;
 // Items that one workgroup sorts alone, and that a workgroup has at least.
 constexpr uint32_t kAlone = 8192;
 constexpr uint32_t kLeastRun = 1024;
+// Counts of all runs at most: every workgroup adds them up.
+constexpr uint32_t kMostCounts = 32768;
 
 struct SortShape {
     uint32_t runs;  // workgroups
     uint32_t run;   // items of each, a multiple of kSortThreads
 };
 
-// With more runs of many keys a workgroup would add up more counts than it has items.
-inline uint32_t most_runs(uint32_t keys) { return std::min(kMaxRuns, std::max(16u, 32768u / keys)); }
+inline uint32_t most_runs(uint32_t keys) { return std::min(kMaxRuns, std::max(16u, kMostCounts / keys)); }
 
 inline SortShape sort_shape(uint64_t items, uint32_t keys) {
     if (items <= kAlone) return {1, (uint32_t)(items + kSortThreads - 1) / kSortThreads * kSortThreads};
@@ -37,13 +39,18 @@ inline SortShape sort_shape(uint64_t items, uint32_t keys) {
     return {(uint32_t)((items + run - 1) / run), (uint32_t)run};
 }
 
-// Bytes of the counts of all runs.
-inline uint64_t sort_bytes(uint32_t keys) { return 4ull * most_runs(keys) * keys; }
+// A run's counts are read four at a time.
+__host__ __device__ constexpr uint32_t in_fours(uint32_t keys) { return (keys + 3) / 4 * 4; }
 
-// The lanes with the same key (below 2^bits) as this one, of those that are `in`.
-__device__ __forceinline__ uint64_t same_key(bool in, uint32_t key, int bits) {
+// Bytes of the counts of all runs.
+inline uint64_t sort_bytes(uint32_t keys) { return 4ull * most_runs(keys) * in_fours(keys); }
+
+// The lanes with the same key (below 2^BITS) as this one, of those that are `in`.
+template <int BITS>
+__device__ __forceinline__ uint64_t same_key(bool in, uint32_t key) {
     uint64_t same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
         const uint64_t set = __ballot(key >> b & 1);
         same &= key >> b & 1 ? set : ~set;
     }
@@ -67,63 +74,105 @@ __device__ __forceinline__ uint32_t sum_ahead(uint32_t x, uint32_t* part) {
     return ahead + s - x;
 }
 
-// counts[run][key].  Keys: key(i) of item i, below `keys`, or kMaxKeys for an item that is
-// left out.
-template <typename Keys>
-__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Keys items, uint64_t n, uint32_t run, uint32_t keys,
+// What is sorted, Items, has
+//   Item load(i)      item i,
+//   key(item)         its key, below `keys`, or above for one that is left out,
+//   put(i, item, key, first, rank)   for each that is not, with the first place of its key
+//                     and its number in it,
+//   drop(i)           for the others,
+//   finish(firsts, keys)   at the end, with the first place of every key and, at [keys],
+//                     the number of all.
+
+// counts[run][in_fours(keys)].
+template <typename Items>
+__global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Items items, uint64_t n, uint32_t run, uint32_t keys,
                                                                   uint32_t* __restrict__ counts) {
     __shared__ uint32_t count[kMaxKeys];
-    for (uint32_t e = threadIdx.x; e < keys; e += kSortThreads) count[e] = 0;
+    const uint32_t width = in_fours(keys);
+    for (uint32_t e = threadIdx.x; e < width; e += kSortThreads) count[e] = 0;
     __syncthreads();
     const uint64_t first = (uint64_t)blockIdx.x * run;
-    for (uint32_t at = threadIdx.x; at < run; at += kSortThreads) {
-        const uint32_t key = first + at < n ? items.key(first + at) : kMaxKeys;
-        if (key < keys) atomicAdd(&count[key], 1u);
+    for (uint32_t at0 = 0; at0 < run; at0 += kSortThreads * kHand) {
+        uint32_t key[kHand];
+#pragma unroll
+        for (int h = 0; h < kHand; ++h) {
+            const uint32_t at = at0 + h * kSortThreads + threadIdx.x;
+            key[h] = at < run && first + at < n ? items.key(items.load(first + at)) : kMaxKeys;
+        }
+#pragma unroll
+        for (int h = 0; h < kHand; ++h)
+            if (key[h] < keys) atomicAdd(&count[key[h]], 1u);
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < keys; e += kSortThreads) counts[(uint64_t)blockIdx.x * keys + e] = count[e];
+    for (uint32_t e = threadIdx.x; e < width; e += kSortThreads) counts[(uint64_t)blockIdx.x * width + e] = count[e];
 }
 
-// Calls items.put(i, key, first place of its key, its number among them) for every item
-// that is not left out and items.drop(i) for the others, then items.finish(firsts, keys)
-// with the first place of every key and, at [keys], their number.
-template <typename Keys>
-__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Keys items, uint64_t n, uint32_t run, uint32_t keys,
-                                                                  int bits, const uint32_t* __restrict__ counts) {
+template <typename Items, int BITS>
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, uint64_t n, uint32_t run, uint32_t keys,
+                                                                  const uint32_t* __restrict__ counts) {
     extern __shared__ uint32_t shared[];
-    uint32_t* next = shared;                                // [wave][key]: the next item's place in its key
-    uint32_t* total = next + kSortWaves * keys;             // [key]
-    uint32_t* ahead = total + keys;                         // [key]: in the runs ahead of this one
-    uint32_t* first = ahead + keys;                         // [key + 1]
-    uint32_t* part = first + keys + 1;                      // [wave]
+    const uint32_t width = in_fours(keys);
+    uint32_t* next = shared;                     // [wave][key]: the next item's place in its key
+    uint32_t* total = next + kSortWaves * keys;  // [width]
+    uint32_t* ahead = total + width;             // [width]: in the runs ahead of this one
+    uint32_t* first = ahead + width;             // [keys + 1]
+    uint32_t* part = first + keys + 1;           // [wave]
     const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    for (uint32_t i = threadIdx.x; i < (kSortWaves + 2) * keys; i += kSortThreads) shared[i] = 0;
-    __syncthreads();
     const uint32_t mine = run / kSortWaves;  // items of a wave, a multiple of kWave
     const uint64_t from = (uint64_t)blockIdx.x * run + (uint64_t)wave * mine;
-    uint32_t* my_next = next + wave * keys;
-    for (uint32_t at = lane; at < mine; at += kWave) {
-        const uint32_t key = from + at < n ? items.key(from + at) : kMaxKeys;
-        if (key < keys) atomicAdd(&my_next[key], 1u);
+    typename Items::Item item[kHand];
+    uint32_t key[kHand];
+    auto read = [&](uint32_t at0) {
+#pragma unroll
+        for (int h = 0; h < kHand; ++h) {
+            const uint32_t at = at0 + h * kWave + lane;
+            const bool here = at < mine && from + at < n;
+            if (here) item[h] = items.load(from + at);
+            key[h] = here ? items.key(item[h]) : kMaxKeys;
+        }
+    };
+    // what is read of memory is on its way before the first barrier
+    read(0);
+    uint32_t all[4] = {}, before[4] = {};
+    const uint32_t share = threadIdx.x / (width / 4), four = (threadIdx.x - share * (width / 4)) * 4;
+    const uint32_t shares = kSortThreads / (width / 4);
+    if (gridDim.x > 1 && share < shares) {
+#pragma unroll 8
+        for (uint32_t b = share; b < gridDim.x; b += shares) {
+            const uint4 c = *reinterpret_cast<const uint4*>(counts + b * width + four);
+            const bool earlier = b < blockIdx.x;
+            all[0] += c.x, all[1] += c.y, all[2] += c.z, all[3] += c.w;
+            before[0] += earlier ? c.x : 0, before[1] += earlier ? c.y : 0;
+            before[2] += earlier ? c.z : 0, before[3] += earlier ? c.w : 0;
+        }
     }
-    if (gridDim.x > 1) {
-        for (uint32_t i = threadIdx.x; i < gridDim.x * keys; i += kSortThreads) {
-            const uint32_t b = i / keys, e = i - b * keys, c = counts[i];
-            if (c) {
-                atomicAdd(&total[e], c);
-                if (b < blockIdx.x) atomicAdd(&ahead[e], c);
-            }
+    for (uint32_t i = threadIdx.x; i < kSortWaves * keys + 2 * width; i += kSortThreads) shared[i] = 0;
+    __syncthreads();
+    uint32_t* my_next = next + wave * keys;
+    for (uint32_t at0 = 0; at0 < mine; at0 += kWave * kHand) {
+        if (at0) read(at0);
+#pragma unroll
+        for (int h = 0; h < kHand; ++h)
+            if (key[h] < keys) atomicAdd(&my_next[key[h]], 1u);
+    }
+    if (gridDim.x > 1 && share < shares) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (all[j]) atomicAdd(&total[four + j], all[j]);
+            if (before[j]) atomicAdd(&ahead[four + j], before[j]);
         }
     }
     __syncthreads();
     // kMaxKeys threads are enough for all keys
     const uint32_t e = threadIdx.x;
     if (e < keys) {
-        uint32_t s = ahead[e];
+        uint32_t s = ahead[e], c[kSortWaves];
+#pragma unroll
+        for (uint32_t w = 0; w < kSortWaves; ++w) c[w] = next[w * keys + e];
+#pragma unroll
         for (uint32_t w = 0; w < kSortWaves; ++w) {
-            const uint32_t c = next[w * keys + e];
             next[w * keys + e] = s;
-            s += c;
+            s += c[w];
         }
         if (gridDim.x == 1) total[e] = s;
     }
@@ -132,36 +181,47 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Keys items, ui
     if (e < keys) first[e] = start;
     if (e + 1 == keys) first[keys] = start + count;
     __syncthreads();
-    for (uint32_t at0 = 0; at0 < mine; at0 += kWave) {
-        const uint64_t i = from + at0 + lane;
-        const uint32_t key = i < n ? items.key(i) : kMaxKeys;
-        const bool in = key < keys;
-        const uint64_t same = same_key(in, key, bits);
-        const uint64_t below = same & ((1ull << lane) - 1);
-        uint32_t rank = 0;
-        if (in) rank = __hip_atomic_load(&my_next[key], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        if (in && below == 0) atomicAdd(&my_next[key], (uint32_t)__popcll(same));  // behind the wave's loads
-        rank += (uint32_t)__popcll(below);
-        if (in)
-            items.put(i, key, first[key], rank);
-        else if (i < n)
-            items.drop(i);
+    for (uint32_t at0 = 0; at0 < mine; at0 += kWave * kHand) {
+        if (at0 || mine > kWave * kHand) read(at0);
+#pragma unroll
+        for (int h = 0; h < kHand; ++h) {
+            if (at0 + h * kWave >= mine) break;
+            const uint64_t i = from + at0 + h * kWave + lane;
+            const bool in = key[h] < keys;
+            const uint64_t same = same_key<BITS>(in, key[h]);
+            const uint64_t below = same & ((1ull << lane) - 1);
+            uint32_t rank = 0;
+            if (in) rank = __hip_atomic_load(&my_next[key[h]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (in && below == 0) atomicAdd(&my_next[key[h]], (uint32_t)__popcll(same));  // behind the wave's loads
+            rank += (uint32_t)__popcll(below);
+            if (in)
+                items.put(i, item[h], key[h], first[key[h]], rank);
+            else if (i < n)
+                items.drop(i);
+        }
     }
     items.finish(first, keys);
 }
 
-inline uint32_t sort_lds(uint32_t keys) { return 4 * ((kSortWaves + 3) * keys + 1 + kSortWaves); }
+inline uint32_t sort_lds(uint32_t keys) { return 4 * (kSortWaves * keys + 2 * in_fours(keys) + keys + 1 + kSortWaves); }
 
-template <typename Keys>
-int32_t launch_sort(const Keys& items, uint64_t n, uint32_t keys, uint32_t* counts, hipStream_t stream) {
+template <typename Items>
+int32_t launch_sort(const Items& items, uint64_t n, uint32_t keys, uint32_t* counts, hipStream_t stream) {
     const SortShape shape = sort_shape(std::max<uint64_t>(n, 1), keys);
     if (shape.runs > 1) {
         sort_count_kernel<<<shape.runs, kSortThreads, 0, stream>>>(items, n, shape.run, keys, counts);
         TATARA_LAUNCHED("sort_count");
     }
-    int bits = 0;
-    while ((1u << bits) < keys) ++bits;
-    sort_place_kernel<<<shape.runs, kSortThreads, sort_lds(keys), stream>>>(items, n, shape.run, keys, bits, counts);
+    auto place = [&](auto bits) {
+        sort_place_kernel<Items, decltype(bits)::value>
+            <<<shape.runs, kSortThreads, sort_lds(keys), stream>>>(items, n, shape.run, keys, counts);
+    };
+    if (keys <= 16)
+        place(std::integral_constant<int, 4>{});
+    else if (keys <= 128)
+        place(std::integral_constant<int, 7>{});
+    else
+        place(std::integral_constant<int, 10>{});
     TATARA_LAUNCHED("sort_place");
     return kOk;
 }

@@ -14,6 +14,8 @@
 namespace tatara {
 namespace {
 
+constexpr uint32_t kBits8Blocks = 4096;
+
 // The largest of what the W waves of a row hold.
 template <int W>
 __device__ __forceinline__ uint32_t row_max(uint32_t x, uint32_t (*part)[W], int slot) {
@@ -83,16 +85,46 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
     auto fix = [&](auto& piece, int i) {
         if (!FEW) piece.fix((int)cols - column(i));
     };
-    // more rows than the grid has room for are taken in turn
-    constexpr int G = W == 1 ? 4 : 1;
+    constexpr int G = W == 1 ? 4 : 1;  // rows that the workgroup has in hand
+    // the weight stays in registers over the workgroup's rows: as f32 it has up to twice
+    // the bytes of a row
+    constexpr bool KEEP = BITS8 && (N * V <= 24 || sizeof(T) == 2);
+    Floats<V> kept[KEEP ? N : 1];
+    auto weights = [&](int i) {
+        Floats<V> w;
+        if (weight) {
+            read(w, weight, i);
+            fix(w, i);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) w.p[j / 4].v[j % 4] = 1.0f;
+        }
+        return w;
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) kept[i] = weights(i);
+    }
+    // An output in 8 bits has few workgroups, and reads a row while it works on the last.
+    Piece<T> px[N], pr[ADD ? N : 1];
+    auto read_row = [&](uint64_t row) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            read(px[i], x + (int64_t)row * x_stride, i);
+            if constexpr (ADD) read(pr[i], residual + (int64_t)row * residual_stride, i);
+        }
+    };
     const uint64_t step = (uint64_t)gridDim.x * G;
+    uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / (kWave * W);
+    if (BITS8 && row < rows) read_row(row);
     int slot = 0;
-    for (uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / (kWave * W); row < rows; row += step, slot ^= 1) {
+    for (; row < rows; row += step, slot ^= 1) {
+        if (!BITS8) read_row(row);
         Piece<T> in[N], more[ADD ? N : 1];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            read(in[i], x + (int64_t)row * x_stride, i);
-            if constexpr (ADD) read(more[i], residual + (int64_t)row * residual_stride, i);
+            in[i] = px[i];
+            if constexpr (ADD) more[i] = pr[i];
         }
         float s = 0.0f;
 #pragma unroll
@@ -106,6 +138,10 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
                 s = fmaf(v, v, s);
             }
         }
+        if constexpr (BITS8) {  // behind the last row nothing uses what is read
+            const uint64_t next = row + step;
+            read_row(next < rows ? next : row);
+        }
         const float r = 1.0f / sqrtf(row_sum<W>(s, part, slot) / (float)cols + eps);
         if (lane == 0 && rstd) rstd[row] = r;
         if constexpr (ADD) {
@@ -116,13 +152,9 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
             }
         }
         auto normed = [&](int i, float* y) {
-            Floats<V> w;
-            if (weight) {
-                read(w, weight, i);
-                fix(w, i);
-            }
+            const Floats<V> w = KEEP ? kept[KEEP ? i : 0] : weights(i);
 #pragma unroll
-            for (int j = 0; j < V; ++j) y[j] = (float)in[i].v[j] * r * (weight ? w[j] : 1.0f);
+            for (int j = 0; j < V; ++j) y[j] = (float)in[i].v[j] * r * w[j];
         };
         if constexpr (!BITS8) {
             T* to = static_cast<T*>(out.y) + (int64_t)row * out.stride;
@@ -350,11 +382,11 @@ void launch_forward(const void* x, int64_t x_stride, const void* residual, int64
                     const float* weight, void* total, int64_t total_stride, const RmsOut& out, float* rstd,
                     uint64_t rows, uint32_t cols, float eps, int32_t dtype, hipStream_t stream) {
     TATARA_FOR_DTYPE(dtype, {
-        with_form<T, false>(norm_form(false, rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
+        auto go = [&](auto w, auto n, auto few) {
             constexpr int W = decltype(w)::value;
             constexpr int N = decltype(n)::value;
             constexpr bool FEW = decltype(few)::value;
-            const uint32_t blocks = (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, kMaxGrid);
+            const uint32_t blocks = (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, BITS8 ? kBits8Blocks : kMaxGrid);
             const uint32_t threads = W == 16 ? 1024 : 256;
             if (residual)
                 rms_forward_kernel<T, W, N, FEW, true, BITS8><<<blocks, threads, 0, stream>>>(
@@ -363,7 +395,8 @@ void launch_forward(const void* x, int64_t x_stride, const void* residual, int64
             else
                 rms_forward_kernel<T, W, N, FEW, false, BITS8><<<blocks, threads, 0, stream>>>(
                     static_cast<const T*>(x), x_stride, nullptr, 0, weight, nullptr, 0, out, rstd, rows, cols, eps);
-        });
+        };
+        with_form<T, false>(norm_form(false, rows, cols, Piece<T>::V), go);
     });
 }
 

@@ -37,16 +37,16 @@ __device__ __forceinline__ void fix(Piece<T>& p, int c, int cols) {
     if (!FEW) p.fix(cols - c);
 }
 
-// K: at least top_k; U: pieces of each row in hand.  FEW: rows of fewer elements than
-// a piece has.
+// K: at least top_k; U: pieces of each row in hand.  FEW: rows of fewer elements than a
+// piece has.
 template <typename T, int K, int U, bool FEW>
-__global__ __launch_bounds__(kThreads) void rows_back_kernel(RowsBack a, uint32_t lanes) {
+__global__ __launch_bounds__(kThreads) void rows_back_kernel(RowsBack a, uint32_t lanes, bool past) {
     constexpr int V = Piece<T>::V;
-    const uint32_t lane = threadIdx.x & (lanes - 1), per_block = kThreads / lanes;
+    const uint32_t lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
     const int cols = (int)a.cols;
     const T* rows = static_cast<const T*>(a.rows);
-    const uint64_t step = (uint64_t)gridDim.x * per_block;
-    for (uint64_t t = (uint64_t)blockIdx.x * per_block + threadIdx.x / lanes; t < a.positions; t += step) {
+    const uint64_t step = (uint64_t)gridDim.x * groups;
+    for (uint64_t t = (uint64_t)blockIdx.x * groups + threadIdx.x / lanes; t < a.positions; t += step) {
         const T* from[K];
         float w[K];
         bool in[K];
@@ -83,44 +83,44 @@ __global__ __launch_bounds__(kThreads) void rows_back_kernel(RowsBack a, uint32_
                 Piece<T> out;
 #pragma unroll
                 for (int e = 0; e < V; ++e) out.v[e] = (T)y[e];
-                out.store(to + c, cols - c);
+                if (past)
+                    out.store_past(to + c, cols - c);
+                else
+                    out.store(to + c, cols - c);
             }
         }
     }
 }
 
-// DOT: the gates' gradient too.  Behind the workgroups of positions, those from `blocks`
-// on clear the rows without a source, kThreads of them each.
+// DOT: the gates' gradient too.  The first `clear` workgroups clear the rows without a
+// source, kWave of them a wave.
 template <typename T, int K, int U, bool FEW, bool DOT>
-__global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t lanes, uint32_t blocks) {
+__global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t lanes, uint32_t clear) {
     constexpr int V = Piece<T>::V;
     const int cols = (int)a.cols;
     T* rows = static_cast<T*>(a.rows);
-    if (blockIdx.x >= blocks) {
-        __shared__ bool none[kThreads];
+    if (blockIdx.x < clear) {
         const uint64_t items = a.positions * a.top_k;
-        for (uint64_t first = (uint64_t)(blockIdx.x - blocks) * kThreads; first < a.n_rows;
-             first += (uint64_t)(gridDim.x - blocks) * kThreads) {
-            __syncthreads();
-            const uint64_t mine = first + threadIdx.x;
-            none[threadIdx.x] = mine < a.n_rows && (uint32_t)a.source[mine] >= items;
-            __syncthreads();
-            for (int r = 0; r < kThreads; ++r) {
-                if (!none[r]) continue;
-                Piece<T> zero;
+        const uint32_t lane = threadIdx.x % kWave;
+        Piece<T> zero;
 #pragma unroll
-                for (int e = 0; e < V; ++e) zero.v[e] = (T)0.0f;
-                T* to = rows + (int64_t)(first + r) * a.rows_stride;
-                for (int c = (int)threadIdx.x * V; c < cols; c += kThreads * V) zero.store(to + c, cols - c);
+        for (int e = 0; e < V; ++e) zero.v[e] = (T)0.0f;
+        for (uint64_t first = (uint64_t)blockIdx.x * kThreads + threadIdx.x / kWave * kWave; first < a.n_rows;
+             first += (uint64_t)clear * kThreads) {
+            const uint64_t mine = first + lane;
+            uint64_t none = __ballot(mine < a.n_rows && (uint32_t)a.source[mine < a.n_rows ? mine : 0] >= items);
+            for (; none; none &= none - 1) {
+                T* to = rows + (int64_t)(first + __builtin_ctzll(none)) * a.rows_stride;
+                for (int c = (int)lane * V; c < cols; c += kWave * V) zero.store(to + c, cols - c);
             }
         }
         return;
     }
-    const uint32_t lane = threadIdx.x & (lanes - 1), per_block = kThreads / lanes;
-    const uint64_t step = (uint64_t)blocks * per_block;
+    const uint32_t lane = threadIdx.x & (lanes - 1), groups = kThreads / lanes;
+    const uint64_t step = (uint64_t)(gridDim.x - clear) * groups;
     const uint64_t rounds = (a.positions + step - 1) / step;
     for (uint64_t i = 0; i < rounds; ++i) {  // the same for every lane: the sums need them all
-        const uint64_t mine = i * step + (uint64_t)blockIdx.x * per_block + threadIdx.x / lanes;
+        const uint64_t mine = i * step + (uint64_t)(blockIdx.x - clear) * groups + threadIdx.x / lanes;
         const bool here = mine < a.positions;
         const uint64_t t = here ? mine : 0;
         int64_t at[K];
@@ -138,14 +138,14 @@ __global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t 
         const T* x = static_cast<const T*>(a.x) + (int64_t)t * a.x_stride;
         const T* from = static_cast<const T*>(a.from);
         for (int c0 = (int)lane * V; c0 < cols; c0 += (int)lanes * V * U) {
-            Piece<T> p[U], q[DOT ? K : 1][U];
+            Piece<T> p[U], r[DOT ? K : 1][U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int c = c0 + u * (int)lanes * V;
                 read<T, FEW>(p[u], x, c, cols);
                 if constexpr (DOT) {
 #pragma unroll
-                    for (int j = 0; j < K; ++j) read<T, FEW>(q[j][u], from + at[j] * a.from_stride, c, cols);
+                    for (int j = 0; j < K; ++j) read<T, FEW>(r[j][u], from + at[j] * a.from_stride, c, cols);
                 }
             }
 #pragma unroll
@@ -155,9 +155,9 @@ __global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t 
 #pragma unroll
                 for (int j = 0; j < K; ++j) {
                     if constexpr (DOT) {
-                        fix<T, FEW>(q[j][u], c, cols);
+                        fix<T, FEW>(r[j][u], c, cols);
 #pragma unroll
-                        for (int e = 0; e < V; ++e) dot[j] = fmaf((float)p[u].v[e], (float)q[j][u].v[e], dot[j]);
+                        for (int e = 0; e < V; ++e) dot[j] = fmaf((float)p[u].v[e], (float)r[j][u].v[e], dot[j]);
                     }
                     if (!in[j]) continue;
                     Piece<T> out = p[u];
@@ -199,16 +199,48 @@ void with_top(uint32_t top_k, F&& f) {
         f(integral_constant<int, 16>{});
 }
 
-// Lanes that hold a row, a power of two up to a wave.
-uint32_t row_lanes(uint32_t cols, int v) {
+// How a row of `cols` lies over lanes: a power of two of them that holds it, up to a wave,
+// of which half or a quarter if that leaves fewer idle (768 columns of 16 bits: 3 pieces
+// of 32 lanes, not 2 of 64 with half of one empty), and pieces a lane has in hand.
+struct RowForm {
+    uint32_t lanes;
+    int pieces;
+};
+RowForm row_form(uint32_t cols, int v, int most_pieces) {
+    const uint32_t n = ceil_div(cols, v);
     uint32_t lanes = 1;
-    while (lanes < kWave && lanes * v < cols) lanes *= 2;
-    return lanes;
+    while (lanes < kWave && lanes < n) lanes *= 2;
+    if (lanes == kWave) {
+        uint32_t best = ceil_div(n, kWave) * kWave;
+        for (uint32_t l = kWave / 2; l >= 16; l /= 2)
+            if (ceil_div(n, l) * l < best && ceil_div(n, l) <= 4) lanes = l, best = ceil_div(n, l) * l;
+    }
+    const uint32_t rounds = ceil_div(n, lanes);
+    return {lanes, (int)ceil_div(rounds, ceil_div(rounds, most_pieces))};
 }
 
+// Calls f with the pieces in hand.
+template <int MOST, typename F>
+void with_pieces(int pieces, F&& f) {
+    auto is = [&](auto u) {
+        if constexpr (decltype(u)::value <= MOST)
+            if (pieces == decltype(u)::value) f(u);
+    };
+    is(std::integral_constant<int, 1>{});
+    is(std::integral_constant<int, 2>{});
+    is(std::integral_constant<int, 3>{});
+    is(std::integral_constant<int, 4>{});
+}
+
+// Whether rows are written past the caches: from half the last-level cache (256 MB) on they
+// would push out what a reader finds there.  Rows of a table looked up and then normalised
+// (bf16): 65536 x 1536, 201 MB, 48 us and with the norm 136, past the caches 40 and 124;
+// 65536 x 768 22.5 and 61.7, past them 18.6 and 68.
+bool past_caches(uint64_t bytes) { return bytes >= 128ull << 20; }
+
 uint32_t position_blocks(uint64_t positions, uint32_t lanes) {
-    const uint64_t per_block = kThreads / lanes;
-    return (uint32_t)std::min<uint64_t>((positions + per_block - 1) / per_block, kMaxGrid);
+    const uint64_t groups = kThreads / lanes;
+    return (uint32_t)std::min<uint64_t>((positions + groups - 1) / groups, kMaxGrid);
 }
 
 }  // namespace
@@ -217,13 +249,19 @@ int32_t launch_rows_back(const RowsBack& a, int32_t dtype, hipStream_t stream) {
     if (a.positions == 0) return kOk;
     TATARA_FOR_DTYPE(dtype, {
         constexpr int V = Piece<T>::V;
-        const uint32_t lanes = row_lanes(a.cols, V), blocks = position_blocks(a.positions, lanes);
+        const bool past = past_caches(a.positions * a.cols * sizeof(T));
         with_top(a.top_k, [&](auto k) {
-            constexpr int K = decltype(k)::value, U = K == 1 ? 4 : K == 2 ? 2 : 1;
-            if (a.cols < (uint32_t)V)
-                rows_back_kernel<T, K, 1, true><<<blocks, kThreads, 0, stream>>>(a, lanes);
-            else
-                rows_back_kernel<T, K, U, false><<<blocks, kThreads, 0, stream>>>(a, lanes);
+            constexpr int K = decltype(k)::value, MOST = K <= 2 ? 4 : 1;
+            if (a.cols < (uint32_t)V) {
+                rows_back_kernel<T, K, 1, true>
+                    <<<position_blocks(a.positions, 1), kThreads, 0, stream>>>(a, 1, past);
+                return;
+            }
+            const RowForm form = row_form(a.cols, V, MOST);
+            with_pieces<MOST>(form.pieces, [&](auto u) {
+                rows_back_kernel<T, K, decltype(u)::value, false>
+                    <<<position_blocks(a.positions, form.lanes), kThreads, 0, stream>>>(a, form.lanes, past);
+            });
         });
     });
     TATARA_LAUNCHED("rows_back");
@@ -234,17 +272,24 @@ int32_t launch_rows_out(const RowsOut& a, int32_t dtype, hipStream_t stream) {
     if (a.positions == 0 && a.n_rows == 0) return kOk;
     TATARA_FOR_DTYPE(dtype, {
         constexpr int V = Piece<T>::V;
-        const uint32_t lanes = row_lanes(a.cols, V), blocks = position_blocks(a.positions, lanes);
-        const uint32_t clear = (uint32_t)std::min<uint64_t>((a.n_rows + kThreads - 1) / kThreads, kMaxGrid);
+        const uint32_t clear = position_blocks(a.n_rows, 1);
         with_top(a.top_k, [&](auto k) {
-            constexpr int K = decltype(k)::value, U = K == 1 ? 4 : K == 2 ? 2 : 1;
-            auto launch = [&](auto few, auto dot) {
-                constexpr bool FEW = decltype(few)::value, DOT = decltype(dot)::value;
-                rows_out_kernel<T, K, FEW ? 1 : DOT ? U : 4, FEW, DOT>
-                    <<<blocks + clear, kThreads, 0, stream>>>(a, lanes, blocks);
+            auto launch = [&](auto dot) {
+                constexpr bool DOT = decltype(dot)::value;
+                constexpr int K = decltype(k)::value, MOST = !DOT || K <= 2 ? 4 : 1;
+                if (a.cols < (uint32_t)V) {
+                    rows_out_kernel<T, K, 1, true, DOT>
+                        <<<clear + position_blocks(a.positions, 1), kThreads, 0, stream>>>(a, 1, clear);
+                    return;
+                }
+                const RowForm form = row_form(a.cols, V, MOST);
+                with_pieces<MOST>(form.pieces, [&](auto u) {
+                    rows_out_kernel<T, K, decltype(u)::value, false, DOT>
+                        <<<clear + position_blocks(a.positions, form.lanes), kThreads, 0, stream>>>(a, form.lanes,
+                                                                                                    clear);
+                });
             };
-            auto with_dot = [&](auto few) { a.dgate ? launch(few, std::true_type{}) : launch(few, std::false_type{}); };
-            a.cols < (uint32_t)V ? with_dot(std::true_type{}) : with_dot(std::false_type{});
+            a.dgate ? launch(std::true_type{}) : launch(std::false_type{});
         });
     });
     TATARA_LAUNCHED("rows_out");

@@ -62,6 +62,13 @@ struct Piece {
             store_few(p, left);
         }
     }
+    // Has the compiler compute again what follows from the values, where it would keep it in
+    // registers that a wide row does not have.
+    __device__ __forceinline__ void forget() {
+        Words w = words();
+        asm volatile("" : "+v"(w));
+        __builtin_memcpy(v, &w, 16);
+    }
 
    private:
     typedef uint32_t Words __attribute__((ext_vector_type(4)));

@@ -23,7 +23,7 @@ constexpr uint32_t kMaxRuns = 256;
 constexpr uint32_t kAlone = 8192;
 constexpr uint32_t kLeastRun = 1024;
 // Counts of all runs at most: every workgroup adds them up.
-constexpr uint32_t kMostCounts = 32768;
+constexpr uint32_t kMostCounts = 16384;
 
 struct SortShape {
     uint32_t runs;  // workgroups

@@ -16,16 +16,19 @@ namespace {
 
 constexpr uint32_t kBits8Blocks = 4096;
 
+// The larger; NaN if either is.
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // The largest of what the W waves of a row hold.
 template <int W>
-__device__ __forceinline__ uint32_t row_max(uint32_t x, uint32_t (*part)[W], int slot) {
-    x = group_join_u<(int)kWave>(x, [](uint32_t a, uint32_t b) { return max(a, b); });
+__device__ __forceinline__ float row_max(float x, float (*part)[W], int slot) {
+    x = group_join<(int)kWave>(x, larger);
     if constexpr (W > 1) {
         if (threadIdx.x % kWave == 0) part[slot][threadIdx.x / kWave] = x;
         __syncthreads();
-        x = 0;
+        x = part[slot][0];
 #pragma unroll
-        for (int i = 0; i < W; ++i) x = max(x, part[slot][i]);
+        for (int i = 1; i < W; ++i) x = larger(x, part[slot][i]);
     }
     return x;
 }
@@ -34,12 +37,15 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, uint32_t (*part)[W], int
 template <int V>
 __device__ __forceinline__ void store_8bit(uint8_t* to, const float* v, bool e4m3, int left) {
     uint32_t word[V / 4];
+    if (e4m3) {
 #pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-        if (e4m3) {
+        for (int i = 0; i < V / 4; ++i) {
             const int low = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
             word[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], low, true);
-        } else {
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
             word[i] = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) word[i] |= ((uint32_t)(int32_t)rintf(v[4 * i + j]) & 0xffu) << (8 * j);
@@ -73,8 +79,9 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
     T* total, int64_t total_stride, RmsOut out, float* __restrict__ rstd, uint64_t rows, uint32_t cols, float eps) {
     constexpr int V = Piece<T>::V;
     __shared__ float part[2][W];
-    __shared__ uint32_t part_max[2][W];
+    __shared__ float part_max[2][W];
     const uint32_t lane = threadIdx.x % (kWave * W);
+    const uint32_t group = __builtin_amdgcn_readfirstlane(threadIdx.x / (kWave * W));
     auto column = [&](int i) { return (int)(i * kWave * W + lane) * V; };
     auto read = [&](auto& piece, const auto* from, int i) {
         if (FEW)
@@ -88,12 +95,14 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
     constexpr int G = W == 1 ? 4 : 1;  // rows that the workgroup has in hand
     // the weight stays in registers over the workgroup's rows: as f32 it has up to twice
     // the bytes of a row
-    constexpr bool KEEP = BITS8 && (N * V <= 24 || sizeof(T) == 2);
+    constexpr bool KEEP = BITS8 && W < 16 && (N * V <= 24 || sizeof(T) == 2);
     Floats<V> kept[KEEP ? N : 1];
     auto weights = [&](int i) {
+        const float* from = weight;
+        if constexpr (W == 16) asm volatile("" : "+s"(from));  // else they are all kept
         Floats<V> w;
-        if (weight) {
-            read(w, weight, i);
+        if (from) {
+            read(w, from, i);
             fix(w, i);
         } else {
 #pragma unroll
@@ -106,6 +115,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
         for (int i = 0; i < N; ++i) kept[i] = weights(i);
     }
     // An output in 8 bits has few workgroups, and reads a row while it works on the last.
+    constexpr bool AHEAD = BITS8 && W < 16;
     Piece<T> px[N], pr[ADD ? N : 1];
     auto read_row = [&](uint64_t row) {
 #pragma unroll
@@ -115,11 +125,11 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
         }
     };
     const uint64_t step = (uint64_t)gridDim.x * G;
-    uint64_t row = (uint64_t)blockIdx.x * G + threadIdx.x / (kWave * W);
-    if (BITS8 && row < rows) read_row(row);
+    uint64_t row = (uint64_t)blockIdx.x * G + group;
+    if (AHEAD && row < rows) read_row(row);
     int slot = 0;
     for (; row < rows; row += step, slot ^= 1) {
-        if (!BITS8) read_row(row);
+        if (!AHEAD) read_row(row);
         Piece<T> in[N], more[ADD ? N : 1];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -138,11 +148,11 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
                 s = fmaf(v, v, s);
             }
         }
-        if constexpr (BITS8) {  // behind the last row nothing uses what is read
+        if constexpr (AHEAD) {  // behind the last row nothing uses what is read
             const uint64_t next = row + step;
             read_row(next < rows ? next : row);
         }
-        const float r = 1.0f / sqrtf(row_sum<W>(s, part, slot) / (float)cols + eps);
+        const float r = rsqrtf(row_sum<W>(s, part, slot) / (float)cols + eps);
         if (lane == 0 && rstd) rstd[row] = r;
         if constexpr (ADD) {
             if (total) {
@@ -170,20 +180,18 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
                 piece.store(to + column(i), left);
             }
         } else {
-            // magnitudes as whole numbers, which order as they do, with infinity and
-            // NaN above the rest
-            float y[N][V];
-            uint32_t top[N], all = 0;
+            // NaN and infinity reach the largest: past the row's end a value is NaN only if
+            // rstd is not finite, and then so is none of the row
+            constexpr bool TWICE = W == 16;  // y is made again for its second use
+            float y[TWICE ? 1 : N][V], top[N], all = 0.0f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                normed(i, y[i]);
-                top[i] = 0;
+                float* yi = y[TWICE ? 0 : i];
+                normed(i, yi);
+                top[i] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const bool in_row = column(i) + j < (int)cols;  // past it a NaN of rstd shows too
-                    top[i] = max(top[i], in_row ? __float_as_uint(y[i][j]) & 0x7fffffffu : 0u);
-                }
-                all = max(all, top[i]);
+                for (int j = 0; j < V; ++j) top[i] = larger(top[i], fabsf(yi[j]));
+                all = larger(all, top[i]);
             }
             if (out.lanes == 0) {
                 all = row_max<W>(all, part_max, slot);
@@ -194,7 +202,8 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
                     constexpr int S = decltype(s)::value;
                     if (out.lanes >> S > 1) {
 #pragma unroll
-                        for (int i = 0; i < N; ++i) top[i] = max(top[i], partner<S>(top[i]));
+                        for (int i = 0; i < N; ++i)
+                            top[i] = larger(top[i], __uint_as_float(partner<S>(__float_as_uint(top[i]))));
                     }
                 };
                 join(std::integral_constant<int, 0>{});
@@ -204,21 +213,29 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
                 join(std::integral_constant<int, 4>{});
             }
             uint8_t* to = static_cast<uint8_t*>(out.y) + (int64_t)row * out.stride;
-            const float most = out.e4m3 ? 448.0f : 127.0f;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int left = (int)cols - column(i);
                 if (left <= 0) break;
-                // a group with a value that is not finite has the scale NaN, and zeros
-                const bool finite = top[i] < 0x7f800000u;
-                const float scale = finite ? fmaxf(__uint_as_float(top[i]), 0x1p-100f) / most : __uint_as_float(0x7fc00000u);
-                // one division a group: a product is an ulp of f32 off y / scale, which
-                // shows where that lies on the border of two results; the largest, M and
-                // two ulps at most, rounds to M
-                const float inv = 1.0f / scale;
+                // Products with reciprocals: three roundings of f32 and one unit of the
+                // reciprocal off y / scale, which shows where that lies on the border of two
+                // results; the largest, off M by as much, rounds to M.
+                const bool finite = top[i] < INFINITY;
+                float scale = fmaxf(top[i], 0x1p-100f) * (out.e4m3 ? 1.0f / 448.0f : 1.0f / 127.0f);
+                const float inv = __builtin_amdgcn_rcpf(scale);
+                if constexpr (TWICE) {
+                    in[i].forget();
+                    normed(i, y[0]);
+                }
                 float v[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = finite ? y[i][j] * inv : 0.0f;
+                for (int j = 0; j < V; ++j) v[j] = y[TWICE ? 0 : i][j] * inv;
+                if (__ballot(!finite)) {
+                    // a group with a value that is not finite has the scale NaN, and zeros
+                    scale = finite ? scale : __uint_as_float(0x7fc00000u);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[j] = finite ? v[j] : 0.0f;
+                }
                 store_8bit<V>(to + column(i), v, out.e4m3, left);
                 const uint32_t in_group = out.lanes ? lane % out.lanes : lane + i;
                 if (in_group == 0)
@@ -238,7 +255,8 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_backward_kernel(
     constexpr int G = W == 1 ? 4 : 1;  // rows that the workgroup has in hand
     __shared__ float part[2][W];
     __shared__ float join[G == 1 ? 1 : (G - 1) * kWave * N * V];
-    const uint32_t lane = threadIdx.x % (kWave * W), group = threadIdx.x / (kWave * W);
+    const uint32_t lane = threadIdx.x % (kWave * W);
+    const uint32_t group = __builtin_amdgcn_readfirstlane(threadIdx.x / (kWave * W));
     auto column = [&](int i) { return (int)(i * kWave * W + lane) * V; };
     auto read = [&](auto& piece, const auto* from, int i) {
         if (FEW)
@@ -249,16 +267,21 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_backward_kernel(
     auto fix = [&](auto& piece, int i) {
         if (!FEW) piece.fix((int)cols - column(i));
     };
-    // the weight stays in registers where they last
-    constexpr bool KEEP = N * V <= 24;
+    // The weight stays in registers where they last.  Of the widest rows, values are made
+    // again for their second use and none is read ahead (f32 4096 x 32768 1037 us, so 707, with
+    // dtotal 8192 x 16384 724 and 402; but bf16 16384 x 8192 158 and 189).
+    constexpr bool LEAN = W == 16 && (N * V > 16 || (N * V > 8 && (ADD || sizeof(T) == 4)));
+    constexpr bool KEEP = !LEAN && N * V <= 24;
     float dw[N * V];
     Floats<V> kept[KEEP ? N : 1];
 #pragma unroll
     for (int i = 0; i < N * V; ++i) dw[i] = 0.0f;
     auto weights = [&](int i) {
+        const float* from = weight;
+        if constexpr (LEAN) asm volatile("" : "+s"(from));  // else they are all kept
         Floats<V> w;
-        if (weight) {
-            read(w, weight, i);
+        if (from) {
+            read(w, from, i);
             fix(w, i);
         } else {
 #pragma unroll
@@ -284,11 +307,22 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_backward_kernel(
     int slot = 0;
     const uint64_t step = (uint64_t)gridDim.x * G;
     uint64_t row = (uint64_t)blockIdx.x * G + group;
-    if (row < rows) read_row(row);
+    if (!LEAN && row < rows) read_row(row);
     for (; row < rows; row += step, slot ^= 1) {
-        float h[N * V], g[N * V];
+        if (LEAN) read_row(row);
+        float h[LEAN ? V : N * V], g[LEAN ? V : N * V];
         Piece<T> add[ADD ? N : 1];
         float sgh = 0.0f;
+        auto terms = [&](int i, float* hi, float* gi) {
+            const Floats<V> w = KEEP ? kept[KEEP ? i : 0] : weights(i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                // past the row's end both are zero (NaN if rstd is not finite, and then so is
+                // what is in the row)
+                hi[j] = (float)ps[i].v[j] * r;
+                gi[j] = (float)pd[i].v[j] * w[j];
+            }
+        };
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             fix(ps[i], i);
@@ -297,31 +331,33 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_backward_kernel(
                 fix(pt[i], i);
                 add[i] = pt[i];
             }
-            const Floats<V> w = KEEP ? kept[KEEP ? i : 0] : weights(i);
+            float *hi = h + (LEAN ? 0 : i * V), *gi = g + (LEAN ? 0 : i * V);
+            terms(i, hi, gi);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const int e = i * V + j;
-                // past the row's end dy and s are zero; a rstd that is not finite shows there
-                const float d = (float)pd[i].v[j];
-                h[e] = column(i) + j < (int)cols ? (float)ps[i].v[j] * r : 0.0f;
-                g[e] = d * w[j];
-                sgh = fmaf(g[e], h[e], sgh);
-                dw[e] = fmaf(d, h[e], dw[e]);
+                sgh = fmaf(gi[j], hi[j], sgh);
+                dw[i * V + j] = fmaf((float)pd[i].v[j], hi[j], dw[i * V + j]);
             }
         }
         const float scale = r;
         // the next row's values are on their way while this one's sum is joined (behind the
         // last row nothing uses what is read)
         const uint64_t next = row + step;
-        read_row(next < rows ? next : row);
+        if (!LEAN) read_row(next < rows ? next : row);
         const float b = row_sum<W>(sgh, part, slot) / (float)cols;
         T* to = dx + (int64_t)row * dx_stride;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
+            float *hi = h + (LEAN ? 0 : i * V), *gi = g + (LEAN ? 0 : i * V);
+            if constexpr (LEAN) {
+                ps[i].forget();
+                pd[i].forget();
+                terms(i, hi, gi);
+            }
             Piece<T> out;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float d = (g[i * V + j] - h[i * V + j] * b) * scale;
+                const float d = (gi[j] - hi[j] * b) * scale;
                 if constexpr (ADD)
                     out.v[j] = (T)(d + (float)add[i].v[j]);
                 else
@@ -382,11 +418,12 @@ void launch_forward(const void* x, int64_t x_stride, const void* residual, int64
                     const float* weight, void* total, int64_t total_stride, const RmsOut& out, float* rstd,
                     uint64_t rows, uint32_t cols, float eps, int32_t dtype, hipStream_t stream) {
     TATARA_FOR_DTYPE(dtype, {
-        auto go = [&](auto w, auto n, auto few) {
+        with_form<T, false>(norm_form(false, rows, cols, Piece<T>::V), [&](auto w, auto n, auto few) {
             constexpr int W = decltype(w)::value;
             constexpr int N = decltype(n)::value;
             constexpr bool FEW = decltype(few)::value;
-            const uint32_t blocks = (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, BITS8 ? kBits8Blocks : kMaxGrid);
+            const uint32_t blocks =
+                (uint32_t)std::min<uint64_t>(W == 1 ? (rows + 3) / 4 : rows, BITS8 ? kBits8Blocks : kMaxGrid);
             const uint32_t threads = W == 16 ? 1024 : 256;
             if (residual)
                 rms_forward_kernel<T, W, N, FEW, true, BITS8><<<blocks, threads, 0, stream>>>(
@@ -395,8 +432,7 @@ void launch_forward(const void* x, int64_t x_stride, const void* residual, int64
             else
                 rms_forward_kernel<T, W, N, FEW, false, BITS8><<<blocks, threads, 0, stream>>>(
                     static_cast<const T*>(x), x_stride, nullptr, 0, weight, nullptr, 0, out, rstd, rows, cols, eps);
-        };
-        with_form<T, false>(norm_form(false, rows, cols, Piece<T>::V), go);
+        });
     });
 }
 

@@ -18,41 +18,62 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr uint32_t kMaxVocab = 1u << 28;
-constexpr uint32_t kClearRows = 64;  // rows of the table that a workgroup looks up, and clears where no position has one
+// Rows of the table that a workgroup looks up at most, and clears where no position has one.
+constexpr uint32_t kClearRows = 128;
 constexpr int kBatch = 8;            // rows that a lane has in hand
 constexpr uint32_t kMostChunks = 1024;  // of rows as wide as a wave
 constexpr uint32_t kLeastChunk = 8;     // positions
+
+// A position and its token.
+struct alignas(8) Place {
+    uint32_t key, at;
+};
 
 // A pass of the radix sort.  The first one reads the tokens, of which those that stand
 // for none become `vocab`, behind the others.
 struct Digit {
     const int32_t* token;
-    const uint32_t* in_key;
-    const uint32_t* in_at;
+    const Place* in;
+    Place* out;
     uint32_t vocab, shift, mask;
-    uint32_t* out_key;
-    uint32_t* out_at;
 
-    struct Item {
-        uint32_t whole, at;
-    };
+    using Item = Place;
     __device__ __forceinline__ Item load(uint64_t i) const {
         if (token) return {min((uint32_t)token[i], vocab), (uint32_t)i};
-        return {in_key[i], in_at[i]};
+        return in[i];
     }
-    __device__ __forceinline__ uint32_t key(Item item) const { return item.whole >> shift & mask; }
+    __device__ __forceinline__ uint32_t key(Item item) const { return item.key >> shift & mask; }
     __device__ __forceinline__ void put(uint64_t, Item item, uint32_t, uint32_t first, uint32_t rank) const {
-        out_key[first + rank] = item.whole;
-        out_at[first + rank] = item.at;
+        out[first + rank] = item;
     }
     __device__ __forceinline__ void drop(uint64_t) const {}
     __device__ __forceinline__ void finish(const uint32_t*, uint32_t) const {}
 };
 
+// The passes go from one list to the other.
+__host__ __device__ __forceinline__ Digit digit_of(int pass, int bits, const int32_t* token, uint32_t vocab,
+                                                   uint32_t mask, Place* even, Place* odd) {
+    return {pass ? nullptr : token, pass % 2 ? even : odd, pass % 2 ? odd : even, vocab, (uint32_t)(pass * bits), mask};
+}
+
+// All passes, of positions that one workgroup sorts.
+template <int BITS>
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_kernel(const int32_t* token, uint32_t n, uint32_t run,
+                                                                      uint32_t vocab, int passes, int bits,
+                                                                      uint32_t keys, uint32_t mask, Place* even,
+                                                                      Place* odd) {
+    extern __shared__ uint32_t shared[];
+    for (int pass = 0; pass < passes; ++pass) {
+        asm volatile("" : "+s"(n), "+s"(keys));  // else what no pass changes is kept in registers that there are not
+        sort_place<BITS, true>(digit_of(pass, bits, token, vocab, mask, even, odd), n, run, keys, nullptr, shared);
+        __syncthreads();  // this pass's places are written before the next one reads them
+    }
+}
+
 struct Sorted {
-    const uint32_t* key;  // [n] tokens
-    const uint32_t* at;   // [n] their positions
+    const Place* place;  // [n], by token
     uint32_t n, chunk, chunks;
+    __device__ __forceinline__ uint32_t key(uint64_t i) const { return place[i].key; }
 };
 
 // A group of G lanes adds the rows of a chunk, V columns a lane; rows wider than a wave
@@ -63,33 +84,46 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
                                                                  uint32_t vocab, uint32_t cols, float scale,
                                                                  float* __restrict__ dtable,
                                                                  float* __restrict__ partial, uint32_t clear,
-                                                                 uint32_t slabs) {
+                                                                 uint32_t clear_rows, uint32_t slabs) {
     constexpr int V = Piece<T>::V;
     // the workgroups that clear lie evenly among the others, which read where they write
     const uint32_t cleared = (uint32_t)((uint64_t)blockIdx.x * clear / gridDim.x);
     const bool clears = cleared != (uint32_t)((uint64_t)(blockIdx.x + 1) * clear / gridDim.x);
     if (clears) {
         __shared__ bool none[kClearRows];
-        const uint32_t per_row = (cols + 3) / 4;
-        for (uint64_t first = (uint64_t)cleared * kClearRows; first < vocab; first += (uint64_t)clear * kClearRows) {
+        constexpr uint32_t LANES = 8, ROWS = kThreads / LANES, TURNS = kClearRows / ROWS;  // lanes look for TURNS rows at once
+        const uint32_t per_row = (cols + 3) / 4, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+        for (uint64_t first = (uint64_t)cleared * clear_rows; first < vocab; first += (uint64_t)clear * clear_rows) {
             __syncthreads();
-            if (threadIdx.x < kClearRows) {
-                const uint64_t v = first + threadIdx.x;
-                uint32_t lo = 0, hi = s.n;  // the first place with a key of v or above
-                while (lo < hi) {
-                    const uint32_t mid = lo + (hi - lo) / 2;
-                    if (s.key[mid] < v)
-                        lo = mid + 1;
-                    else
-                        hi = mid;
+            uint32_t lo[TURNS], hi[TURNS];  // the first place with a key of the row or above lies in lo..hi
+#pragma unroll
+            for (uint32_t q = 0; q < TURNS; ++q) lo[q] = 0, hi[q] = q * ROWS + group < clear_rows ? s.n : 0;
+            for (bool more = true; more;) {
+                uint32_t wide = 0;
+#pragma unroll
+                for (uint32_t q = 0; q < TURNS; ++q) {
+                    // a lane looks at the last place of each of LANES parts
+                    const uint32_t part = max((hi[q] - lo[q] + LANES - 1) / LANES, 1u);
+                    const uint32_t mine = lo[q] + (lane + 1) * part - 1;
+                    const uint64_t v = first + q * ROWS + group;
+                    const uint64_t below = __ballot(mine < hi[q] && s.key(mine < hi[q] ? mine : 0) < v);
+                    const uint32_t mask = (uint32_t)(below >> (threadIdx.x % kWave - lane)) & ((1u << LANES) - 1);
+                    lo[q] += __popc(mask) * part;
+                    hi[q] = min(hi[q], lo[q] + part - 1);
+                    wide |= hi[q] - lo[q];
                 }
-                none[threadIdx.x] = v < vocab && !(lo < s.n && s.key[lo] == v);
+                more = __ballot(wide) != 0;
+            }
+#pragma unroll
+            for (uint32_t q = 0; q < TURNS; ++q) {
+                const uint64_t v = first + q * ROWS + group;
+                if (lane == 0) none[q * ROWS + group] = v < vocab && !(lo[q] < s.n && s.key(lo[q]) == v);
             }
             __syncthreads();
             Piece<float> zero;
 #pragma unroll
             for (int e = 0; e < 4; ++e) zero.v[e] = 0.0f;
-            for (uint32_t i = threadIdx.x; i < kClearRows * per_row; i += kThreads) {
+            for (uint32_t i = threadIdx.x; i < clear_rows * per_row; i += kThreads) {
                 const uint32_t r = i / per_row, c = (i - r * per_row) * 4;
                 if (none[r]) zero.store(dtable + (first + r) * cols + c, (int)(cols - c));
             }
@@ -107,7 +141,7 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[e] = 0.0f;
     // whether the token's first row lies in the chunk
-    bool began = begin == 0 || s.key[begin - 1] != s.key[begin];
+    bool began = begin == 0 || s.key(begin - 1) != s.key(begin);
     bool open = false;
     auto flush = [&](float* to, float by) {
 #pragma unroll
@@ -122,9 +156,9 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
         uint32_t key[kBatch + 1], at[kBatch];
 #pragma unroll
         for (int j = 0; j <= kBatch; ++j) {
-            const uint32_t i = min(i0 + j, s.n - 1);
-            key[j] = s.key[i];
-            if (j < kBatch) at[j] = s.at[min(i, end - 1)];
+            const Place place = s.place[min(i0 + j, s.n - 1)];
+            key[j] = place.key;
+            if (j < kBatch) at[j] = place.at;
         }
         Piece<T> p[kBatch];
 #pragma unroll
@@ -171,12 +205,12 @@ __global__ __launch_bounds__(kThreads) void embedding_join_kernel(Sorted s, uint
     auto chain = [&](uint32_t chunk) {
         const uint64_t begin = (uint64_t)chunk * s.chunk, next = begin + s.chunk;
         if (next >= s.n) return 0u;
-        const uint32_t key = s.key[next];
-        if (key >= vocab || s.key[next - 1] != key || (begin > 0 && s.key[begin - 1] == key)) return 0u;
+        const uint32_t key = s.key(next);
+        if (key >= vocab || s.key(next - 1) != key || (begin > 0 && s.key(begin - 1) == key)) return 0u;
         uint32_t more = 0, got;
         do {
             const uint64_t place = next + (uint64_t)(more + lane) * s.chunk;
-            got = (uint32_t)__popcll(__ballot(place < s.n && s.key[place < s.n ? place : 0] == key));
+            got = (uint32_t)__popcll(__ballot(place < s.n && s.key(place < s.n ? place : 0) == key));
             more += got;
         } while (got == kWave);
         return more + 1;
@@ -204,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void embedding_join_kernel(Sorted s, uint
         Piece<float> out;
 #pragma unroll
         for (int e = 0; e < 4; ++e) out.v[e] = acc[e] * scale;
-        out.store(dtable + (uint64_t)s.key[(uint64_t)(chunk + 1) * s.chunk] * cols + c, left);
+        out.store(dtable + (uint64_t)s.key((uint64_t)(chunk + 1) * s.chunk) * cols + c, left);
     };
     const uint32_t mine = chain(four + wave);
     if (mine && mine <= FEW) {
@@ -243,7 +277,7 @@ struct Plan {
     int passes, bits;  // of the sort
     uint32_t keys;
     uint32_t chunk, chunks;
-    uint64_t counts, list, partial, bytes;  // where the workspace's parts begin; four lists
+    uint64_t counts, list, partial, bytes;  // where the workspace's parts begin; two lists
 };
 
 uint64_t whole_lines(uint64_t bytes) { return (bytes + 127) / 128 * 128; }
@@ -262,7 +296,7 @@ Plan plan(uint64_t n, uint32_t vocab, uint32_t cols, int32_t dtype) {
     p.chunks = (uint32_t)((n + p.chunk - 1) / p.chunk);
     p.counts = 0;
     p.list = whole_lines(sort_bytes(p.keys));
-    p.partial = p.list + 4 * whole_lines(4 * n);
+    p.partial = p.list + 2 * whole_lines(sizeof(Place) * n);
     // of any smaller number of positions too
     const uint64_t some = std::min<uint64_t>((n + kLeastChunk - 1) / kLeastChunk, most);
     p.bytes = std::max<uint64_t>(p.partial + 8 * some * cols, 128);
@@ -318,18 +352,27 @@ int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const in
     TATARA_REQUIRE_ALIGNED(workspace, 16);
     if (int32_t st = check_stream(stream)) return st;
     char* base = static_cast<char*>(workspace);
-    auto list = [&](int i) { return reinterpret_cast<uint32_t*>(base + p.list + i * whole_lines(4 * positions)); };
+    Place* list[2];
+    for (int i = 0; i < 2; ++i)
+        list[i] = reinterpret_cast<Place*>(base + p.list + i * whole_lines(sizeof(Place) * positions));
     float* partial = reinterpret_cast<float*>(base + p.partial);
-    for (int i = 0; positions && i < p.passes; ++i) {
-        const int to = i % 2 * 2, from = 2 - to;
-        const Digit digit{i ? nullptr : token, list(from), list(from + 1), vocab, (uint32_t)(i * p.bits),
-                          p.passes == 1 ? ~0u : p.keys - 1, list(to), list(to + 1)};
-        if (int32_t st = launch_sort(digit, positions, p.keys, reinterpret_cast<uint32_t*>(base + p.counts), raw(stream)))
-            return st;
+    const uint32_t mask = p.passes == 1 ? ~0u : p.keys - 1;
+    const SortShape shape = sort_shape(std::max<uint64_t>(positions, 1), p.keys);
+    if (positions && shape.runs == 1) {
+        with_bits(p.keys, [&](auto bits) {
+            embedding_sort_kernel<decltype(bits)::value><<<1, kSortThreads, sort_lds(p.keys), raw(stream)>>>(
+                token, (uint32_t)positions, shape.run, vocab, p.passes, p.bits, p.keys, mask, list[0], list[1]);
+        });
+        TATARA_LAUNCHED("embedding_sort");
     }
-    const int last = (p.passes - 1) % 2 * 2;
-    const Sorted s{list(last), list(last + 1), (uint32_t)positions, p.chunk, p.chunks};
-    const uint32_t clear = std::min(ceil_div(vocab, kClearRows), 1u << 20);
+    for (int i = 0; shape.runs > 1 && i < p.passes; ++i)
+        if (int32_t st = launch_sort(digit_of(i, p.bits, token, vocab, mask, list[0], list[1]), positions, p.keys,
+                                     reinterpret_cast<uint32_t*>(base + p.counts), raw(stream)))
+            return st;
+    const Sorted s{list[(p.passes - 1) % 2], (uint32_t)positions, p.chunk, p.chunks};
+    // of a small table few rows a workgroup, which clears them at one CU's rate
+    const uint32_t clear_rows = std::max(4u, std::min(kClearRows, vocab / 1024));
+    const uint32_t clear = std::min(ceil_div(vocab, clear_rows), 1u << 20);
     TATARA_FOR_DTYPE(dtype, {
         constexpr int V = Piece<T>::V;
         const uint32_t lanes = sum_lanes(cols, V), slabs = ceil_div(cols, lanes * V);
@@ -337,7 +380,8 @@ int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const in
             constexpr int G = decltype(g)::value;
             const uint32_t blocks = clear + ceil_div((uint64_t)p.chunks * slabs, kThreads / G);
             embedding_sum_kernel<T, G, decltype(few)::value><<<blocks, kThreads, 0, raw(stream)>>>(
-                static_cast<const T*>(dy), dy_stride, s, vocab, cols, scale, dtable, partial, clear, slabs);
+                static_cast<const T*>(dy), dy_stride, s, vocab, cols, scale, dtable, partial, clear, clear_rows,
+                slabs);
         };
         using std::integral_constant;
         if (cols < (uint32_t)V)

@@ -107,10 +107,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_count_kernel(Items items, u
     for (uint32_t e = threadIdx.x; e < width; e += kSortThreads) counts[(uint64_t)blockIdx.x * width + e] = count[e];
 }
 
-template <typename Items, int BITS>
-__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, uint64_t n, uint32_t run, uint32_t keys,
-                                                                  const uint32_t* __restrict__ counts) {
-    extern __shared__ uint32_t shared[];
+// What a workgroup of kSortThreads threads does, with sort_lds(keys) bytes of LDS.  ALONE:
+// there is no other, and no counts.
+template <int BITS, bool ALONE, typename Items>
+__device__ __forceinline__ void sort_place(const Items& items, uint64_t n, uint32_t run, uint32_t keys,
+                                           const uint32_t* __restrict__ counts, uint32_t* shared) {
     const uint32_t width = in_fours(keys);
     uint32_t* next = shared;                     // [wave][key]: the next item's place in its key
     uint32_t* total = next + kSortWaves * keys;  // [width]
@@ -119,10 +120,10 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, u
     uint32_t* part = first + keys + 1;           // [wave]
     const uint32_t wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const uint32_t mine = run / kSortWaves;  // items of a wave, a multiple of kWave
-    const uint64_t from = (uint64_t)blockIdx.x * run + (uint64_t)wave * mine;
+    const uint64_t from = (ALONE ? 0 : (uint64_t)blockIdx.x * run) + (uint64_t)wave * mine;
     typename Items::Item item[kHand];
     uint32_t key[kHand];
-    auto read = [&](uint32_t at0) {
+    auto read = [&](uint32_t at0) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < kHand; ++h) {
             const uint32_t at = at0 + h * kWave + lane;
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, u
     uint32_t all[4] = {}, before[4] = {};
     const uint32_t share = threadIdx.x / (width / 4), four = (threadIdx.x - share * (width / 4)) * 4;
     const uint32_t shares = kSortThreads / (width / 4);
-    if (gridDim.x > 1 && share < shares) {
+    if (!ALONE && share < shares) {
 #pragma unroll 8
         for (uint32_t b = share; b < gridDim.x; b += shares) {
             const uint4 c = *reinterpret_cast<const uint4*>(counts + b * width + four);
@@ -155,7 +156,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, u
         for (int h = 0; h < kHand; ++h)
             if (key[h] < keys) atomicAdd(&my_next[key[h]], 1u);
     }
-    if (gridDim.x > 1 && share < shares) {
+    if (!ALONE && share < shares) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (all[j]) atomicAdd(&total[four + j], all[j]);
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, u
             next[w * keys + e] = s;
             s += c[w];
         }
-        if (gridDim.x == 1) total[e] = s;
+        if (ALONE) total[e] = s;
     }
     const uint32_t count = e < keys ? total[e] : 0u;
     const uint32_t start = sum_ahead(count, part);
@@ -185,25 +186,45 @@ __global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, u
         if (at0 || mine > kWave * kHand) read(at0);
 #pragma unroll
         for (int h = 0; h < kHand; ++h) {
-            if (at0 + h * kWave >= mine) break;
-            const uint64_t i = from + at0 + h * kWave + lane;
-            const bool in = key[h] < keys;
-            const uint64_t same = same_key<BITS>(in, key[h]);
-            const uint64_t below = same & ((1ull << lane) - 1);
-            uint32_t rank = 0;
-            if (in) rank = __hip_atomic_load(&my_next[key[h]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            if (in && below == 0) atomicAdd(&my_next[key[h]], (uint32_t)__popcll(same));  // behind the wave's loads
-            rank += (uint32_t)__popcll(below);
-            if (in)
-                items.put(i, item[h], key[h], first[key[h]], rank);
-            else if (i < n)
-                items.drop(i);
+            if (at0 + h * kWave < mine) {
+                const uint64_t i = from + at0 + h * kWave + lane;
+                const bool in = key[h] < keys;
+                const uint64_t same = same_key<BITS>(in, key[h]);
+                const uint64_t below = same & ((1ull << lane) - 1);
+                uint32_t rank = 0;
+                if (in) rank = __hip_atomic_load(&my_next[key[h]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                // behind the wave's loads
+                if (in && below == 0) atomicAdd(&my_next[key[h]], (uint32_t)__popcll(same));
+                rank += (uint32_t)__popcll(below);
+                if (in)
+                    items.put(i, item[h], key[h], first[key[h]], rank);
+                else if (i < n)
+                    items.drop(i);
+            }
         }
     }
     items.finish(first, keys);
 }
 
+template <typename Items, int BITS, bool ALONE>
+__global__ __launch_bounds__(kSortThreads) void sort_place_kernel(Items items, uint64_t n, uint32_t run, uint32_t keys,
+                                                                  const uint32_t* __restrict__ counts) {
+    extern __shared__ uint32_t shared[];
+    sort_place<BITS, ALONE>(items, n, run, keys, counts, shared);
+}
+
 inline uint32_t sort_lds(uint32_t keys) { return 4 * (kSortWaves * keys + 2 * in_fours(keys) + keys + 1 + kSortWaves); }
+
+// Calls f with bits that tell the keys apart.
+template <typename F>
+void with_bits(uint32_t keys, F&& f) {
+    if (keys <= 16)
+        f(std::integral_constant<int, 4>{});
+    else if (keys <= 128)
+        f(std::integral_constant<int, 7>{});
+    else
+        f(std::integral_constant<int, 10>{});
+}
 
 template <typename Items>
 int32_t launch_sort(const Items& items, uint64_t n, uint32_t keys, uint32_t* counts, hipStream_t stream) {
@@ -212,16 +233,15 @@ int32_t launch_sort(const Items& items, uint64_t n, uint32_t keys, uint32_t* cou
         sort_count_kernel<<<shape.runs, kSortThreads, 0, stream>>>(items, n, shape.run, keys, counts);
         TATARA_LAUNCHED("sort_count");
     }
-    auto place = [&](auto bits) {
-        sort_place_kernel<Items, decltype(bits)::value>
-            <<<shape.runs, kSortThreads, sort_lds(keys), stream>>>(items, n, shape.run, keys, counts);
-    };
-    if (keys <= 16)
-        place(std::integral_constant<int, 4>{});
-    else if (keys <= 128)
-        place(std::integral_constant<int, 7>{});
-    else
-        place(std::integral_constant<int, 10>{});
+    with_bits(keys, [&](auto bits) {
+        constexpr int BITS = decltype(bits)::value;
+        if (shape.runs > 1)
+            sort_place_kernel<Items, BITS, false>
+                <<<shape.runs, kSortThreads, sort_lds(keys), stream>>>(items, n, shape.run, keys, counts);
+        else
+            sort_place_kernel<Items, BITS, true>
+                <<<1, kSortThreads, sort_lds(keys), stream>>>(items, n, shape.run, keys, nullptr);
+    });
     TATARA_LAUNCHED("sort_place");
     return kOk;
 }

@@ -123,9 +123,17 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
             Piece<float> zero;
 #pragma unroll
             for (int e = 0; e < 4; ++e) zero.v[e] = 0.0f;
-            for (uint32_t i = threadIdx.x; i < clear_rows * per_row; i += kThreads) {
-                const uint32_t r = i / per_row, c = (i - r * per_row) * 4;
-                if (none[r]) zero.store(dtable + (first + r) * cols + c, (int)(cols - c));
+            if (per_row >= kWave) {  // a row a wave
+                for (uint32_t r = threadIdx.x / kWave; r < clear_rows; r += kThreads / kWave) {
+                    if (!none[r]) continue;
+                    float* to = dtable + (first + r) * cols;
+                    for (uint32_t c = threadIdx.x % kWave * 4; c < cols; c += kWave * 4) zero.store(to + c, (int)(cols - c));
+                }
+            } else {
+                for (uint32_t i = threadIdx.x; i < clear_rows * per_row; i += kThreads) {
+                    const uint32_t r = i / per_row, c = (i - r * per_row) * 4;
+                    if (none[r]) zero.store(dtable + (first + r) * cols + c, (int)(cols - c));
+                }
             }
         }
         return;
@@ -191,15 +199,16 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
 
 // The rows of tokens that reach over several chunks, of 256 columns.  A wave looks at a
 // chunk: where a token begins in it and goes on, it adds the sums of the chunks that the
-// token is in, and if they are many the workgroup's waves take a quarter of them each.
-__global__ __launch_bounds__(kThreads) void embedding_join_kernel(Sorted s, uint32_t vocab, uint32_t cols, float scale,
+// token is in, and if they are many the workgroup's waves take a part of them each.
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void embedding_join_kernel(Sorted s, uint32_t vocab, uint32_t cols, float scale,
                                                                   const float* __restrict__ partial,
                                                                   float* __restrict__ dtable, uint32_t slabs) {
-    constexpr uint32_t WAVES = kThreads / kWave, FEW = 16;
+    constexpr uint32_t FEW = 16;
     __shared__ float join[WAVES - 1][kWave * 4];
     __shared__ uint32_t many[WAVES];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
-    const uint32_t four = blockIdx.x / slabs * WAVES;
+    const uint32_t chunk0 = blockIdx.x / slabs * WAVES;
     const int c = (int)((blockIdx.x % slabs) * kWave + lane) * 4, left = (int)cols - c;
     // the chunks that the token is in which begins in this one, 0 if it ends there
     auto chain = [&](uint32_t chunk) {
@@ -240,17 +249,17 @@ __global__ __launch_bounds__(kThreads) void embedding_join_kernel(Sorted s, uint
         for (int e = 0; e < 4; ++e) out.v[e] = acc[e] * scale;
         out.store(dtable + (uint64_t)s.key((uint64_t)(chunk + 1) * s.chunk) * cols + c, left);
     };
-    const uint32_t mine = chain(four + wave);
+    const uint32_t mine = chain(chunk0 + wave);
     if (mine && mine <= FEW) {
-        add(four + wave, 0, mine);
-        write(four + wave);
+        add(chunk0 + wave, 0, mine);
+        write(chunk0 + wave);
     }
     if (lane == 0) many[wave] = mine > FEW ? mine : 0;
     __syncthreads();
     for (uint32_t w = 0; w < WAVES; ++w) {
         const uint32_t terms = many[w];
         if (!terms) continue;
-        add(four + w, (uint32_t)((uint64_t)terms * wave / WAVES), (uint32_t)((uint64_t)terms * (wave + 1) / WAVES));
+        add(chunk0 + w, (uint32_t)((uint64_t)terms * wave / WAVES), (uint32_t)((uint64_t)terms * (wave + 1) / WAVES));
         if (wave) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) join[wave - 1][lane * 4 + e] = acc[e];
@@ -260,8 +269,8 @@ __global__ __launch_bounds__(kThreads) void embedding_join_kernel(Sorted s, uint
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (uint32_t o = 0; o < WAVES - 1; ++o) acc[e] += join[o][lane * 4 + e];
-            write(four + w);
+                for (int o = 0; o < WAVES - 1; ++o) acc[e] += join[o][lane * 4 + e];
+            write(chunk0 + w);
         }
         __syncthreads();
     }
@@ -396,8 +405,17 @@ int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const in
     TATARA_LAUNCHED("embedding_sum");
     if (p.chunks > 1) {
         const uint32_t slabs = ceil_div(cols, kWave * 4);
-        embedding_join_kernel<<<ceil_div(p.chunks - 1, kThreads / kWave) * slabs, kThreads, 0, raw(stream)>>>(s, vocab, cols, scale, partial,
-                                                                                  dtable, slabs);
+        auto launch = [&](auto waves) {
+            constexpr int WAVES = decltype(waves)::value;
+            embedding_join_kernel<WAVES><<<ceil_div(p.chunks - 1, WAVES) * slabs, WAVES * kWave, 0, raw(stream)>>>(
+                s, vocab, cols, scale, partial, dtable, slabs);
+        };
+        // sixteen waves where a token is in many chunks (65536 x 1536 f32 of 2 tokens: the call 104
+        // us, so 97; of 73305 217 and 222)
+        if (positions / vocab > 16ull * p.chunk)
+            launch(std::integral_constant<int, 16>{});
+        else
+            launch(std::integral_constant<int, 4>{});
         TATARA_LAUNCHED("embedding_join");
     }
     return kOk;

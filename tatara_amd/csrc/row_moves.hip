@@ -93,9 +93,10 @@ __global__ __launch_bounds__(kThreads) void rows_back_kernel(RowsBack a, uint32_
 }
 
 // DOT: the gates' gradient too.  The first `clear` workgroups clear the rows without a
-// source, kWave of them a wave.
+// source, of which a wave looks at `clear_rows`.
 template <typename T, int K, int U, bool FEW, bool DOT>
-__global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t lanes, uint32_t clear) {
+__global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t lanes, uint32_t clear,
+                                                           uint32_t clear_rows) {
     constexpr int V = Piece<T>::V;
     const int cols = (int)a.cols;
     T* rows = static_cast<T*>(a.rows);
@@ -105,10 +106,12 @@ __global__ __launch_bounds__(kThreads) void rows_out_kernel(RowsOut a, uint32_t 
         Piece<T> zero;
 #pragma unroll
         for (int e = 0; e < V; ++e) zero.v[e] = (T)0.0f;
-        for (uint64_t first = (uint64_t)blockIdx.x * kThreads + threadIdx.x / kWave * kWave; first < a.n_rows;
-             first += (uint64_t)clear * kThreads) {
+        constexpr uint32_t WAVES = kThreads / kWave;
+        for (uint64_t first = ((uint64_t)blockIdx.x * WAVES + threadIdx.x / kWave) * clear_rows; first < a.n_rows;
+             first += (uint64_t)clear * WAVES * clear_rows) {
             const uint64_t mine = first + lane;
-            uint64_t none = __ballot(mine < a.n_rows && (uint32_t)a.source[mine < a.n_rows ? mine : 0] >= items);
+            const bool look = lane < clear_rows && mine < a.n_rows;
+            uint64_t none = __ballot(look && (uint32_t)a.source[look ? mine : first] >= items);
             for (; none; none &= none - 1) {
                 T* to = rows + (int64_t)(first + __builtin_ctzll(none)) * a.rows_stride;
                 for (int c = (int)lane * V; c < cols; c += kWave * V) zero.store(to + c, cols - c);
@@ -251,7 +254,7 @@ int32_t launch_rows_back(const RowsBack& a, int32_t dtype, hipStream_t stream) {
         constexpr int V = Piece<T>::V;
         const bool past = past_caches(a.positions * a.cols * sizeof(T));
         with_top(a.top_k, [&](auto k) {
-            constexpr int K = decltype(k)::value, MOST = K <= 2 ? 4 : 1;
+            constexpr int K = decltype(k)::value, MOST = K <= 4 ? 4 : 1;
             if (a.cols < (uint32_t)V) {
                 rows_back_kernel<T, K, 1, true>
                     <<<position_blocks(a.positions, 1), kThreads, 0, stream>>>(a, 1, past);
@@ -272,21 +275,26 @@ int32_t launch_rows_out(const RowsOut& a, int32_t dtype, hipStream_t stream) {
     if (a.positions == 0 && a.n_rows == 0) return kOk;
     TATARA_FOR_DTYPE(dtype, {
         constexpr int V = Piece<T>::V;
-        const uint32_t clear = position_blocks(a.n_rows, 1);
+        // few rows a wave where there are few: it clears them one after the other
+        uint32_t clear_rows = 1;
+        while (clear_rows < kWave && a.n_rows > 4096ull * clear_rows) clear_rows *= 2;
+        const uint32_t clear = (uint32_t)std::min<uint64_t>(
+            (a.n_rows + kThreads / kWave * clear_rows - 1) / (kThreads / kWave * clear_rows), kMaxGrid);
         with_top(a.top_k, [&](auto k) {
             auto launch = [&](auto dot) {
                 constexpr bool DOT = decltype(dot)::value;
-                constexpr int K = decltype(k)::value, MOST = !DOT || K <= 2 ? 4 : 1;
+                constexpr int K = decltype(k)::value, MOST = !DOT || K <= 4 ? 4 : 1;
                 if (a.cols < (uint32_t)V) {
                     rows_out_kernel<T, K, 1, true, DOT>
-                        <<<clear + position_blocks(a.positions, 1), kThreads, 0, stream>>>(a, 1, clear);
+                        <<<clear + position_blocks(a.positions, 1), kThreads, 0, stream>>>(a, 1, clear,
+                                                                                             clear_rows);
                     return;
                 }
                 const RowForm form = row_form(a.cols, V, MOST);
                 with_pieces<MOST>(form.pieces, [&](auto u) {
                     rows_out_kernel<T, K, decltype(u)::value, false, DOT>
                         <<<clear + position_blocks(a.positions, form.lanes), kThreads, 0, stream>>>(a, form.lanes,
-                                                                                                    clear);
+                                                                                                    clear, clear_rows);
                 });
             };
             a.dgate ? launch(std::true_type{}) : launch(std::false_type{});

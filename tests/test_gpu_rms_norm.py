@@ -18,7 +18,8 @@ EPS32 = 2.0**-24
 
 # either side of a piece, of the widths where more waves share a row, of the rows where one does
 SHAPES = [(1, 1), (1, 1536), (3, 7), (5, 64), (2, 65), (70, 256), (33, 257), (9, 770), (2100, 96), (2049, 513),
-          (1100, 1536), (1100, 1537), (4, 2049), (3, 6145), (2, 8193), (2, 32768)]
+          (1100, 1536), (1100, 1537), (4, 2049), (3, 6145), (2, 8193), (2, 32768),
+          (5000, 33), (4097, 16), (3000, 9), (2051, 128), (1029, 130), (2500, 3)]
 
 
 def rows_of(g, rows, cols, pad, dtype, scale=1.0):

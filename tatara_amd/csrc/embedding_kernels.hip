@@ -21,8 +21,12 @@ constexpr uint32_t kMaxVocab = 1u << 28;
 // Rows of the table that a workgroup looks up at most, and clears where no position has one.
 constexpr uint32_t kClearRows = 128;
 constexpr int kBatch = 8;            // rows that a lane has in hand
-constexpr uint32_t kMostChunks = 1024;  // of rows as wide as a wave
-constexpr uint32_t kLeastChunk = 8;     // positions
+// Waves that have a chunk each, at most (200000 x 256 f32 of 9 rows: with 1024 62 us, 2048 49, 4096
+// 55), and chunks, of which wide rows take several waves each.
+constexpr uint32_t kMostWaves = 2048, kMostChunks = 1024;
+// Positions of a chunk at least; twice as many of narrow rows, whose waves have several chunks
+// (65536 x 16 f32 of 81 rows: 25 us, so 19.4).
+constexpr uint32_t kLeastChunk = 8;
 
 // A position and its token.
 struct alignas(8) Place {
@@ -279,7 +283,7 @@ __global__ __launch_bounds__(WAVES * kWave) void embedding_join_kernel(Sorted s,
 // Lanes of a row.
 uint32_t sum_lanes(uint32_t cols, int v) {
     const uint32_t pieces = ceil_div(cols, v);
-    return pieces <= 4 ? 4 : pieces <= 16 ? 16 : kWave;
+    return pieces <= 4 ? 4 : pieces <= 16 ? 16 : pieces <= 32 ? 32 : kWave;
 }
 
 struct Plan {
@@ -299,8 +303,9 @@ Plan plan(uint64_t n, uint32_t vocab, uint32_t cols, int32_t dtype) {
     p.bits = (bits + p.passes - 1) / p.passes;
     p.keys = p.passes == 1 ? vocab + 1 : 1u << p.bits;
     // chunks enough to fill the GPU, of rows enough that few of them are joined
-    const uint64_t most = (uint64_t)kMostChunks * (kWave / sum_lanes(cols, 16 / elem_bytes(dtype)));
-    p.chunk = kLeastChunk;
+    const uint32_t v = 16 / elem_bytes(dtype), lanes = sum_lanes(cols, v), slabs = ceil_div(cols, lanes * v);
+    const uint64_t most = (uint64_t)std::max(kMostChunks, kMostWaves / slabs) * (kWave / lanes);
+    p.chunk = lanes == kWave ? kLeastChunk : 2 * kLeastChunk;
     while ((n + p.chunk - 1) / p.chunk > most) p.chunk *= 2;
     p.chunks = (uint32_t)((n + p.chunk - 1) / p.chunk);
     p.counts = 0;
@@ -399,6 +404,8 @@ int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const in
             launch(integral_constant<int, 4>{}, std::false_type{});
         else if (lanes == 16)
             launch(integral_constant<int, 16>{}, std::false_type{});
+        else if (lanes == 32)
+            launch(integral_constant<int, 32>{}, std::false_type{});
         else
             launch(integral_constant<int, 64>{}, std::false_type{});
     });

@@ -35,7 +35,8 @@ struct Choices {
     __device__ __forceinline__ void drop(uint64_t i) const { slot[i] = -1; }
     // The rows that no choice has.
     __device__ __forceinline__ void finish(const uint32_t* first, uint32_t keys) const {
-        const uint64_t threads = (uint64_t)gridDim.x * kSortThreads, me = (uint64_t)blockIdx.x * kSortThreads + threadIdx.x;
+        const uint64_t threads = (uint64_t)gridDim.x * kSortThreads;
+        const uint64_t me = (uint64_t)blockIdx.x * kSortThreads + threadIdx.x;
         if (capacity) {
             for (uint64_t r = me; r < n_rows; r += threads) {
                 const uint32_t e = (uint32_t)r / capacity;

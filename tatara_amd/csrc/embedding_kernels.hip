@@ -10,6 +10,10 @@
 // that a token that nearly all positions have costs no more than others.  A chunk's
 // first and last token may reach into its neighbours: their sums go to `partial` and are
 // joined in order by a last launch.
+//
+// 65536 x 1536 f32 of 73305 rows, 453 MB of them zeros or sums: 217 us, of which the sums and
+// zeros take 182 (853 MB, 4.7 TB/s, as a copy of that size), four launches of the sort 29 and the
+// join 9.  Of 2 rows 97 us (floor 81).  1000 x 768 of 2000 rows: 16.5 us in three launches.
 #include "key_sort.hpp"
 #include "row_moves.hpp"
 
@@ -20,7 +24,7 @@ constexpr int kThreads = 256;
 constexpr uint32_t kMaxVocab = 1u << 28;
 // Rows of the table that a workgroup looks up at most, and clears where no position has one.
 constexpr uint32_t kClearRows = 128;
-constexpr int kBatch = 8;            // rows that a lane has in hand
+constexpr int kBatch = 8;  // rows that a lane has in hand
 // Waves that have a chunk each, at most (200000 x 256 f32 of 9 rows: with 1024 62 us, 2048 49, 4096
 // 55), and chunks, of which wide rows take several waves each.
 constexpr uint32_t kMostWaves = 2048, kMostChunks = 1024;
@@ -95,7 +99,8 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
     const bool clears = cleared != (uint32_t)((uint64_t)(blockIdx.x + 1) * clear / gridDim.x);
     if (clears) {
         __shared__ bool none[kClearRows];
-        constexpr uint32_t LANES = 8, ROWS = kThreads / LANES, TURNS = kClearRows / ROWS;  // lanes look for TURNS rows at once
+        // eight lanes look for a row, for TURNS of them at once
+        constexpr uint32_t LANES = 8, ROWS = kThreads / LANES, TURNS = kClearRows / ROWS;
         const uint32_t per_row = (cols + 3) / 4, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
         for (uint64_t first = (uint64_t)cleared * clear_rows; first < vocab; first += (uint64_t)clear * clear_rows) {
             __syncthreads();
@@ -131,7 +136,8 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
                 for (uint32_t r = threadIdx.x / kWave; r < clear_rows; r += kThreads / kWave) {
                     if (!none[r]) continue;
                     float* to = dtable + (first + r) * cols;
-                    for (uint32_t c = threadIdx.x % kWave * 4; c < cols; c += kWave * 4) zero.store(to + c, (int)(cols - c));
+                    for (uint32_t c = threadIdx.x % kWave * 4; c < cols; c += kWave * 4)
+                        zero.store(to + c, (int)(cols - c));
                 }
             } else {
                 for (uint32_t i = threadIdx.x; i < clear_rows * per_row; i += kThreads) {
@@ -205,9 +211,9 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
 // chunk: where a token begins in it and goes on, it adds the sums of the chunks that the
 // token is in, and if they are many the workgroup's waves take a part of them each.
 template <int WAVES>
-__global__ __launch_bounds__(WAVES * kWave) void embedding_join_kernel(Sorted s, uint32_t vocab, uint32_t cols, float scale,
-                                                                  const float* __restrict__ partial,
-                                                                  float* __restrict__ dtable, uint32_t slabs) {
+__global__ __launch_bounds__(WAVES * kWave) void embedding_join_kernel(Sorted s, uint32_t vocab, uint32_t cols,
+                                                                       float scale, const float* __restrict__ partial,
+                                                                       float* __restrict__ dtable, uint32_t slabs) {
     constexpr uint32_t FEW = 16;
     __shared__ float join[WAVES - 1][kWave * 4];
     __shared__ uint32_t many[WAVES];
@@ -342,8 +348,9 @@ int32_t tatara_op_embedding_forward(const int32_t* token, uint64_t positions, co
     TATARA_REQUIRE_ALIGNED(table, elem_bytes(dtype));
     TATARA_REQUIRE_ALIGNED(y, elem_bytes(dtype));
     if (int32_t st = check_stream(stream)) return st;
-    return launch_rows_back(RowsBack{table, table_stride, vocab, token, nullptr, scale, y, y_stride, positions, 1, cols},
-                            dtype, raw(stream));
+    return launch_rows_back(
+        RowsBack{table, table_stride, vocab, token, nullptr, scale, y, y_stride, positions, 1, cols}, dtype,
+        raw(stream));
 }
 
 int32_t tatara_op_embedding_backward_workspace(uint64_t positions, uint32_t vocab, uint32_t cols, int32_t dtype,

@@ -7,6 +7,10 @@
 // ahead.  With one workgroup all of that is one launch; with more, a first launch
 // counts the keys of every run.  Counts are whole numbers: nothing depends on the order
 // in which they are added.
+//
+// Bound by latency: 8192 items of 9 keys in one workgroup 7.8 us, 65536 in 64 of them 2.7 and
+// 5.8, of 512 keys 2.7 and 9.3 (every workgroup adds up the counts of all; read one key at a
+// time and not ahead 14.8).
 #pragma once
 
 #include "elem.hpp"
@@ -22,7 +26,7 @@ constexpr uint32_t kMaxRuns = 256;
 // Items that one workgroup sorts alone, and that a workgroup has at least.
 constexpr uint32_t kAlone = 8192;
 constexpr uint32_t kLeastRun = 1024;
-// Counts of all runs at most: every workgroup adds them up.
+// Counts of all runs at most (65536 items of 512 keys: 9.3 us, with twice as many 10.0).
 constexpr uint32_t kMostCounts = 16384;
 
 struct SortShape {

@@ -9,11 +9,20 @@
 //             ds = rstd (g - h sum_c (g h) / C) + dtotal,  dw = sum_r dy h
 //
 // Every sum is f32 and in a fixed order (no atomics).
+//
+// A row stays in registers between its sum and its use, so each value is read and
+// written once: bound by memory, 65536 x 1536 bf16 with a residual and its sum 144 us
+// (5.6 TB/s; a copy of 400 MB runs at 5.4).  In 8 bits also by instructions, 140 a lane of
+// eight values: 16381 x 2048 f16 with scales of 128 columns 21 to 23 us (100 MB; a plain cast
+// 21.8).  A row alone takes 3 us, the backward pass of 1009 x 769 f32 5.9 and 3.2 in two
+// launches.
 #include "norm_rows.hpp"
 
 namespace tatara {
 namespace {
 
+// Workgroups of an output in 8 bits at most: four rows each of 16384, so that the weight is
+// loaded once for them (16381 x 2048 f16: 23.0 us, with one row each 25.0, with 2048 23.4).
 constexpr uint32_t kBits8Blocks = 4096;
 
 // The larger; NaN if either is.

@@ -5,6 +5,11 @@
 // a wave), so that a position's own row is read or written once, however many choices it
 // has, and the rows it meets elsewhere are whole ones.  A lane keeps the slots and
 // weights of its position's K choices in registers.
+//
+// Bound by memory: 65536 x 1536 f32 gathered 146 us (805 MB, 5.5 TB/s), 32768 x 768 f16 with
+// two choices back with the gates' gradient 49 (252 MB, 5.1), 65536 x 768 bf16 of a table of
+// 1629 rows 22.4 (writes at 4.5; the table comes from the last-level cache as often as the
+// rows written push it out of the L2).  More positions in hand a lane are no faster.
 #include "row_moves.hpp"
 
 namespace tatara {

@@ -412,7 +412,7 @@ TATARA_API int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride
  * stored.  The step is `step`, plus *more_steps if that is given (device memory, read
  * when the call runs: a captured graph's replays take other masks by it).  p in [0, 1).
  * A dropped value is 0 whatever it was.  The gradient of x is the same call on dy with
- * no residual. */
+ * no residual.  y may be x or residual, with the same stride. */
 TATARA_API int32_t tatara_op_dropout(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
                                      void* y, int64_t y_stride, uint64_t rows, uint32_t cols, double p, uint64_t seed,
                                      uint64_t step, const uint64_t* more_steps, uint32_t first_row, int32_t dtype,

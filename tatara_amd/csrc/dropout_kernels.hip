@@ -43,13 +43,14 @@ __device__ __forceinline__ Words philox(uint32_t a, uint32_t b, uint32_t c, uint
 }
 
 // A workgroup takes kThreads * kPieces consecutive pieces of the rows, `per_row` of
-// them a row.  FEW: rows of fewer elements than a piece has.
-template <typename T, bool FEW, bool ADD>
+// them a row.  FEW: rows of fewer elements than a piece has.  In place, a row's last piece
+// is read again by elements where it is not a whole one: what stands for it otherwise, the
+// row's last 16 bytes, another wave may have written by then.
+template <typename T, bool FEW, bool ADD, bool IN_PLACE>
 __global__ __launch_bounds__(kThreads) void dropout_kernel(
-    const T* __restrict__ x, int64_t x_stride, const T* __restrict__ residual, int64_t residual_stride,
-    T* __restrict__ y, int64_t y_stride, uint64_t pieces, uint32_t per_row, uint32_t cols, uint32_t first_row,
-    uint32_t threshold, float scale, uint32_t key0, uint32_t key1, uint64_t step,
-    const uint64_t* __restrict__ more_steps) {
+    const T* x, int64_t x_stride, const T* residual, int64_t residual_stride, T* y, int64_t y_stride, uint64_t pieces,
+    uint32_t per_row, uint32_t cols, uint32_t first_row, uint32_t threshold, float scale, uint32_t key0, uint32_t key1,
+    uint64_t step, const uint64_t* __restrict__ more_steps) {
     constexpr int V = Piece<T>::V;
     if (more_steps) step += *more_steps;
     constexpr uint32_t kAtOnce = kThreads * kPieces;
@@ -90,8 +91,13 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(
                 for (int j = 0; j < 4; ++j) u[4 * b + j] = w.v[j];
             }
             if (!FEW) {
-                in[i].fix(left);
-                if constexpr (ADD) add[i].fix(left);
+                if (IN_PLACE && left < V) {
+                    in[i].load_few(x + (int64_t)row[i] * x_stride + col[i], left);
+                    if constexpr (ADD) add[i].load_few(residual + (int64_t)row[i] * residual_stride + col[i], left);
+                } else {
+                    in[i].fix(left);
+                    if constexpr (ADD) add[i].fix(left);
+                }
             }
             Piece<T> out;
 #pragma unroll
@@ -99,6 +105,7 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(
                 // what is dropped is zero whatever it was
                 float v = u[j] >= threshold ? (float)in[i].v[j] * scale : 0.0f;
                 if constexpr (ADD) v += (float)add[i].v[j];
+                asm("" : "+v"(v));  // f16: rounded to f32 first in every form of this kernel
                 out.v[j] = (T)v;
             }
             if (here[i]) out.store(y + (int64_t)row[i] * y_stride + col[i], left);
@@ -128,6 +135,8 @@ extern "C" int32_t tatara_op_dropout(const void* x, int64_t x_stride, const void
     TATARA_REQUIRE_ALIGNED(residual, elem_bytes(dtype));
     TATARA_REQUIRE_ALIGNED(y, elem_bytes(dtype));
     TATARA_REQUIRE_ALIGNED(more_steps, 8);
+    TATARA_REQUIRE((y != x || y_stride == x_stride) && (y != residual || y_stride == residual_stride),
+                   "in place the strides are the same");
     if (int32_t st = check_stream(stream)) return st;
     // p next to 1 rounds to 2^32, which no number reaches
     const uint32_t threshold = (uint32_t)std::min(nearbyint(p * 0x1p32), 0x1p32 - 1.0);
@@ -138,13 +147,20 @@ extern "C" int32_t tatara_op_dropout(const void* x, int64_t x_stride, const void
         const uint64_t pieces = rows * per_row;
         constexpr uint64_t AT_ONCE = kThreads * kPieces;
         const uint32_t blocks = (uint32_t)std::min<uint64_t>((pieces + AT_ONCE - 1) / AT_ONCE, kMaxGrid);
-        auto launch = [&](auto few, auto add) {
-            dropout_kernel<T, decltype(few)::value, decltype(add)::value><<<blocks, kThreads, 0, raw(stream)>>>(
-                static_cast<const T*>(x), x_stride, static_cast<const T*>(residual), residual_stride,
-                static_cast<T*>(y), y_stride, pieces, per_row, cols, first_row, threshold, scale, (uint32_t)seed,
-                (uint32_t)(seed >> 32), step, more_steps);
+        auto launch = [&](auto few, auto add, auto in_place) {
+            dropout_kernel<T, decltype(few)::value, decltype(add)::value, decltype(in_place)::value>
+                <<<blocks, kThreads, 0, raw(stream)>>>(
+                    static_cast<const T*>(x), x_stride, static_cast<const T*>(residual), residual_stride,
+                    static_cast<T*>(y), y_stride, pieces, per_row, cols, first_row, threshold, scale, (uint32_t)seed,
+                    (uint32_t)(seed >> 32), step, more_steps);
         };
-        auto with_add = [&](auto few) { residual ? launch(few, std::true_type{}) : launch(few, std::false_type{}); };
+        auto with_place = [&](auto few, auto add) {
+            (y == x || y == residual) && cols % V ? launch(few, add, std::true_type{})
+                                                  : launch(few, add, std::false_type{});
+        };
+        auto with_add = [&](auto few) {
+            residual ? with_place(few, std::true_type{}) : with_place(few, std::false_type{});
+        };
         cols < (uint32_t)V ? with_add(std::true_type{}) : with_add(std::false_type{});
     });
     TATARA_LAUNCHED("dropout");

@@ -87,7 +87,10 @@ __global__ __launch_bounds__(kThreads) void rows_back_kernel(RowsBack a, uint32_
                 }
                 Piece<T> out;
 #pragma unroll
-                for (int e = 0; e < V; ++e) out.v[e] = (T)y[e];
+                for (int e = 0; e < V; ++e) {
+                    asm("" : "+v"(y[e]));  // f16: rounded to f32 first in every form
+                    out.v[e] = (T)y[e];
+                }
                 if (past)
                     out.store_past(to + c, cols - c);
                 else

@@ -518,8 +518,8 @@ class Dropout:
         self._lib = _lib.load()
 
     def forward(self, x, y, step: int = 0, residual=None, more_steps=None, first_row: int = 0, stream=None) -> None:
-        """Writes y.  The step is `step` plus more_steps ([1], int64) if that is given,
-        which is read when the call runs."""
+        """Writes y, which may be x or residual.  The step is `step` plus more_steps ([1],
+        int64) if that is given, which is read when the call runs."""
         here, queue = _place(x, stream)
         rows = _count("x", x, self.cols, self.dtype)
         shape = (rows, self.cols)
@@ -538,8 +538,8 @@ class Dropout:
             check(status)
 
     def backward(self, dy, dx, step: int = 0, more_steps=None, first_row: int = 0, stream=None) -> None:
-        """Writes dx of the forward call with the same step (the residual's gradient is
-        dy itself)."""
+        """Writes dx, which may be dy, of the forward call with the same step (the
+        residual's gradient is dy itself)."""
         self.forward(dy, dx, step, None, more_steps, first_row, stream)
 
 

@@ -116,6 +116,8 @@ def test_dropout_refuses():
         refused(dropout(**{stride: 15}), b"stride")
     for p in ("x", "res", "y", "more"):
         refused(dropout(**{p: FAKE + 2}), b"aligned")
+    refused(dropout(ys=17), b"in place")
+    refused(dropout(x=2 * FAKE, ys=17), b"in place")
 
 
 def test_bucket_rows_refuse():

@@ -48,6 +48,22 @@ def test_forward_and_backward(gpu, rows, cols, dtype, p, add):
     assert torch.equal(dx, expected(dy, None, keep, p))
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,cols", [(3, 2), (700, 7), (5000, 130), (40, 1537), (3, 40000)])
+def test_in_place(gpu, rows, cols, dtype):
+    g = torch.Generator().manual_seed(cols)
+    x, res = rows_of(g, rows, cols, 5, dtype), rows_of(g, rows, cols, 5, dtype)
+    op, y = ops.Dropout(cols, 0.4, dtype, SEED), torch.empty(rows, cols, dtype=TYPES[dtype], device="cuda")
+    op.forward(x, y, 9, res)
+    for to in (0, 1):
+        pair = [x.clone(), res.clone()]
+        op.forward(pair[0], pair[to], 9, pair[1])
+        assert torch.equal(pair[to], y)
+    op.forward(x, y, 9)
+    op.backward(x, x, 9)
+    assert torch.equal(x, y)
+
+
 def test_a_part_of_a_batch_and_steps_on_the_device(gpu):
     g = torch.Generator().manual_seed(0)
     x = torch.randn(300, 77, generator=g).cuda()

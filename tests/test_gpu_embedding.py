@@ -39,11 +39,11 @@ def test_forward(gpu, n, v, cols, dtype):
     t, table = tokens(g, n, v, "any").cuda(), rows_of(g, v, cols, pad, dtype)
     wide = torch.full((n, cols + 3), 7.0, dtype=TYPES[dtype], device="cuda")
     y = wide[:, 1:cols + 1]
-    scale = 5.25
-    ops.Embedding(v, cols, n, dtype, scale).forward(t, table, y)
     known = (t >= 0) & (t < v)
-    want = table[torch.where(known, t, 0).long()].float() * scale
-    assert torch.equal(y, torch.where(known[:, None], want, 0.0).to(TYPES[dtype]))
+    for scale in (5.25, 768.0**0.5):
+        ops.Embedding(v, cols, n, dtype, scale).forward(t, table, y)
+        want = table[torch.where(known, t, 0).long()].float() * scale
+        assert torch.equal(y, torch.where(known[:, None], want, 0.0).to(TYPES[dtype]))
     assert (wide[:, :1] == 7.0).all() and (wide[:, cols + 1:] == 7.0).all()
 
 

@@ -13,7 +13,8 @@
 //
 // 65536 x 1536 f32 of 73305 rows, 453 MB of them zeros or sums: 217 us, of which the sums and
 // zeros take 182 (853 MB, 4.7 TB/s, as a copy of that size), four launches of the sort 29 and the
-// join 9.  Of 2 rows 97 us (floor 81).  1000 x 768 of 2000 rows: 16.5 us in three launches.
+// join 9.  Of 2 rows 97 us (floor 81).  1000 x 768 of 2000 rows: 16.5 us in three launches; up to
+// 256 positions take one.
 #include "key_sort.hpp"
 #include "row_moves.hpp"
 
@@ -31,6 +32,10 @@ constexpr uint32_t kMostWaves = 2048, kMostChunks = 1024;
 // Positions of a chunk at least; twice as many of narrow rows, whose waves have several chunks
 // (65536 x 16 f32 of 81 rows: 25 us, so 19.4).
 constexpr uint32_t kLeastChunk = 8;
+
+// Positions that need no sort: a thread each where rows are cleared.
+constexpr uint32_t kFewPositions = 256;
+static_assert(kFewPositions <= kThreads && kClearRows <= kThreads, "one turn of a workgroup");
 
 // A position and its token.
 struct alignas(8) Place {
@@ -84,6 +89,26 @@ struct Sorted {
     __device__ __forceinline__ uint32_t key(uint64_t i) const { return place[i].key; }
 };
 
+// Zeros in the rows that no position has.
+__device__ __forceinline__ void clear_rows_of(const bool* none, uint32_t rows, float* table, uint32_t cols) {
+    const uint32_t per_row = (cols + 3) / 4;
+    Piece<float> zero;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) zero.v[e] = 0.0f;
+    if (per_row >= kWave) {  // a row a wave
+        for (uint32_t r = threadIdx.x / kWave; r < rows; r += kThreads / kWave) {
+            if (!none[r]) continue;
+            float* to = table + (uint64_t)r * cols;
+            for (uint32_t c = threadIdx.x % kWave * 4; c < cols; c += kWave * 4) zero.store(to + c, (int)(cols - c));
+        }
+    } else {
+        for (uint32_t i = threadIdx.x; i < rows * per_row; i += kThreads) {
+            const uint32_t r = i / per_row, c = (i - r * per_row) * 4;
+            if (none[r]) zero.store(table + (uint64_t)r * cols + c, (int)(cols - c));
+        }
+    }
+}
+
 // A group of G lanes adds the rows of a chunk, V columns a lane; rows wider than a wave
 // are cut into `slabs`.  `clear` workgroups write the rows of the table that no position
 // has.
@@ -101,7 +126,7 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
         __shared__ bool none[kClearRows];
         // eight lanes look for a row, for TURNS of them at once
         constexpr uint32_t LANES = 8, ROWS = kThreads / LANES, TURNS = kClearRows / ROWS;
-        const uint32_t per_row = (cols + 3) / 4, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+        const uint32_t lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
         for (uint64_t first = (uint64_t)cleared * clear_rows; first < vocab; first += (uint64_t)clear * clear_rows) {
             __syncthreads();
             uint32_t lo[TURNS], hi[TURNS];  // the first place with a key of the row or above lies in lo..hi
@@ -129,22 +154,7 @@ __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const T* __rest
                 if (lane == 0) none[q * ROWS + group] = v < vocab && !(lo[q] < s.n && s.key(lo[q]) == v);
             }
             __syncthreads();
-            Piece<float> zero;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) zero.v[e] = 0.0f;
-            if (per_row >= kWave) {  // a row a wave
-                for (uint32_t r = threadIdx.x / kWave; r < clear_rows; r += kThreads / kWave) {
-                    if (!none[r]) continue;
-                    float* to = dtable + (first + r) * cols;
-                    for (uint32_t c = threadIdx.x % kWave * 4; c < cols; c += kWave * 4)
-                        zero.store(to + c, (int)(cols - c));
-                }
-            } else {
-                for (uint32_t i = threadIdx.x; i < clear_rows * per_row; i += kThreads) {
-                    const uint32_t r = i / per_row, c = (i - r * per_row) * 4;
-                    if (none[r]) zero.store(dtable + (first + r) * cols + c, (int)(cols - c));
-                }
-            }
+            clear_rows_of(none, clear_rows, dtable + first * cols, cols);
         }
         return;
     }
@@ -286,6 +296,93 @@ __global__ __launch_bounds__(WAVES * kWave) void embedding_join_kernel(Sorted s,
     }
 }
 
+// The whole gradient of few positions in one launch, without a sort: a wave a position and
+// 64 V columns adds the rows of all positions with its token if none ahead of it has that token.
+// (64 x 256 f32 of 1000 rows 2.5 us, by sort, sum and join 11.6; 256 x 1536 of 2 rows, 128
+// positions each, 11.0 and 12.)
+template <typename T, bool FEW>
+__global__ __launch_bounds__(kThreads) void embedding_few_kernel(const T* __restrict__ dy, int64_t dy_stride,
+                                                                 const int32_t* __restrict__ token, uint32_t n,
+                                                                 uint32_t vocab, uint32_t cols, float scale,
+                                                                 float* __restrict__ dtable, uint32_t clear,
+                                                                 uint32_t clear_rows, uint32_t slabs) {
+    constexpr int V = Piece<T>::V;
+    if (blockIdx.x < clear) {
+        __shared__ bool none[kClearRows];
+        for (uint64_t first = (uint64_t)blockIdx.x * clear_rows; first < vocab; first += (uint64_t)clear * clear_rows) {
+            __syncthreads();
+            if (threadIdx.x < clear_rows) none[threadIdx.x] = first + threadIdx.x < vocab;
+            __syncthreads();
+            if (threadIdx.x < n) {
+                const uint64_t row = (uint64_t)(uint32_t)token[threadIdx.x] - first;  // wraps below it
+                if (row < clear_rows) none[row] = false;
+            }
+            __syncthreads();
+            clear_rows_of(none, clear_rows, dtable + first * cols, cols);
+        }
+        return;
+    }
+    const uint32_t unit = __builtin_amdgcn_readfirstlane((blockIdx.x - clear) * (kThreads / kWave) + threadIdx.x / kWave);
+    const uint32_t i = unit / slabs, lane = threadIdx.x % kWave;
+    if (i >= n) return;
+    const uint32_t key = (uint32_t)token[i];
+    uint64_t same[kFewPositions / kWave];
+#pragma unroll
+    for (uint32_t k = 0; k < kFewPositions / kWave; ++k) {
+        const uint32_t j = k * kWave + lane;
+        same[k] = __ballot(j < n && (uint32_t)token[j < n ? j : 0] == key);
+    }
+    if (key >= vocab) return;
+#pragma unroll
+    for (uint32_t k = 0; k < kFewPositions / kWave; ++k) {
+        const uint64_t ahead = i >= (k + 1) * kWave ? ~0ull : i > k * kWave ? (1ull << (i - k * kWave)) - 1 : 0;
+        if (same[k] & ahead) return;
+    }
+    const int c = (int)((unit - i * slabs) * kWave + lane) * V, left = (int)cols - c;
+    if (left <= 0) return;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+    auto add = [&](auto hand, uint64_t& from, uint32_t base) __attribute__((always_inline)) {
+        constexpr int HAND = decltype(hand)::value;
+        Piece<T> p[HAND];
+        const uint64_t all = from;
+        uint32_t at = 0;
+#pragma unroll
+        for (int k = 0; k < HAND; ++k) {  // behind the last the last again
+            at = from ? base + (uint32_t)__builtin_ctzll(from) : at;
+            from &= from - 1;
+            const T* row = dy + (int64_t)at * dy_stride;
+            if (FEW)
+                p[k].load_few(row, (int)cols);
+            else
+                p[k].load(row, c, (int)cols);
+        }
+        const int count = __popcll(all);
+#pragma unroll
+        for (int k = 0; k < HAND; ++k) {
+            if (!FEW) p[k].fix(left);
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] = k < count ? acc[e] + (float)p[k].v[e] : acc[e];
+        }
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < kFewPositions / kWave; ++k)
+        while (same[k]) {
+            if (__popcll(same[k]) <= 2)
+                add(std::integral_constant<int, 2>{}, same[k], k * kWave);
+            else
+                add(std::integral_constant<int, 16>{}, same[k], k * kWave);
+        }
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+        Piece<float> out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out.v[e] = acc[4 * h + e] * scale;
+        out.store(dtable + (uint64_t)key * cols + c + 4 * h, left - 4 * h);
+    }
+}
+
 // Lanes of a row.
 uint32_t sum_lanes(uint32_t cols, int v) {
     const uint32_t pieces = ceil_div(cols, v);
@@ -372,14 +469,31 @@ int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const in
     TATARA_REQUIRE(workspace && workspace_bytes >= p.bytes, "workspace too small");
     TATARA_REQUIRE_ALIGNED(workspace, 16);
     if (int32_t st = check_stream(stream)) return st;
+    // of a small table few rows a workgroup, which clears them at one CU's rate
+    const uint32_t clear_rows = std::max(4u, std::min(kClearRows, vocab / 1024));
+    const uint32_t clear = std::min(ceil_div(vocab, clear_rows), 1u << 20);
+    if (positions <= kFewPositions) {
+        TATARA_FOR_DTYPE(dtype, {
+            const uint32_t slabs = ceil_div(cols, kWave * Piece<T>::V);
+            const uint32_t blocks = clear + ceil_div(positions * slabs, kThreads / kWave);
+            auto launch = [&](auto few) {
+                embedding_few_kernel<T, decltype(few)::value><<<blocks, kThreads, 0, raw(stream)>>>(
+                    static_cast<const T*>(dy), dy_stride, token, (uint32_t)positions, vocab, cols, scale, dtable,
+                    clear, clear_rows, slabs);
+            };
+            cols < (uint32_t)Piece<T>::V ? launch(std::true_type{}) : launch(std::false_type{});
+        });
+        TATARA_LAUNCHED("embedding_few");
+        return kOk;
+    }
     char* base = static_cast<char*>(workspace);
     Place* list[2];
     for (int i = 0; i < 2; ++i)
         list[i] = reinterpret_cast<Place*>(base + p.list + i * whole_lines(sizeof(Place) * positions));
     float* partial = reinterpret_cast<float*>(base + p.partial);
     const uint32_t mask = p.passes == 1 ? ~0u : p.keys - 1;
-    const SortShape shape = sort_shape(std::max<uint64_t>(positions, 1), p.keys);
-    if (positions && shape.runs == 1) {
+    const SortShape shape = sort_shape(positions, p.keys);
+    if (shape.runs == 1) {
         with_bits(p.keys, [&](auto bits) {
             embedding_sort_kernel<decltype(bits)::value><<<1, kSortThreads, sort_lds(p.keys), raw(stream)>>>(
                 token, (uint32_t)positions, shape.run, vocab, p.passes, p.bits, p.keys, mask, list[0], list[1]);
@@ -391,9 +505,6 @@ int32_t tatara_op_embedding_backward(const void* dy, int64_t dy_stride, const in
                                      reinterpret_cast<uint32_t*>(base + p.counts), raw(stream)))
             return st;
     const Sorted s{list[(p.passes - 1) % 2], (uint32_t)positions, p.chunk, p.chunks};
-    // of a small table few rows a workgroup, which clears them at one CU's rate
-    const uint32_t clear_rows = std::max(4u, std::min(kClearRows, vocab / 1024));
-    const uint32_t clear = std::min(ceil_div(vocab, clear_rows), 1u << 20);
     TATARA_FOR_DTYPE(dtype, {
         constexpr int V = Piece<T>::V;
         const uint32_t lanes = sum_lanes(cols, V), slabs = ceil_div(cols, lanes * V);

@@ -14,8 +14,8 @@
 // written once: bound by memory, 65536 x 1536 bf16 with a residual and its sum 144 us
 // (5.6 TB/s; a copy of 400 MB runs at 5.4).  In 8 bits also by instructions, 140 a lane of
 // eight values: 16381 x 2048 f16 with scales of 128 columns 21 to 23 us (100 MB; a plain cast
-// 21.8).  A row alone takes 3 us, the backward pass of 1009 x 769 f32 5.9 and 3.2 in two
-// launches.
+// 21.8).  A row alone takes 3 us, the backward pass of 1009 x 769 f32 7.8 (2049 x 769
+// in two launches 8.6).
 #include "norm_rows.hpp"
 
 namespace tatara {
@@ -24,6 +24,15 @@ namespace {
 // Workgroups of an output in 8 bits at most: four rows each of 16384, so that the weight is
 // loaded once for them (16381 x 2048 f16: 23.0 us, with one row each 25.0, with 2048 23.4).
 constexpr uint32_t kBits8Blocks = 4096;
+
+// Whether the weight's gradient is made beside dx by workgroups of its own, which read dy and
+// the sum again, instead of from the others' partial sums by a second launch: up to 1024 rows
+// of 4 MB, an XCD's L2 (in a graph 100 x 769 f32 2.8 us, by two launches 6.4; 1009 x 769 7.8 and
+// 7.4, but 9.5 and 11.4 where the host makes the launches; 1009 x 1536 10.4 and 8.7).
+bool weight_beside(uint64_t rows, uint64_t row_bytes) { return rows <= 1024 && rows * row_bytes <= 4u << 20; }
+
+// Lanes on a row for it.
+constexpr uint32_t kWeightLanes = 4;
 
 // The larger; NaN if either is.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -264,14 +273,80 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_forward_kernel(
     }
 }
 
-// dx may be dtotal, as total above.
+// dw of a few columns over all rows, by a workgroup: four lanes with a piece each and a
+// group of rows for each four of them, joined in order.  Of few rows this needs no second
+// launch, since rstd is known.
+template <typename T, int THREADS, bool FEW>
+__device__ __forceinline__ void weight_columns(const T* __restrict__ dy, int64_t dy_stride,
+                                               const T* __restrict__ total, int64_t total_stride,
+                                               const float* __restrict__ rstd, float* __restrict__ dweight,
+                                               uint32_t rows, uint32_t cols, uint32_t block) {
+    constexpr int V = Piece<T>::V, WAVES = THREADS / kWave;
+    __shared__ float join[WAVES][kWeightLanes * V];
+    const uint32_t lane = threadIdx.x % kWeightLanes;
+    const int c = (int)((block * kWeightLanes + lane) * V), left = (int)cols - c;
+    float acc[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+    constexpr uint32_t GROUPS = THREADS / kWeightLanes;
+    constexpr int HAND = 8;  // rows that a lane reads at once
+    for (uint32_t row0 = threadIdx.x / kWeightLanes; row0 < rows; row0 += GROUPS * HAND) {
+        Piece<T> s[HAND], d[HAND];
+        float r[HAND];
+#pragma unroll
+        for (int k = 0; k < HAND; ++k) {
+            const uint32_t row = row0 + k * GROUPS < rows ? row0 + k * GROUPS : row0;
+            const T *sr = total + (int64_t)row * total_stride, *dr = dy + (int64_t)row * dy_stride;
+            if (FEW) {
+                s[k].load_few(sr, left);
+                d[k].load_few(dr, left);
+            } else {
+                s[k].load(sr, min(c, (int)cols), (int)cols);
+                d[k].load(dr, min(c, (int)cols), (int)cols);
+            }
+            r[k] = rstd[row];
+        }
+#pragma unroll
+        for (int k = 0; k < HAND; ++k) {
+            if (row0 + k * GROUPS >= rows) break;
+            if (!FEW) {
+                s[k].fix(left);
+                d[k].fix(left);
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[j] = fmaf((float)d[k].v[j], (float)s[k].v[j] * r[k], acc[j]);
+        }
+    }
+    const uint32_t wave = threadIdx.x / kWave;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float sum = column_join<(int)kWeightLanes>(acc[j], [](float x, float y) { return x + y; });
+        if (threadIdx.x % kWave < kWeightLanes) join[wave][lane * V + j] = sum;
+    }
+    __syncthreads();
+    const uint32_t mine = threadIdx.x, at = block * kWeightLanes * V + mine;
+    if (mine >= kWeightLanes * V || at >= cols) return;
+    float sum = join[0][mine];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) sum += join[w][mine];
+    dweight[at] = sum;
+}
+
+// dx may be dtotal, as total above.  With a partial, every workgroup leaves its sums of dw
+// there; with a dweight, the workgroups from `dx_blocks` on make it.
 template <typename T, int W, int L, int N, bool FEW, bool ADD>
 __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_backward_kernel(
     const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ total, int64_t total_stride,
     const float* __restrict__ weight, const float* __restrict__ rstd, const T* dtotal, int64_t dtotal_stride, T* dx,
-    int64_t dx_stride, float* __restrict__ partial, uint64_t rows, uint32_t cols) {
+    int64_t dx_stride, float* __restrict__ partial, float* __restrict__ dweight, uint32_t dx_blocks, uint64_t rows,
+    uint32_t cols) {
     constexpr int V = Piece<T>::V;
     constexpr int G = W == 1 ? 256 / L : 1;  // rows that the workgroup has in hand
+    if (blockIdx.x >= dx_blocks) {
+        weight_columns<T, W == 16 ? 1024 : 256, FEW>(dy, dy_stride, total, total_stride, rstd, dweight, (uint32_t)rows,
+                                                     cols, blockIdx.x - dx_blocks);
+        return;
+    }
     __shared__ float part[2][W];
     __shared__ float join[W > 1 ? 1 : 3 * kWave * N * V];
     const uint32_t lane = threadIdx.x % (L * W);
@@ -325,7 +400,7 @@ __global__ __launch_bounds__(W == 16 ? 1024 : 256) void rms_backward_kernel(
         r = rstd[row];
     };
     int slot = 0;
-    const uint64_t step = (uint64_t)gridDim.x * G;
+    const uint64_t step = (uint64_t)dx_blocks * G;
     uint64_t row = (uint64_t)blockIdx.x * G + group;
     if (!LEAN && row < rows) read_row(row);
     for (; row < rows; row += step, slot ^= 1) {
@@ -561,7 +636,8 @@ int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride, const voi
         TATARA_REQUIRE_ALIGNED(dx, elem_bytes(dtype));
     }
     if (int32_t st = check_stream(stream)) return st;
-    float* partial = dweight ? static_cast<float*>(workspace) : nullptr;
+    const bool beside = dweight && rows && weight_beside(rows, (uint64_t)cols * elem_bytes(dtype));
+    float* partial = dweight && !beside ? static_cast<float*>(workspace) : nullptr;
     uint32_t blocks = 0;
     if (rows) {
         TATARA_FOR_DTYPE(dtype, {
@@ -569,22 +645,22 @@ int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride, const voi
                 constexpr int W = decltype(w)::value, L = decltype(l)::value, G = W == 1 ? 256 / L : 1;
                 constexpr int N = decltype(n)::value;
                 constexpr bool FEW = decltype(few)::value;
-                blocks = grad_blocks((rows + G - 1) / G);
-                const uint32_t threads = W == 16 ? 1024 : 256;
-                if (dtotal)
-                    rms_backward_kernel<T, W, L, N, FEW, true><<<blocks, threads, 0, raw(stream)>>>(
-                        static_cast<const T*>(dy), dy_stride, static_cast<const T*>(total), total_stride, weight, rstd,
-                        static_cast<const T*>(dtotal), dtotal_stride, static_cast<T*>(dx), dx_stride, partial, rows,
-                        cols);
-                else
-                    rms_backward_kernel<T, W, L, N, FEW, false><<<blocks, threads, 0, raw(stream)>>>(
-                        static_cast<const T*>(dy), dy_stride, static_cast<const T*>(total), total_stride, weight, rstd,
-                        nullptr, 0, static_cast<T*>(dx), dx_stride, partial, rows, cols);
+                const uint64_t units = (rows + G - 1) / G;
+                blocks = beside ? (uint32_t)units : grad_blocks(units);
+                const uint32_t more = beside ? ceil_div(cols, kWeightLanes * Piece<T>::V) : 0;
+                auto launch = [&](auto add) {
+                    rms_backward_kernel<T, W, L, N, FEW, decltype(add)::value>
+                        <<<blocks + more, W == 16 ? 1024 : 256, 0, raw(stream)>>>(
+                            static_cast<const T*>(dy), dy_stride, static_cast<const T*>(total), total_stride, weight,
+                            rstd, static_cast<const T*>(dtotal), dtotal_stride, static_cast<T*>(dx), dx_stride,
+                            partial, dweight, blocks, rows, cols);
+                };
+                dtotal ? launch(std::true_type{}) : launch(std::false_type{});
             });
         });
         TATARA_LAUNCHED("rms_backward");
     }
-    if (dweight) {
+    if (dweight && !beside) {
         norm_param_grad_kernel<<<ceil_div(cols, kWave), 1024, 0, raw(stream)>>>(partial, blocks, cols, cols, dweight,
                                                                                 nullptr);
         TATARA_LAUNCHED("rms_weight_grad");

@@ -13,7 +13,7 @@ EPS32 = 2.0**-24
 SHAPES = [(0, 5, 16), (1, 1, 1), (1, 73305, 64), (7, 3, 3), (9, 81, 7), (65, 9, 256), (300, 1023, 33),
           (500, 1024, 100), (3000, 1022, 770), (8192, 2, 16), (8193, 300, 30), (20000, 81, 64), (4099, 40000, 257),
           (30000, 1, 130), (50000, 2000000, 4), (2000, 9, 4100), (100000, 5, 5), (257, 81, 32768),
-          (20000, 600000, 4), (40000, 200, 128)]
+          (20000, 600000, 4), (40000, 200, 128), (128, 9, 100), (256, 5, 300), (255, 2, 16), (200, 30000, 1000)]
 
 
 def rows_of(g, rows, cols, pad, dtype):

@@ -322,7 +322,8 @@ __global__ __launch_bounds__(kThreads) void embedding_few_kernel(const T* __rest
         }
         return;
     }
-    const uint32_t unit = __builtin_amdgcn_readfirstlane((blockIdx.x - clear) * (kThreads / kWave) + threadIdx.x / kWave);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t unit = (blockIdx.x - clear) * (kThreads / kWave) + wave;
     const uint32_t i = unit / slabs, lane = threadIdx.x % kWave;
     if (i >= n) return;
     const uint32_t key = (uint32_t)token[i];

@@ -370,7 +370,8 @@ TATARA_API int32_t tatara_op_muon_step(float* weights, float* momentum, const vo
 /* Root-mean-square norm of rows of 1..32768 columns:
  *   s = x + residual (rounded to the element type; residual may be NULL: s = x),
  *   y = s * rstd * weight,  rstd = 1 / sqrt(sum(s^2) / cols + eps).
- * weight is f32 and may be NULL (1).  total takes s and may be NULL, and may be x or
+ * Squares are summed in f32: where they pass its range (values of about 1e19) rstd and
+ * with it the row's finite values become 0.  weight is f32 and may be NULL (1).  total takes s and may be NULL, and may be x or
  * residual, with the same stride; it needs a residual.  rstd, f32 per row, is what the
  * backward pass reads and may be NULL. */
 TATARA_API int32_t tatara_op_rms_norm_forward(const void* x, int64_t x_stride, const void* residual,
@@ -384,7 +385,8 @@ TATARA_API int32_t tatara_op_rms_norm_forward(const void* x, int64_t x_stride, c
  * groups = 1):
  *   scale = max(largest |y| of the group, 2^-100) / M,  q = y / scale rounded to nearest,
  * M = 448 for TATARA_E4M3 (4 bits of exponent, 3 of fraction, no infinity), 127 for
- * TATARA_I8.  A group with a y that is not finite gets the scale NaN and q 0. */
+ * TATARA_I8.  The quotient is y times a reciprocal, three roundings of f32 from y / scale:
+ * on the border of two results either may stand.  A group with a y that is not finite gets the scale NaN and q 0. */
 #define TATARA_E4M3 0
 #define TATARA_I8 1
 TATARA_API int32_t tatara_op_rms_norm_forward_8bit(const void* x, int64_t x_stride, const void* residual,
@@ -406,7 +408,7 @@ TATARA_API int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride
                                                TataraStream* stream);
 
 /* Dropout of rows of 1..2^24 columns:
- *   y = u >= round(p * 2^32) ? x / (1 - p) : 0, plus residual (may be NULL),
+ *   y = u >= min(round(p * 2^32), 2^32 - 1) ? x / (1 - p) : 0, plus residual (may be NULL),
  * u of row r and column c: word c % 4 of Philox4x32-10 at the counter (c / 4,
  * first_row + r, low and high half of the step) with seed's halves as the key, so no mask is
  * stored.  The step is `step`, plus *more_steps if that is given (device memory, read

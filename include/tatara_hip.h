@@ -371,9 +371,9 @@ TATARA_API int32_t tatara_op_muon_step(float* weights, float* momentum, const vo
  *   s = x + residual (rounded to the element type; residual may be NULL: s = x),
  *   y = s * rstd * weight,  rstd = 1 / sqrt(sum(s^2) / cols + eps).
  * Squares are summed in f32: where they pass its range (values of about 1e19) rstd and
- * with it the row's finite values become 0.  weight is f32 and may be NULL (1).  total takes s and may be NULL, and may be x or
- * residual, with the same stride; it needs a residual.  rstd, f32 per row, is what the
- * backward pass reads and may be NULL. */
+ * with it the row's finite values become 0.  weight is f32 and may be NULL (1).  total
+ * takes s and may be NULL, and may be x or residual, with the same stride; it needs a
+ * residual.  rstd, f32 per row, is what the backward pass reads and may be NULL. */
 TATARA_API int32_t tatara_op_rms_norm_forward(const void* x, int64_t x_stride, const void* residual,
                                               int64_t residual_stride, const float* weight, void* total,
                                               int64_t total_stride, void* y, int64_t y_stride, float* rstd,
@@ -386,7 +386,8 @@ TATARA_API int32_t tatara_op_rms_norm_forward(const void* x, int64_t x_stride, c
  *   scale = max(largest |y| of the group, 2^-100) / M,  q = y / scale rounded to nearest,
  * M = 448 for TATARA_E4M3 (4 bits of exponent, 3 of fraction, no infinity), 127 for
  * TATARA_I8.  The quotient is y times a reciprocal, three roundings of f32 from y / scale:
- * on the border of two results either may stand.  A group with a y that is not finite gets the scale NaN and q 0. */
+ * on the border of two results either may stand.  A group with a y that is not finite
+ * gets the scale NaN and q 0. */
 #define TATARA_E4M3 0
 #define TATARA_I8 1
 TATARA_API int32_t tatara_op_rms_norm_forward_8bit(const void* x, int64_t x_stride, const void* residual,

@@ -533,6 +533,9 @@ int32_t check_forward(const void* x, int64_t x_stride, const void* residual, int
     TATARA_REQUIRE(x_stride >= (int64_t)cols && y_stride >= (int64_t)cols &&
                        (!residual || residual_stride >= (int64_t)cols) && (!total || total_stride >= (int64_t)cols),
                    "a row stride is smaller than the row");
+    TATARA_REQUIRE(!total || ((total != x || total_stride == x_stride) &&
+                              (total != residual || total_stride == residual_stride)),
+                   "in place the strides are the same");
     TATARA_REQUIRE_ALIGNED(x, elem_bytes(dtype));
     TATARA_REQUIRE_ALIGNED(residual, elem_bytes(dtype));
     TATARA_REQUIRE_ALIGNED(total, elem_bytes(dtype));
@@ -630,6 +633,7 @@ int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride, const voi
         TATARA_REQUIRE(dy_stride >= (int64_t)cols && total_stride >= (int64_t)cols && dx_stride >= (int64_t)cols &&
                            (!dtotal || dtotal_stride >= (int64_t)cols),
                        "a row stride is smaller than the row");
+        TATARA_REQUIRE(dx != dtotal || dx_stride == dtotal_stride, "in place the strides are the same");
         TATARA_REQUIRE_ALIGNED(dy, elem_bytes(dtype));
         TATARA_REQUIRE_ALIGNED(total, elem_bytes(dtype));
         TATARA_REQUIRE_ALIGNED(dtotal, elem_bytes(dtype));

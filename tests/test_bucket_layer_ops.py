@@ -83,6 +83,9 @@ def test_rms_norm_refuses():
             refused(call(**{stride: 15}), b"stride")
         for p in ("x", "res", "total"):
             refused(call(**{p: FAKE + 2}), b"aligned")
+        refused(call(ts=17), b"in place")
+        refused(call(x=2 * FAKE, ts=17), b"in place")
+    refused(rms_back(dxs=17), b"in place")
     refused(rms(y=FAKE + 1, t=2), b"aligned")
     refused(rms8(format=2), b"format")
     refused(rms8(group=16), b"scale")

@@ -274,7 +274,7 @@ class LayerNorm(_Operator):
     def backward(self, dy, x, weight, mean, rstd, dx, dweight=None, dbias=None, stream=None) -> None:
         """Writes dx, and the weight's and bias's gradients [cols] if given (overwritten)."""
         cols, dtype = self.cols, self.dtype
-        here, queue = _place(x, stream)
+        here, queue = _place(dy, stream)
         rows = _count("x", x, cols, dtype)
         shape, vec, param = (rows, cols), (rows,), (cols,)
         dyp, dys = _rows("dy", dy, shape, dtype, here)
@@ -482,7 +482,7 @@ class RMSNorm(_Operator):
         gradient dtotal that reaches the sum by itself (dx may be dtotal), and the
         weight's gradient [cols] if given (overwritten)."""
         cols, dtype = self.cols, self.dtype
-        here, queue = _place(total, stream)
+        here, queue = _place(dy, stream)
         rows = _count("total", total, cols, dtype)
         shape = (rows, cols)
         dyp, dys = _rows("dy", dy, shape, dtype, here)
@@ -684,7 +684,7 @@ class Embedding(_Operator):
 
     def backward(self, dy, token, dtable, stream=None) -> None:
         """Writes dtable [vocab, cols] (overwritten)."""
-        here, queue = _place(token, stream)
+        here, queue = _place(dy, stream)
         n = self._tokens(token)
         if n > self.positions:
             raise ValueError(f"a backward call takes up to {self.positions} positions, not {n}")

@@ -61,6 +61,14 @@ __device__ __forceinline__ uint64_t same_key(bool in, uint32_t key) {
     return same;
 }
 
+// Between the lanes' reads of their keys' counters, the additions of the first lane of each
+// key, and the next reads: lanes read what others of the wave add to.  The wave's LDS accesses
+// are done in their order, which the compiler has to keep; no instruction.
+__device__ __forceinline__ void in_wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Exclusive sum over the workgroup's kSortThreads threads.
 __device__ __forceinline__ uint32_t sum_ahead(uint32_t x, uint32_t* part) {
     const uint32_t lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
@@ -197,8 +205,9 @@ __device__ __forceinline__ void sort_place(const Items& items, uint64_t n, uint3
                 const uint64_t below = same & ((1ull << lane) - 1);
                 uint32_t rank = 0;
                 if (in) rank = __hip_atomic_load(&my_next[key[h]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                // behind the wave's loads
+                in_wave_order();
                 if (in && below == 0) atomicAdd(&my_next[key[h]], (uint32_t)__popcll(same));
+                in_wave_order();
                 rank += (uint32_t)__popcll(below);
                 if (in)
                     items.put(i, item[h], key[h], first[key[h]], rank);

@@ -371,7 +371,9 @@ TATARA_API int32_t tatara_op_muon_step(float* weights, float* momentum, const vo
  *   s = x + residual (rounded to the element type; residual may be NULL: s = x),
  *   y = s * rstd * weight,  rstd = 1 / sqrt(sum(s^2) / cols + eps).
  * Squares are summed in f32: where they pass its range (values of about 1e19) rstd and
- * with it the row's finite values become 0.  weight is f32 and may be NULL (1).  total
+ * with it the row's finite values become 0.  Those below 2^-126 (values below about 1e-19)
+ * lose digits, and up to 2^-150 they are 0: a row of such values alone has with an eps of 0
+ * an infinite rstd, and its values become infinite, 0 becomes NaN.  weight is f32 and may be NULL (1).  total
  * takes s and may be NULL, and may be x or residual, with the same stride; it needs a
  * residual.  rstd, f32 per row, is what the backward pass reads and may be NULL. */
 TATARA_API int32_t tatara_op_rms_norm_forward(const void* x, int64_t x_stride, const void* residual,

@@ -400,8 +400,9 @@ TATARA_API int32_t tatara_op_rms_norm_forward_8bit(const void* x, int64_t x_stri
 /* With s the forward call's, h = s * rstd and g = dy * weight:
  *   dx = rstd * (g - h * sum(g * h) / cols) + dtotal,  dweight = sum over rows of dy * h.
  * dx is the gradient of x and of the residual alike.  dtotal, the gradient that reaches
- * s by itself, may be NULL; dx may be dtotal, with the same stride.  dweight (f32,
- * overwritten) may be NULL, and then no workspace is needed.  No rows: it becomes 0. */
+ * s by itself, may be NULL; dx may be dtotal, with the same stride, and neither dy nor
+ * the sum.  dweight (f32, overwritten) may be NULL, and then no workspace is needed.  No
+ * rows: it becomes 0. */
 TATARA_API int32_t tatara_op_rms_norm_backward_workspace(uint32_t cols, uint64_t* bytes);
 TATARA_API int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride, const void* total,
                                                int64_t total_stride, const float* weight, const float* rstd,

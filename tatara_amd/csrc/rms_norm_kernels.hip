@@ -638,6 +638,8 @@ int32_t tatara_op_rms_norm_backward(const void* dy, int64_t dy_stride, const voi
         TATARA_REQUIRE_ALIGNED(total, elem_bytes(dtype));
         TATARA_REQUIRE_ALIGNED(dtotal, elem_bytes(dtype));
         TATARA_REQUIRE_ALIGNED(dx, elem_bytes(dtype));
+        // the weight's workgroups may read what others have written by then
+        TATARA_REQUIRE(dx != dy && dx != total, "dx must not be dy or the sum");
     }
     if (int32_t st = check_stream(stream)) return st;
     const bool beside = dweight && rows && weight_beside(rows, (uint64_t)cols * elem_bytes(dtype));

@@ -22,7 +22,8 @@ type is "f32", "f16" or "bf16"; a DeviceArray holds bf16 as uint16 (and e4m3 as 
 their work on `stream` (a runtime.Stream or a torch.cuda.Stream; None is torch's
 current stream where the call's first tensor is torch's, else the null stream) and return;
 one operator's calls belong on one stream at a time, since they share the
-workspace.  All tensors of a call lie on the thread's current device.  The first call
+workspace.  All tensors of a call lie on the thread's current device, and what it
+writes overlaps nothing else of it unless its description says so.  The first call
 there that needs the workspace makes it, which waits for the device and cannot be
 recorded into a graph; prepare() makes it ahead.  Wrong shapes, types and devices raise
 ValueError, device errors TataraError.
@@ -479,8 +480,8 @@ class RMSNorm(_Operator):
 
     def backward(self, dy, total, weight, rstd, dx, dweight=None, dtotal=None, stream=None) -> None:
         """Writes dx, the gradient of x and residual alike, from dy and, if given, the
-        gradient dtotal that reaches the sum by itself (dx may be dtotal), and the
-        weight's gradient [cols] if given (overwritten)."""
+        gradient dtotal that reaches the sum by itself (dx may be dtotal, not dy or total),
+        and the weight's gradient [cols] if given (overwritten)."""
         cols, dtype = self.cols, self.dtype
         here, queue = _place(dy, stream)
         rows = _count("total", total, cols, dtype)

@@ -27,8 +27,12 @@ constexpr uint32_t kBits8Blocks = 4096;
 
 // Whether the weight's gradient is made beside dx by workgroups of its own, which read dy and
 // the sum again, instead of from the others' partial sums by a second launch: up to 1024 rows
-// of 4 MB, an XCD's L2 (in a graph 100 x 769 f32 2.8 us, by two launches 6.4; 1009 x 769 7.8 and
-// 7.4, but 9.5 and 11.4 where the host makes the launches; 1009 x 1536 10.4 and 8.7).
+// of 4 MB, an XCD's L2.  In a graph, with dtotal, f32 100 x 769 3.0 us and by two launches 6.5,
+// 1000 x 32 4.0 and 4.8, 1024 x 1024 6.6 and 7.8, bf16 512 x 4096 5.5 and 11.2, 1024 x 2048 7.8 and
+// 9.6; slower only in rows that start inside a line, f32 1009 x 769 8.3 and 7.6, where calls from
+// the host take 8.2 and 11.0.  Of more rows f32 1500 x 256 5.5 and 6.1, but 2048 x 32 5.8 and 5.4,
+// 2048 x 128 6.2 and 5.4, bf16 2048 x 256 7.7 and 5.8; of more bytes f32 1024 x 1536 11.4 and 9.5,
+// 512 x 4096 12.8 and 11.1.
 bool weight_beside(uint64_t rows, uint64_t row_bytes) { return rows <= 1024 && rows * row_bytes <= 4u << 20; }
 
 // Lanes on a row for it.

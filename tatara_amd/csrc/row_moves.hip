@@ -9,7 +9,9 @@
 // Bound by memory: 65536 x 1536 f32 gathered 146 us (805 MB, 5.5 TB/s), 32768 x 768 f16 with
 // two choices back with the gates' gradient 49 (252 MB, 5.1), 65536 x 768 bf16 of a table of
 // 1629 rows 22.4 (writes at 4.5; the table comes from the last-level cache as often as the
-// rows written push it out of the L2).  More positions in hand a lane are no faster.
+// rows written push it out of the L2).  More positions in hand a lane are no faster.  Five to
+// sixteen choices share one form (16381 x 512 bf16 back: four 16.3 us, five 42.0, eight 47.0,
+// sixteen 64.9, of which bytes take 17, 20, 30 and 57; 8192 x 1536 f32, eight 94 and 91).
 #include "row_moves.hpp"
 
 namespace tatara {
